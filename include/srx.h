@@ -37,8 +37,8 @@ int srx_version(void);
 const char* srx_last_error(void);
 /* sizeof() of the ABI structs, for binding self-checks: 0 srx_conv_desc, 1 srx_wgrad_task,
  * 2 srx_wgrad_desc, 3 srx_pack_seg, 4 srx_pack_layer, 5 srx_unpack_item, 6 srx_sn_layer,
- * 7 srx_sn_bwd_layer, 8 srx_generic_args, 9 srx_op, 10 srx_tile, 11 srx_crop, 12 srx_rdb_desc; -1 for an
- * unknown id. */
+ * 7 srx_sn_bwd_layer, 8 srx_generic_args, 9 srx_op, 10 srx_tile, 11 srx_crop, 12 srx_rdb_desc,
+ * 13 srx_adamw_tensor, 14 srx_adamw_chunk, 15 srx_adamw_group, 16 srx_adamw_desc; -1 for an unknown id. */
 int srx_sizeof(int which);
 /* Host-side self-check (no GPU call): kernel attributes such as the dynamic LDS limit are set
  * once per DEVICE a kernel is launched on, not once per process.  0 = ok.  No counterpart in the
@@ -351,6 +351,73 @@ int srx_pack_weights_flat(int dtype, const srx_pack_layer* layers, const srx_pac
  * fp32 parameter range: p,g,m,v of n elements; bias corrections from step. */
 int srx_adam(float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
              float beta2, float eps, float weight_decay, int step, float gscale, void* stream);
+
+/* One AdamW step (decoupled weight decay) over many tensors, in a handful of launches.  The reference trains with
+ * optim.Adam over every parameter tensor (esrgan/train_esrgan.py:134-135); this is the step for what that one
+ * does not cover: parameters that are not one flat fp32 range, weight decay for some tensors only, gradient clipping,
+ * bf16 parameters with fp32 masters, moments in 8 bits.  Per element, with t the tensor's own step count:
+ *     g  = grad * factor
+ *     m  = beta1 m + (1 - beta1) g            v = beta2 v + (1 - beta2) g^2
+ *     p  = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * factor = grad_scale * min(1, max_norm / (norm + 1e-6)) where max_norm > 0, else grad_scale;
+ * norm = |grad_scale| * sqrt(sum of grad^2 over all tensors), summed in 64 bits in a fixed order (same inputs, same
+ * bits), computed only where max_norm > 0 or skip_nonfinite is set, and written to norm[0].  With skip_nonfinite a
+ * step whose norm is not finite changes nothing, not even the step counts.  Everything is decided on the device.
+ *
+ * state_bits 32: m, v are fp32 [256 * blocks].  8: m, v are one byte an element, with one fp32 scale for each 256
+ * elements of a tensor: scale = the largest magnitude in the block, and each value's ratio to it is rounded to
+ * nearest (ties to even) to a float with 3 mantissa bits, m with its sign down to 1.25 * 2^-16 (below: 0), v down to
+ * 1.25 * 2^-32 (below: that value).  The step itself uses the new moments before they are rounded.  A value that is
+ * not finite makes the moments of its whole block NaN. */
+#define SRX_ADAMW_BLOCK 256
+#define SRX_ADAMW_CHUNK 4096
+#define SRX_ADAMW_MAX_GROUPS 32
+typedef struct srx_adamw_tensor {
+  void* p;               /* parameter, contiguous: fp32, or bf16 with `master`                    */
+  float* master;         /* fp32 copy of a bf16 parameter (NULL for an fp32 one).  Where the parameter is
+                            not the master rounded to bf16, somebody has written the parameter since, and it
+                            replaces the master                                                    */
+  int64_t n;             /* elements                                                              */
+  int64_t first_block;   /* its moments start at element 256 * first_block                        */
+  int64_t g_off;         /* its gradient's first element in flat_grad                             */
+  int32_t group;
+  int32_t pad_;
+} srx_adamw_tensor;
+typedef struct srx_adamw_chunk {    /* elements [4096 index, 4096 (index + 1)) of a tensor        */
+  int32_t tensor, index;
+} srx_adamw_chunk;
+typedef struct srx_adamw_group {
+  double lr, beta1, beta2, eps, weight_decay;
+} srx_adamw_group;
+typedef struct srx_adamw_desc {
+  int32_t state_bits;    /* 32 or 8                                                               */
+  int32_t ntensors, ngroups;
+  int32_t skip_nonfinite;
+  const srx_adamw_tensor* tensors;    /* DEVICE [ntensors]                                        */
+  const srx_adamw_chunk* chunks;      /* DEVICE, the chunks of tensor 0, then of tensor 1, ...    */
+  const int32_t* chunk_start;         /* HOST [ntensors + 1]: where each tensor's chunks start    */
+  const srx_adamw_group* groups;      /* HOST [ngroups]                                           */
+  const void* const* grads;           /* HOST [ntensors] device addresses (NULL: that tensor and its step count
+                                         stay as they are), or NULL with flat_grad                */
+  const uint8_t* grad_dtypes;         /* HOST [ntensors] SRX_F32 / SRX_BF16; NULL: all fp32       */
+  const void* flat_grad;              /* all gradients in one buffer (srx_adamw_tensor.g_off)     */
+  int32_t flat_dtype;
+  int32_t pad_;
+  void* m; void* v;                   /* moments, 16-byte aligned                                 */
+  float* m_scale; float* v_scale;     /* 8 bits: one scale for each block                         */
+  int32_t* steps;                     /* DEVICE [ntensors] step counts, advanced by the call      */
+  float* coef;                        /* DEVICE workspace, 4 + 8 * ntensors floats                */
+  double* partial;                    /* DEVICE workspace, one per chunk (norm only)              */
+  float* norm;                        /* DEVICE result (norm only)                                */
+  double grad_scale, max_norm;
+} srx_adamw_desc;
+int srx_adamw_step(const srx_adamw_desc* d, void* stream);
+/* fp32 moments of whole blocks of 256 to their 8-bit form and back (checkpoints hold fp32 moments; what was 8 bits
+ * comes back as the same 8 bits).  All four moment buffers 16-byte aligned. */
+int srx_adamw_moments_to8(const float* m, const float* v, void* m_code, void* v_code, float* m_scale, float* v_scale,
+                          int64_t nblocks, void* stream);
+int srx_adamw_moments_from8(const void* m_code, const void* v_code, const float* m_scale, const float* v_scale,
+                            float* m, float* v, int64_t nblocks, void* stream);
 
 /* -------------------------------------------------------- tiled inference */
 /* Tiling around the generator, reference inference.py:187-230 (_infer_tiled).

@@ -25,7 +25,9 @@ OP_ACT_BWD = 12
 OP_RDB_FWD = 13
 OP_RDB_BWD = 14
 
-vp, i32, i64, f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+vp, i32, i64, f32, f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_double
+
+ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_GROUPS = 256, 4096, 32
 
 
 class PackSeg(C.Structure):
@@ -102,6 +104,26 @@ class RdbDesc(C.Structure):
                 ("res2", vp), ("res2_img_stride", i64), ("act", vp), ("act_img_stride", i64)]
 
 
+class AdamwTensor(C.Structure):
+    _fields_ = [("p", vp), ("master", vp), ("n", i64), ("first_block", i64), ("g_off", i64), ("group", i32), ("pad_", i32)]
+
+
+class AdamwChunk(C.Structure):
+    _fields_ = [("tensor", i32), ("index", i32)]
+
+
+class AdamwGroup(C.Structure):
+    _fields_ = [("lr", f64), ("beta1", f64), ("beta2", f64), ("eps", f64), ("weight_decay", f64)]
+
+
+class AdamwDesc(C.Structure):
+    _fields_ = [("state_bits", i32), ("ntensors", i32), ("ngroups", i32), ("skip_nonfinite", i32),
+                ("tensors", vp), ("chunks", vp), ("chunk_start", vp), ("groups", vp), ("grads", vp),
+                ("grad_dtypes", vp), ("flat_grad", vp), ("flat_dtype", i32), ("pad_", i32),
+                ("m", vp), ("v", vp), ("m_scale", vp), ("v_scale", vp), ("steps", vp), ("coef", vp),
+                ("partial", vp), ("norm", vp), ("grad_scale", f64), ("max_norm", f64)]
+
+
 class _OpU(C.Union):
     _fields_ = [("conv", ConvDesc), ("wgrad", WgradDesc), ("g", GenericArgs), ("rdb", RdbDesc)]
 
@@ -146,6 +168,9 @@ _SIGS = {
     "srx_sn_scratch_floats": (C.c_int, []),
     "srx_sn_backward": (C.c_int, [vp, C.c_int, C.c_int, C.c_int, vp]),
     "srx_adam": (C.c_int, [vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, C.c_int, f32, vp]),
+    "srx_adamw_step": (C.c_int, [C.POINTER(AdamwDesc), vp]),
+    "srx_adamw_moments_to8": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, vp]),
+    "srx_adamw_moments_from8": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, vp]),
     "srx_run_ops": (C.c_int, [vp, C.c_int, vp]),
     "srx_stream_create": (C.c_int, [C.c_int, C.POINTER(vp)]),
     "srx_stream_destroy": (C.c_int, [vp]),
@@ -174,7 +199,8 @@ def lib():
             fn.restype = res
             fn.argtypes = args
         structs = (ConvDesc, WgradTask, WgradDesc, PackSeg, PackLayer, UnpackItem, SnLayer,
-                   SnBwdLayer, GenericArgs, Op, Tile, Crop, RdbDesc)
+                   SnBwdLayer, GenericArgs, Op, Tile, Crop, RdbDesc,
+                   AdamwTensor, AdamwChunk, AdamwGroup, AdamwDesc)
         for i, st in enumerate(structs):
             if l.srx_sizeof(i) != C.sizeof(st):
                 raise RuntimeError(f"libsrx ABI mismatch: sizeof({st.__name__}) is {C.sizeof(st)} in "

@@ -35,6 +35,10 @@ int srx_sizeof(int which) {
     case 10: return (int)sizeof(srx_tile);
     case 11: return (int)sizeof(srx_crop);
     case 12: return (int)sizeof(srx_rdb_desc);
+    case 13: return (int)sizeof(srx_adamw_tensor);
+    case 14: return (int)sizeof(srx_adamw_chunk);
+    case 15: return (int)sizeof(srx_adamw_group);
+    case 16: return (int)sizeof(srx_adamw_desc);
     default: return -1;
   }
 }

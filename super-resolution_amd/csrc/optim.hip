@@ -1,0 +1,440 @@
+// AdamW over many tensors at once, moments in 32 or 8 bits, with the global gradient norm, clipping and the skip of a
+// step whose gradients are not finite.  See include/srx.h (srx_adamw_step) for the formulas and the buffers.
+//
+// Launches of one step: [norm pass over the gradients, 448 tensors a launch] + one "prepare" workgroup (finishes the
+// norm, advances the step counts, computes each tensor's bias-corrected constants) + the update, 448 tensors a launch.
+// The gradients' addresses travel in the kernel arguments: they change from step to step (autograd allocates new
+// gradients), and a table in device memory would need a host-to-device copy that a captured graph could not repeat.
+#include "srx_common.h"
+
+namespace {
+
+constexpr int BLOCK = SRX_ADAMW_BLOCK;          // elements that share one scale in the 8-bit moments
+constexpr int CHUNK = SRX_ADAMW_CHUNK;          // elements of one tensor that one workgroup updates
+constexpr int TPB = 256;
+constexpr int MAX_GRADS = 448;                  // addresses per launch: 3.6 KB of the 4 KB of kernel arguments
+constexpr int PREP_TENSORS = 16384;             // tensors per prepare launch: one bit each, 2 KB of kernel arguments
+constexpr int PREP_TPB = 1024;
+
+// The top 12 bits of a float are its exponent and three mantissa bits; 1.0 has 1016 there.  Code c > 0 stands for the
+// float with base + c there: 127 signed codes reach from 1 down to 1.25 * 2^-16, 255 unsigned ones to 1.25 * 2^-32.
+constexpr unsigned M_BASE = 889, V_BASE = 761;
+
+struct Ctl { float factor; int skip; float pad[2]; };            // first 16 bytes of the coefficient workspace
+struct Coef { float decay, step_size, root, eps, b1, ob1, b2, ob2; };
+
+struct PrepArgs {
+  const srx_adamw_tensor* tensors;
+  int32_t* steps;
+  float* coef;
+  const double* partial;
+  float* norm;
+  double grad_scale, max_norm;
+  int ntensors, t0, nchunks;
+  int norm_mode;             // 0 none, 1 finish the norm here, 2 already finished by an earlier launch
+  int skip_nonfinite;
+  srx_adamw_group groups[SRX_ADAMW_MAX_GROUPS];
+  uint32_t has_grad[PREP_TENSORS / 32];
+};
+
+template <int NG> struct StepArgs {
+  const srx_adamw_tensor* tensors;
+  const srx_adamw_chunk* chunks;
+  const float* coef;
+  double* partial;
+  void* m; void* v;
+  float* m_scale; float* v_scale;
+  const void* flat;          // NG == 1: the flat gradient
+  int chunk0, t0;
+  int norm_mode;
+  int flat_dtype;
+  uint64_t is_bf16[(NG + 63) / 64];
+  const void* g[NG];
+};
+
+struct Grad { const void* p; bool bf; };
+template <int NG> __device__ __forceinline__ Grad grad_of(const StepArgs<NG>& a, const srx_adamw_tensor& t, int ti) {
+  Grad r;
+  if constexpr (NG == 1) {
+    r.bf = a.flat_dtype == SRX_BF16;
+    r.p = static_cast<const char*>(a.flat) + t.g_off * (r.bf ? 2 : 4);
+  } else {
+    const int k = ti - a.t0;
+    r.p = a.g[k];
+    r.bf = (a.is_bf16[k >> 6] >> (k & 63)) & 1;
+  }
+  return r;
+}
+__device__ __forceinline__ float grad_at(const Grad& g, int64_t i) {
+  return g.bf ? (float)static_cast<const bf16*>(g.p)[i] : static_cast<const float*>(g.p)[i];
+}
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// Non-negative floats order like their bits, and a NaN's bits are above every number's: one NaN or infinity in a
+// block makes its scale, and with it the whole block, NaN, as it would make the 32-bit moments it touches.
+__device__ __forceinline__ unsigned wave_max_u(unsigned v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const unsigned w = (unsigned)__shfl_xor((int)v, o, 64);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+__device__ __forceinline__ float decode(unsigned k, unsigned base) { return k ? __uint_as_float((k + base) << 20) : 0.f; }
+// |x| / s in [0, 1] -> nearest code (ties to even); below code 1: `least` (0 stays 0).  The second moment takes least = 1:
+// a moment rounded down to 0 would leave only eps in the denominator of its update.
+__device__ __forceinline__ unsigned encode(float t, unsigned base, unsigned least) {
+  if (!(t > 0.f)) return 0;
+  const unsigned b = __float_as_uint(t);
+  const int c = (int)((b + 0x7FFFFu + ((b >> 20) & 1u)) >> 20) - (int)base;
+  return c < (int)least ? least : (unsigned)c;
+}
+
+// a first moment that rounds to 0 loses its sign: one code for each value
+__device__ __forceinline__ unsigned encode_signed(float x, float s) {
+  const unsigned c = encode(fabsf(x) / s, M_BASE, 0);
+  return c && x < 0 ? c | 128u : c;
+}
+
+// sum of squares of one chunk of gradients, in 64 bits (a square can leave 32 bits' range, and the sum runs over
+// millions of terms); a fixed order, so the norm is the same every time
+template <int NG> __global__ __launch_bounds__(TPB) void adamw_norm_kernel(const StepArgs<NG> a) {
+  const int c = a.chunk0 + blockIdx.x;
+  const srx_adamw_chunk ch = a.chunks[c];
+  const srx_adamw_tensor t = a.tensors[ch.tensor];
+  const Grad g = grad_of<NG>(a, t, ch.tensor);
+  double s = 0;
+  if (g.p) {
+    const int64_t lo = (int64_t)ch.index * CHUNK;
+    const int64_t hi = lo + CHUNK < t.n ? lo + CHUNK : t.n;
+    for (int64_t i = lo + threadIdx.x; i < hi; i += TPB) {
+      const double x = grad_at(g, i);
+      s += x * x;
+    }
+  }
+  __shared__ double part[TPB / 64];
+  s = wave_sum_d(s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) a.partial[c] = part[0] + part[1] + part[2] + part[3];
+}
+
+__device__ double int_pow(double b, int n) {
+  double r = 1;
+  for (; n > 0; n >>= 1, b *= b)
+    if (n & 1) r *= b;
+  return r;
+}
+
+__global__ __launch_bounds__(PREP_TPB) void adamw_prepare_kernel(const PrepArgs a) {
+  Ctl* ctl = reinterpret_cast<Ctl*>(a.coef);
+  Coef* coef = reinterpret_cast<Coef*>(a.coef + 4);
+  __shared__ double part[PREP_TPB / 64];
+  __shared__ int skip_s;
+  int skip = 0;
+  if (a.norm_mode == 1) {
+    double s = 0;
+    for (int i = threadIdx.x; i < a.nchunks; i += PREP_TPB) s += a.partial[i];
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double total = 0;
+      for (int i = 0; i < PREP_TPB / 64; ++i) total += part[i];
+      total = sqrt(total) * fabs(a.grad_scale);
+      double c = 1;
+      if (a.max_norm > 0) {
+        c = a.max_norm / (total + 1e-6);
+        c = c > 1 ? 1 : c;                       // a NaN norm stays NaN and reaches every parameter, as in torch
+      }
+      const bool finite = total - total == 0;
+      skip_s = a.skip_nonfinite && !finite;
+      ctl->factor = (float)(a.grad_scale * c);
+      ctl->skip = skip_s;
+      a.norm[0] = (float)total;
+    }
+    __syncthreads();
+    skip = skip_s;
+  } else if (a.norm_mode == 2) {
+    skip = ctl->skip;
+  } else if (threadIdx.x == 0) {
+    ctl->factor = (float)a.grad_scale;
+    ctl->skip = 0;
+  }
+  if (skip) return;
+  for (int k = threadIdx.x; k < PREP_TENSORS && a.t0 + k < a.ntensors; k += PREP_TPB) {
+    if (!((a.has_grad[k >> 5] >> (k & 31)) & 1)) continue;
+    const int i = a.t0 + k;
+    const int step = a.steps[i] + 1;
+    a.steps[i] = step;
+    const srx_adamw_group& g = a.groups[a.tensors[i].group];
+    Coef r;
+    r.decay = (float)(1 - g.lr * g.weight_decay);
+    r.step_size = (float)(g.lr / (1 - int_pow(g.beta1, step)));
+    r.root = (float)(1 / sqrt(1 - int_pow(g.beta2, step)));
+    r.eps = (float)g.eps;
+    r.b1 = (float)g.beta1;
+    r.ob1 = (float)(1 - g.beta1);
+    r.b2 = (float)g.beta2;
+    r.ob2 = (float)(1 - g.beta2);
+    coef[i] = r;
+  }
+}
+
+// The moments' new values, each operation rounded on its own: the 8-bit codes are then the same whatever code computes
+// them (a fused multiply-add would move one value in ten million to the neighbouring code, a tenth away).
+__device__ __forceinline__ void moments(float& m, float& v, float g, const Coef& c) {
+#pragma clang fp contract(off)
+  const float mg = g * c.ob1, gg = g * g;
+  m = m * c.b1;
+  m = m + mg;
+  const float vg = gg * c.ob2;
+  v = v * c.b2;
+  v = v + vg;
+}
+__device__ __forceinline__ float updated(float w, float m, float v, const Coef& c) {
+  return w * c.decay - c.step_size * (m / (sqrtf(v) * c.root + c.eps));
+}
+
+template <int BITS, int NG> __global__ __launch_bounds__(TPB) void adamw_step_kernel(const StepArgs<NG> a) {
+  const Ctl* ctl = reinterpret_cast<const Ctl*>(a.coef);
+  if (ctl->skip) return;
+  const srx_adamw_chunk ch = a.chunks[a.chunk0 + blockIdx.x];
+  const srx_adamw_tensor t = a.tensors[ch.tensor];
+  const Grad g = grad_of<NG>(a, t, ch.tensor);
+  if (!g.p) return;
+  const Coef c = reinterpret_cast<const Coef*>(a.coef + 4)[ch.tensor];
+  const float factor = ctl->factor;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int b = wave; b < CHUNK / BLOCK; b += TPB / 64) {
+    const int64_t lo = (int64_t)ch.index * CHUNK + b * BLOCK;      // first element of the block in its tensor
+    if (lo >= t.n) break;
+    const int64_t blk = t.first_block + lo / BLOCK;
+    float m[4], v[4];
+    float ms = 0, vs = 0;
+    if constexpr (BITS == 8) { ms = a.m_scale[blk]; vs = a.v_scale[blk]; }
+    unsigned mmax = 0, vmax = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = lane + 64 * j;
+      const int64_t i = lo + e, s = blk * BLOCK + e;
+      m[j] = v[j] = 0;
+      if (i >= t.n) continue;
+      if constexpr (BITS == 8) {
+        const unsigned mc = static_cast<const uint8_t*>(a.m)[s], vc = static_cast<const uint8_t*>(a.v)[s];
+        m[j] = decode(mc & 127, M_BASE) * ms;
+        if (mc & 128) m[j] = -m[j];
+        v[j] = decode(vc, V_BASE) * vs;
+      } else {
+        m[j] = static_cast<const float*>(a.m)[s];
+        v[j] = static_cast<const float*>(a.v)[s];
+      }
+      float gi;
+      {
+#pragma clang fp contract(off)
+        gi = grad_at(g, i) * factor;
+      }
+      moments(m[j], v[j], gi, c);
+      if (t.master) {
+        // the parameter is what the user sees and may have written: where it is not the master's rounding, it wins
+        bf16* p = static_cast<bf16*>(t.p) + i;
+        const float w0 = t.master[i];
+        const float w = updated((float)(bf16)w0 == (float)*p ? w0 : (float)*p, m[j], v[j], c);
+        t.master[i] = w;
+        *p = (bf16)w;
+      } else {
+        float* p = static_cast<float*>(t.p) + i;
+        *p = updated(*p, m[j], v[j], c);
+      }
+      if constexpr (BITS == 32) {
+        static_cast<float*>(a.m)[s] = m[j];
+        static_cast<float*>(a.v)[s] = v[j];
+      } else {
+        const unsigned mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+        mmax = mb > mmax ? mb : mmax;
+        vmax = vb > vmax ? vb : vmax;
+      }
+    }
+    if constexpr (BITS == 8) {
+      ms = __uint_as_float(wave_max_u(mmax));
+      vs = __uint_as_float(wave_max_u(vmax));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = lane + 64 * j;
+        if (lo + e >= t.n) continue;
+        const int64_t s = blk * BLOCK + e;
+        static_cast<uint8_t*>(a.m)[s] = (uint8_t)encode_signed(m[j], ms);
+        static_cast<uint8_t*>(a.v)[s] = (uint8_t)encode(v[j] / vs, V_BASE, 1);
+      }
+      if (lane == 0) { a.m_scale[blk] = ms; a.v_scale[blk] = vs; }
+    }
+  }
+}
+
+// one wave per block of 256
+__global__ __launch_bounds__(TPB) void moments_to8_kernel(const float* m, const float* v, uint8_t* mc, uint8_t* vc, float* ms,
+                                                          float* vs, int64_t nblocks) {
+  const int64_t blk = (int64_t)blockIdx.x * (TPB / 64) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (blk >= nblocks) return;
+  const int64_t s = blk * BLOCK + lane * 4;
+  const f32x4 a = *reinterpret_cast<const f32x4*>(m + s), b = *reinterpret_cast<const f32x4*>(v + s);
+  unsigned am = 0, bm = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned x = __float_as_uint(a[j]) & 0x7FFFFFFFu, y = __float_as_uint(b[j]) & 0x7FFFFFFFu;
+    am = x > am ? x : am;
+    bm = y > bm ? y : bm;
+  }
+  const float sm = __uint_as_float(wave_max_u(am)), sv = __uint_as_float(wave_max_u(bm));
+  uint32_t cm = 0, cv = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    cm |= encode_signed(a[j], sm) << (8 * j);
+    cv |= encode(b[j] / sv, V_BASE, 1) << (8 * j);
+  }
+  *reinterpret_cast<uint32_t*>(mc + s) = cm;
+  *reinterpret_cast<uint32_t*>(vc + s) = cv;
+  if (lane == 0) { ms[blk] = sm; vs[blk] = sv; }
+}
+
+__global__ __launch_bounds__(TPB) void moments_from8_kernel(const uint8_t* mc, const uint8_t* vc, const float* ms, const float* vs,
+                                                            float* m, float* v, int64_t nblocks) {
+  const int64_t blk = (int64_t)blockIdx.x * (TPB / 64) + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (blk >= nblocks) return;
+  const int64_t s = blk * BLOCK + lane * 4;
+  const uint32_t cm = *reinterpret_cast<const uint32_t*>(mc + s), cv = *reinterpret_cast<const uint32_t*>(vc + s);
+  const float sm = ms[blk], sv = vs[blk];
+  f32x4 a, b;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned x = (cm >> (8 * j)) & 255, y = (cv >> (8 * j)) & 255;
+    const float z = decode(x & 127, M_BASE) * sm;
+    a[j] = x & 128 ? -z : z;
+    b[j] = decode(y, V_BASE) * sv;
+  }
+  *reinterpret_cast<f32x4*>(m + s) = a;
+  *reinterpret_cast<f32x4*>(v + s) = b;
+}
+
+int check_moments(const char* what, const void* a, const void* b, const void* c, const void* d, const void* e, const void* f,
+                  int64_t nblocks) {
+  SRX_CHECK_ARG(nblocks >= 0 && nblocks < (1LL << 33), "%s: nblocks %lld out of range", what, (long long)nblocks);
+  SRX_CHECK_ARG(nblocks == 0 || (a && b && c && d && e && f), "%s: null pointer", what);
+  SRX_CHECK_ARG(((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16 == 0, "%s: moments must be 16-byte aligned", what);
+  return SRX_OK;
+}
+
+// One pass over the tensors in launches of at most NG gradients, `fn(args, chunks)` each.
+template <int NG, typename F> int each_launch(const srx_adamw_desc* d, int norm_mode, F fn) {
+  const int per = NG == 1 ? d->ntensors : NG;
+  for (int t0 = 0; t0 < d->ntensors; t0 += per) {
+    const int t1 = t0 + per < d->ntensors ? t0 + per : d->ntensors;
+    const int c0 = d->chunk_start[t0], c1 = d->chunk_start[t1];
+    if (c1 <= c0) continue;
+    StepArgs<NG> a = {};
+    a.tensors = d->tensors; a.chunks = d->chunks; a.coef = d->coef; a.partial = d->partial;
+    a.m = d->m; a.v = d->v; a.m_scale = d->m_scale; a.v_scale = d->v_scale;
+    a.flat = d->flat_grad; a.flat_dtype = d->flat_dtype; a.chunk0 = c0; a.t0 = t0; a.norm_mode = norm_mode;
+    if (NG > 1)
+      for (int k = 0; k < t1 - t0; ++k) {
+        a.g[k] = d->grads[t0 + k];
+        if (d->grad_dtypes && d->grad_dtypes[t0 + k] == SRX_BF16) a.is_bf16[k >> 6] |= 1ull << (k & 63);
+      }
+    if (int rc = fn(a, c1 - c0)) return rc;
+  }
+  return SRX_OK;
+}
+
+template <int NG> int step_launches(const srx_adamw_desc* d, hipStream_t s) {
+  const int norm = d->max_norm > 0 || d->skip_nonfinite;
+  if (norm) {
+    int rc = each_launch<NG>(d, norm, [&](const StepArgs<NG>& a, int n) {
+      hipLaunchKernelGGL(adamw_norm_kernel<NG>, dim3(n), dim3(TPB), 0, s, a);
+      return srx_check_launch("adamw_norm");
+    });
+    if (rc) return rc;
+  }
+  for (int t0 = 0; t0 < d->ntensors; t0 += PREP_TENSORS) {
+    PrepArgs p = {};
+    p.tensors = d->tensors; p.steps = d->steps; p.coef = d->coef; p.partial = d->partial; p.norm = d->norm;
+    p.grad_scale = d->grad_scale; p.max_norm = d->max_norm; p.ntensors = d->ntensors; p.t0 = t0;
+    p.nchunks = d->chunk_start[d->ntensors];
+    p.norm_mode = !norm ? 0 : t0 ? 2 : 1;
+    p.skip_nonfinite = d->skip_nonfinite;
+    for (int g = 0; g < d->ngroups; ++g) p.groups[g] = d->groups[g];
+    for (int k = 0; k < PREP_TENSORS && t0 + k < d->ntensors; ++k)
+      if (NG == 1 || d->grads[t0 + k]) p.has_grad[k >> 5] |= 1u << (k & 31);
+    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(PREP_TPB), 0, s, p);
+    if (int rc = srx_check_launch("adamw_prepare")) return rc;
+  }
+  return each_launch<NG>(d, norm, [&](const StepArgs<NG>& a, int n) {
+    if (d->state_bits == 8) hipLaunchKernelGGL((adamw_step_kernel<8, NG>), dim3(n), dim3(TPB), 0, s, a);
+    else hipLaunchKernelGGL((adamw_step_kernel<32, NG>), dim3(n), dim3(TPB), 0, s, a);
+    return srx_check_launch("adamw_step");
+  });
+}
+
+}  // namespace
+
+extern "C" {
+
+int srx_adamw_step(const srx_adamw_desc* d, void* stream) {
+  SRX_CHECK_ARG(d != nullptr, "srx_adamw_step: null descriptor");
+  SRX_CHECK_ARG(d->state_bits == 32 || d->state_bits == 8, "srx_adamw_step: state_bits must be 32 or 8, got %d", d->state_bits);
+  SRX_CHECK_ARG(d->ntensors > 0, "srx_adamw_step: ntensors must be positive");
+  SRX_CHECK_ARG(d->ngroups > 0 && d->ngroups <= SRX_ADAMW_MAX_GROUPS, "srx_adamw_step: %d groups, 1 to %d are supported",
+                d->ngroups, SRX_ADAMW_MAX_GROUPS);
+  SRX_CHECK_ARG(d->tensors && d->chunks && d->chunk_start && d->groups && d->steps && d->coef, "srx_adamw_step: null table");
+  SRX_CHECK_ARG((d->grads != nullptr) != (d->flat_grad != nullptr), "srx_adamw_step: give either grads or flat_grad");
+  SRX_CHECK_ARG(!d->flat_grad || d->flat_dtype == SRX_BF16 || d->flat_dtype == SRX_F32, "srx_adamw_step: bad flat_dtype %d", d->flat_dtype);
+  SRX_CHECK_ARG(d->m && d->v && (d->state_bits == 32 || (d->m_scale && d->v_scale)), "srx_adamw_step: null moments");
+  SRX_CHECK_ARG(((uintptr_t)d->m | (uintptr_t)d->v) % 16 == 0, "srx_adamw_step: moments must be 16-byte aligned");
+  SRX_CHECK_ARG(!(d->max_norm < 0) && d->max_norm == d->max_norm, "srx_adamw_step: max_norm must not be negative or NaN");
+  SRX_CHECK_ARG(!(d->max_norm > 0 || d->skip_nonfinite) || (d->partial && d->norm), "srx_adamw_step: the norm needs partial and norm");
+  SRX_CHECK_ARG(d->grad_scale - d->grad_scale == 0, "srx_adamw_step: grad_scale must be finite");
+  SRX_CHECK_ARG(d->chunk_start[0] == 0, "srx_adamw_step: chunk_start must begin at 0");
+  for (int i = 0; i < d->ntensors; ++i) {
+    SRX_CHECK_ARG(d->chunk_start[i + 1] >= d->chunk_start[i], "srx_adamw_step: chunk_start must not decrease (tensor %d)", i);
+    SRX_CHECK_ARG(!d->grad_dtypes || d->grad_dtypes[i] == SRX_BF16 || d->grad_dtypes[i] == SRX_F32,
+                  "srx_adamw_step: bad gradient dtype %d of tensor %d", d->grad_dtypes[i], i);
+    if (d->grads)
+      SRX_CHECK_ARG((uintptr_t)d->grads[i] % (d->grad_dtypes && d->grad_dtypes[i] == SRX_BF16 ? 2 : 4) == 0,
+                    "srx_adamw_step: gradient %d is not aligned to its type", i);
+  }
+  for (int g = 0; g < d->ngroups; ++g) {
+    const srx_adamw_group& q = d->groups[g];
+    SRX_CHECK_ARG(q.beta1 >= 0 && q.beta1 < 1 && q.beta2 >= 0 && q.beta2 < 1 && q.eps >= 0 && q.lr >= 0 && q.weight_decay >= 0 &&
+                      q.lr - q.lr == 0 && q.weight_decay - q.weight_decay == 0 && q.eps - q.eps == 0,
+                  "srx_adamw_step: bad hyper-parameters in group %d (lr %g, betas %g %g, eps %g, weight_decay %g)", g, q.lr,
+                  q.beta1, q.beta2, q.eps, q.weight_decay);
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return d->flat_grad ? step_launches<1>(d, s) : step_launches<MAX_GRADS>(d, s);
+}
+
+int srx_adamw_moments_to8(const float* m, const float* v, void* m_code, void* v_code, float* m_scale, float* v_scale,
+                          int64_t nblocks, void* stream) {
+  if (int rc = check_moments("srx_adamw_moments_to8", m, v, m_code, v_code, m_scale, v_scale, nblocks)) return rc;
+  if (nblocks == 0) return SRX_OK;
+  hipLaunchKernelGGL(moments_to8_kernel, dim3((unsigned)((nblocks + 3) / 4)), dim3(TPB), 0, reinterpret_cast<hipStream_t>(stream), m, v,
+                     (uint8_t*)m_code, (uint8_t*)v_code, m_scale, v_scale, nblocks);
+  return srx_check_launch("moments_to8");
+}
+
+int srx_adamw_moments_from8(const void* m_code, const void* v_code, const float* m_scale, const float* v_scale, float* m,
+                            float* v, int64_t nblocks, void* stream) {
+  if (int rc = check_moments("srx_adamw_moments_from8", m, v, m_code, v_code, m_scale, v_scale, nblocks)) return rc;
+  if (nblocks == 0) return SRX_OK;
+  hipLaunchKernelGGL(moments_from8_kernel, dim3((unsigned)((nblocks + 3) / 4)), dim3(TPB), 0, reinterpret_cast<hipStream_t>(stream),
+                     (const uint8_t*)m_code, (const uint8_t*)v_code, m_scale, v_scale, m, v, nblocks);
+  return srx_check_launch("moments_from8");
+}
+
+}  // extern "C"

@@ -79,10 +79,12 @@ def fit(gen, disc, vgg_loss, train_loader: Iterable, val_loader: Iterable, check
         epochs: int, pretrain_epochs: int = 0, mode: str = "all", resume: bool = False, lr: float = 2e-4,
         lambda_l1: float = 1.0, lambda_adv: float = 5e-3, lambda_percep: float = 1.0,
         compute_dtype=torch.bfloat16, grad_sync_g: Optional[Callable] = None,
-        grad_sync_d: Optional[Callable] = None, log: Callable[[str], None] = print) -> List[Dict[str, float]]:
+        grad_sync_d: Optional[Callable] = None, log: Callable[[str], None] = print,
+        optimizer: Optional[Callable] = None) -> List[Dict[str, float]]:
     """The body of the reference's ``main`` (:139-208) for modules that already sit on the GPU.
     ``train_loader`` / ``val_loader`` are re-iterated every epoch and yield ``(lr, hr)`` batches
-    in [-1, 1]; ``batch_shape`` is the LR batch shape ``(B, 3, h, w)``.  Returns one dictionary
+    in [-1, 1]; ``batch_shape`` is the LR batch shape ``(B, 3, h, w)``; ``optimizer(module)``, if given, builds
+    the optimizers (default Adam with ``lr``; the epoch's learning rate is set on them either way).  Returns one dictionary
     per finished adversarial epoch (losses, learning rate, validation numbers)."""
     if mode not in ("pretrain", "train", "all"):
         raise ValueError(f"mode must be pretrain, train or all (got {mode!r})")
@@ -92,7 +94,7 @@ def fit(gen, disc, vgg_loss, train_loader: Iterable, val_loader: Iterable, check
 
     adv = T.AdversarialTrainer(gen, disc, vgg_loss, batch_shape, compute_dtype, lr=lr, lambda_l1=lambda_l1,
                                lambda_adv=lambda_adv, lambda_percep=lambda_percep,
-                               grad_sync_g=grad_sync_g, grad_sync_d=grad_sync_d)
+                               grad_sync_g=grad_sync_g, grad_sync_d=grad_sync_d, optimizer=optimizer)
     log(f"--- Perceptual loss: VGG19 weights from {getattr(vgg_loss, 'weights_source', 'unknown')} ---")
     start_epoch, best_psnr = 0, 0.0
     if resume:
@@ -102,7 +104,7 @@ def fit(gen, disc, vgg_loss, train_loader: Iterable, val_loader: Iterable, check
 
     if mode in ("pretrain", "all") and not pretrained.exists() and start_epoch == 0 and pretrain_epochs > 0:
         log("--- Starting Generator Pre-training (L1 Loss only) ---")
-        warm = T.GeneratorWarmupTrainer(gen, batch_shape, compute_dtype, lr=lr, grad_sync=grad_sync_g)
+        warm = T.GeneratorWarmupTrainer(gen, batch_shape, compute_dtype, lr=lr, grad_sync=grad_sync_g, optimizer=optimizer)
         for epoch in range(pretrain_epochs):
             l1 = pretrain_one_epoch(warm, train_loader, batch_shape)
             log(f"Pre-train epoch {epoch + 1} | L1: {l1:.5f}")

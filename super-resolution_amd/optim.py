@@ -1,0 +1,387 @@
+"""AdamW over a list of tensors (``srx_adamw_step``): what ``train.FlatAdam`` does not cover.
+
+``FlatAdam`` is ``torch.optim.Adam`` (esrgan/train_esrgan.py:134-135) over ONE flat fp32 range.  ``AdamW`` takes the
+parameters as they are — any number of tensors, in groups with a learning rate and a (decoupled) weight decay of
+their own, fp32 or bf16 with an fp32 master — and adds clipping by the global gradient norm, the skip of a step
+whose gradients are not finite, and moments in 8 bits (2 bytes and a bit per parameter instead of 8).  All
+decisions are taken on the device: a step never waits for the host and can be captured into a HIP graph.
+"""
+from __future__ import annotations
+
+import array
+import ctypes as C
+import math
+from operator import attrgetter
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
+
+import numpy as np
+import torch
+
+from . import _lib as L
+from . import engine
+
+_ptr = torch.Tensor.data_ptr
+_numel = torch.Tensor.numel
+_contiguous = torch.Tensor.is_contiguous
+_device = torch.Tensor.get_device
+_dtype, _grad = attrgetter("dtype"), attrgetter("grad")
+_DTYPE_ID = {torch.bfloat16: L.BF16, torch.float32: L.F32}
+
+
+def decay_groups(module: torch.nn.Module, weight_decay: float = 1e-2) -> List[dict]:
+    """Two parameter groups of a module, in ``parameters()`` order within each: tensors with two or more dimensions
+    (kernels) decay; norm weights, gates and biases do not."""
+    params = [p for p in module.parameters() if p.requires_grad]
+    groups = [{"params": [p for p in params if p.dim() >= 2], "weight_decay": weight_decay},
+              {"params": [p for p in params if p.dim() < 2], "weight_decay": 0.0}]
+    return [g for g in groups if g["params"]]
+
+
+class AdamW:
+    """One step = ``p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)`` (``torch.optim.AdamW``).
+
+    params: tensors, or dicts ``{"params": [...], "lr": ..., "betas": ..., "eps": ..., "weight_decay": ...}`` (at most 32);
+        contiguous fp32 or bf16 tensors on one GPU.  A bf16 parameter gets an fp32 master copy; writing the
+        parameter (loading a checkpoint, say) also moves its master.
+    state_bits: 32, or 8: moments of one byte with a scale for every 256 elements of a tensor.
+    max_grad_norm: gradients are scaled by ``min(1, max_grad_norm / (norm + 1e-6))``, norm over all tensors.
+    skip_nonfinite: a step whose gradient norm is infinite or NaN changes nothing.
+
+    ``param_groups`` holds the hyper-parameters under torch's names and is read at every step; ``lr`` sets them all.
+    A captured step replays with the hyper-parameters and ``grad_scale`` it was captured with; its step count
+    advances.  One optimizer's steps share its state and workspaces: they must not overlap."""
+
+    def __init__(self, params: Iterable, lr: float = 2e-4, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, *, state_bits: int = 32, max_grad_norm: Optional[float] = None,
+                 skip_nonfinite: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if max_grad_norm is not None and not 0 < max_grad_norm < math.inf:
+            raise ValueError(f"max_grad_norm must be positive and finite, got {max_grad_norm}")
+        params = list(params)
+        if not params:
+            raise ValueError("no parameters")
+        if not all(isinstance(g, dict) for g in params):
+            if any(isinstance(g, dict) for g in params):
+                raise TypeError("params: tensors or dicts, not both")
+            params = [{"params": params}]
+        if len(params) > L.ADAMW_MAX_GROUPS:
+            raise ValueError(f"{len(params)} parameter groups: at most {L.ADAMW_MAX_GROUPS} are supported")
+        defaults = {"lr": lr, "betas": tuple(betas), "eps": eps, "weight_decay": weight_decay}
+        self.param_groups: List[dict] = []
+        for g in params:
+            if not set(g) <= {"params", "lr", "betas", "eps", "weight_decay", "initial_lr"}:
+                raise ValueError(f"unknown keys in a parameter group: {sorted(set(g) - set(defaults) - {'params'})}")
+            ps = g["params"]
+            ps = [ps] if isinstance(ps, torch.Tensor) else list(ps)
+            group = {**defaults, **g, "params": ps}
+            group["betas"] = tuple(group["betas"])
+            group.setdefault("initial_lr", group["lr"])
+            self.param_groups.append(group)
+        self.params: List[torch.Tensor] = [p for g in self.param_groups for p in g["params"]]
+        if not self.params:
+            raise ValueError("no parameters")
+        for i, p in enumerate(self.params):
+            if not isinstance(p, torch.Tensor):
+                raise TypeError(f"parameter {i} is a {type(p).__name__}, not a tensor")
+            if p.device.type != "cuda":
+                raise RuntimeError(f"libsrx runs on a ROCm GPU only (parameter {i} is on {p.device})")
+            if p.device != self.params[0].device:
+                raise ValueError(f"parameters on {self.params[0].device} and on {p.device}: all must be on one GPU")
+            if p.dtype not in _DTYPE_ID:
+                raise ValueError(f"parameter {i} is {p.dtype}: float32 or bfloat16 are supported")
+        self._check_hyper()
+        self.device = self.params[0].device
+        self.state_bits, self.max_grad_norm, self.skip_nonfinite = state_bits, max_grad_norm, bool(skip_nonfinite)
+        self._lib = L.lib()
+        self._n = [p.numel() for p in self.params]
+        self._shapes = [p.shape for p in self.params]
+        self._dtypes = [p.dtype for p in self.params]
+        blocks = [-(-n // L.ADAMW_BLOCK) for n in self._n]
+        self._first = [0]
+        for b in blocks:
+            self._first.append(self._first[-1] + b)
+        self.nblocks = self._first[-1]
+        chunks = [-(-n // L.ADAMW_CHUNK) for n in self._n]
+        start = np.concatenate([[0], np.cumsum(chunks)]).astype(np.int32)
+        table = np.empty((int(start[-1]), 2), dtype=np.int32)
+        table[:, 0] = np.repeat(np.arange(len(chunks)), chunks)
+        table[:, 1] = np.arange(start[-1]) - np.repeat(start[:-1], chunks)
+        dev, padded = self.device, L.ADAMW_BLOCK * self.nblocks
+        with torch.cuda.device(dev):
+            zeros = lambda n, t=torch.float32: torch.zeros(max(n, 1), dtype=t, device=dev)  # noqa: E731
+            self._chunks = torch.from_numpy(table.reshape(-1) if table.size else np.zeros(2, np.int32)).to(dev)
+            self._m = torch.zeros(padded, dtype=torch.float32 if state_bits == 32 else torch.uint8, device=dev)
+            self._v = torch.zeros_like(self._m)
+            self._m_scale, self._v_scale = (zeros(self.nblocks), zeros(self.nblocks)) if state_bits == 8 else (None, None)
+            self._steps = zeros(len(self.params), torch.int32)
+            self._coef = zeros(4 + 8 * len(self.params))
+            self._partial = zeros(int(start[-1]), torch.float64)
+            half = [n if t == torch.bfloat16 else 0 for n, t in zip(self._n, self._dtypes)]
+            self._master_at = [0]
+            for n in half:
+                self._master_at.append(self._master_at[-1] + n)
+            #: fp32 masters of the bf16 parameters, one after the other (None: there are none)
+            self.master = zeros(self._master_at[-1]) if sum(half) else None
+            self._ptrs: List[int] = []
+            self._bind()
+            self._copy_masters()
+            d = self._desc = L.AdamwDesc()
+            d.state_bits, d.ntensors, d.ngroups = state_bits, len(self.params), len(self.param_groups)
+            self._start = start
+            d.chunks, d.chunk_start = self._chunks.data_ptr(), start.ctypes.data
+            d.m, d.v = self._m.data_ptr() or self._steps.data_ptr(), self._v.data_ptr() or self._steps.data_ptr()
+            if state_bits == 8:
+                d.m_scale, d.v_scale = self._m_scale.data_ptr(), self._v_scale.data_ptr()
+            d.steps, d.coef, d.partial = self._steps.data_ptr(), self._coef.data_ptr(), self._partial.data_ptr()
+            self._groups = (L.AdamwGroup * len(self.param_groups))()
+            d.groups = C.addressof(self._groups)
+            torch.cuda.current_stream(dev).synchronize()     # ready for a first step on any stream
+
+    # ---------------------------------------------------------------- hyper-parameters
+    @property
+    def lr(self) -> float:
+        return self.param_groups[0]["lr"]
+
+    @lr.setter
+    def lr(self, value: float) -> None:
+        for g in self.param_groups:
+            g["lr"] = value
+
+    def _check_hyper(self) -> None:
+        for i, g in enumerate(self.param_groups):
+            b = g["betas"]
+            if not (0 <= g["lr"] < math.inf and len(b) == 2 and 0 <= b[0] < 1 and 0 <= b[1] < 1 and 0 <= g["eps"] < math.inf
+                    and 0 <= g["weight_decay"] < math.inf):
+                raise ValueError(f"parameter group {i}: lr, eps and weight_decay must be finite and not negative, betas in [0, 1): "
+                                 f"{ {k: v for k, v in g.items() if k != 'params'} }")
+
+    # ---------------------------------------------------------------- tables
+    def _bind(self) -> None:
+        """Write the parameters' addresses into the device table: at construction, and again when a parameter has got new
+        storage since (``module.to()``, ``flatten_parameters``)."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: the parameters have got new storage; run one step outside of the capture first")
+        ptrs = list(map(_ptr, self.params))
+        for i, p in enumerate(self.params):
+            if p.device != self.device or p.dtype != self._dtypes[i] or p.numel() != self._n[i]:
+                raise RuntimeError(f"AdamW: parameter {i} was {self._dtypes[i]} of {self._n[i]} elements on {self.device} and is now "
+                                   f"{p.dtype} of {p.numel()} on {p.device}: build a new optimizer")
+            if not p.is_contiguous():
+                raise ValueError(f"AdamW: parameter {i} is not contiguous")
+        spans = sorted((a, a + n * p.element_size(), i) for i, (a, n, p) in enumerate(zip(ptrs, self._n, self.params)) if n)
+        for (_, end, i), (begin, _, k) in zip(spans, spans[1:]):
+            if begin < end:
+                raise ValueError(f"AdamW: parameters {i} and {k} share memory (or are the same tensor)")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("AdamW: a parameter is given twice")
+        # views of one buffer that cover it without gaps: their gradients may come as one buffer too
+        base, esize = (spans[0][0], self.params[0].element_size()) if spans else (0, 1)
+        self._flat = bool(spans) and len(set(self._dtypes)) == 1 and spans[-1][1] - base == sum(self._n) * esize
+        arr = (L.AdamwTensor * len(self.params))()
+        i = 0
+        for gi, g in enumerate(self.param_groups):
+            for _ in g["params"]:
+                t = arr[i]
+                t.p, t.n, t.first_block, t.group = ptrs[i] or None, self._n[i], self._first[i], gi
+                if self._dtypes[i] == torch.bfloat16:
+                    t.master = self.master.data_ptr() + 4 * self._master_at[i]
+                t.g_off = (ptrs[i] - base) // esize if self._flat and self._n[i] else 0
+                i += 1
+        raw = torch.frombuffer(bytearray(C.string_at(C.addressof(arr), C.sizeof(arr))), dtype=torch.uint8)
+        if self._ptrs:
+            torch.cuda.synchronize(self.device)      # steps in flight still read the old table
+        self._tensors = raw.to(self.device)
+        self._ptrs = ptrs
+
+    def _copy_masters(self) -> None:
+        for i, p in enumerate(self.params):
+            if p.dtype == torch.bfloat16:
+                self.master[self._master_at[i]:self._master_at[i + 1]].copy_(p.detach().reshape(-1))
+
+    # ---------------------------------------------------------------- the step
+    def step(self, grads: Union[None, torch.Tensor, Sequence[Optional[torch.Tensor]]] = None,
+             grad_scale: float = 1.0) -> Optional[torch.Tensor]:
+        """One step on the current stream.  grads: None (each parameter's ``.grad``), a list with one gradient (fp32 or
+        bf16) or None per parameter — None leaves that parameter, its moments and its step count as they are — or,
+        where the parameters are views that cover one flat buffer, one flat gradient of the same layout.
+        ``grad_scale`` multiplies every gradient first (1 / loss scale).  Returns the gradient norm before clipping
+        (0-dim tensor, not synchronised) if ``max_grad_norm`` or ``skip_nonfinite`` is set, else None."""
+        if torch.cuda.current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.step(grads, grad_scale)
+        if not math.isfinite(grad_scale):
+            raise ValueError(f"grad_scale must be finite, got {grad_scale}")
+        if list(map(_ptr, self.params)) != self._ptrs:
+            self._bind()
+        d, keep = self._desc, None
+        if isinstance(grads, torch.Tensor):
+            if not self._flat:
+                raise ValueError("a flat gradient needs parameters of one type that are views covering one flat buffer")
+            if grads.device != self.device or grads.dtype not in _DTYPE_ID or grads.numel() != sum(self._n) or not grads.is_contiguous():
+                raise ValueError(f"flat gradient: {sum(self._n)} contiguous float32 or bfloat16 values on {self.device} expected, got "
+                                 f"{grads.dtype} of {tuple(grads.shape)} on {grads.device}")
+            d.grads, d.grad_dtypes = None, None
+            d.flat_grad, d.flat_dtype = grads.data_ptr(), _DTYPE_ID[grads.dtype]
+            if grads.numel() == 0:
+                return self._empty_norm()
+        else:
+            addresses, types, keep = self._addresses(grads)
+            d.grads, d.grad_dtypes, d.flat_grad = addresses.buffer_info()[0], types, None
+        self._check_hyper()
+        for q, g in zip(self._groups, self.param_groups):
+            q.lr, (q.beta1, q.beta2), q.eps, q.weight_decay = g["lr"], g["betas"], g["eps"], g["weight_decay"]
+        d.tensors = self._tensors.data_ptr()
+        d.grad_scale, d.max_norm, d.skip_nonfinite = grad_scale, self.max_grad_norm or 0.0, self.skip_nonfinite
+        norm = None
+        if self.max_grad_norm or self.skip_nonfinite:
+            norm = torch.empty((), dtype=torch.float32, device=self.device)
+            d.norm = norm.data_ptr()
+        L.check(self._lib.srx_adamw_step(C.byref(d), engine.stream_ptr(self.device)), "srx_adamw_step")
+        del keep
+        return norm
+
+    def _empty_norm(self):
+        return torch.zeros((), device=self.device) if self.max_grad_norm or self.skip_nonfinite else None
+
+    def _addresses(self, grads):
+        """(addresses, C array of dtypes or None, what has to live until the launch) of a list of gradients."""
+        given = grads is not None
+        grads = list(grads) if given else list(map(_grad, self.params))
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        some = grads if all(g is not None for g in grads) else [g for g in grads if g is not None]
+        # whole lists are compared in C: 702 tensors cost tens of microseconds here, not hundreds
+        index = self.device.index
+        n = self._n if some is grads else [k for k, g in zip(self._n, grads) if g is not None]
+        if list(map(_numel, some)) != n or any(i != index for i in map(_device, some)) or \
+                (given and any(g.shape != p.shape for g, p in zip(grads, self.params) if g is not None)):
+            for i, (g, p) in enumerate(zip(grads, self.params)):
+                if g is not None and (g.shape != p.shape or g.device != p.device):
+                    raise ValueError(f"gradient {i} has shape {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {p.device}")
+        types = list(map(_dtype, some))
+        if not set(types) <= set(_DTYPE_ID):
+            raise ValueError(f"gradients must be float32 or bfloat16, got {sorted(str(t) for t in set(types) - set(_DTYPE_ID))}")
+        if not all(map(_contiguous, some)):
+            grads = [g if g is None else g.contiguous() for g in grads]
+            some = [g for g in grads if g is not None]
+        ptrs = list(map(_ptr, some))
+        if 0 in ptrs:                     # an empty tensor has no address, but it takes its step: any that is not 0 will do
+            ptrs = [p or self._steps.data_ptr() for p in ptrs]
+        if some is not grads:
+            left = iter(ptrs)
+            ptrs = [0 if g is None else next(left) for g in grads]
+        ids = None
+        if torch.bfloat16 in types:
+            ids = bytes(L.F32 if g is None else _DTYPE_ID[g.dtype] for g in grads)
+        return array.array("Q", ptrs), (C.cast(C.c_char_p(ids), C.c_void_p) if ids is not None else None), (grads, ids)
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        for p in self.params:
+            if p.grad is not None:
+                if set_to_none:
+                    p.grad = None
+                else:
+                    p.grad.zero_()
+
+    # ---------------------------------------------------------------- state
+    def moments(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(m, v) in fp32, flat: every parameter's start at a multiple of 256 elements, zeros between.  The optimizer's own
+        buffers with 32-bit moments; with 8-bit ones new tensors of the values that they stand for."""
+        if self.state_bits == 32:
+            return self._m, self._v
+        with torch.cuda.device(self.device):
+            m, v = (torch.empty(self._m.numel(), dtype=torch.float32, device=self.device) for _ in range(2))
+            L.check(self._lib.srx_adamw_moments_from8(self._m.data_ptr(), self._v.data_ptr(), self._m_scale.data_ptr(),
+                                                      self._v_scale.data_ptr(), m.data_ptr(), v.data_ptr(), self.nblocks,
+                                                      engine.stream_ptr(self.device)), "srx_adamw_moments_from8")
+        return m, v
+
+    def load_moments(self, m: torch.Tensor, v: torch.Tensor, step: Union[int, Sequence[int]],
+                     master: Optional[torch.Tensor] = None) -> None:
+        """Set the whole state: moments as :meth:`moments` returns them, step counts (one, or one per parameter), and the
+        masters of the bf16 parameters (None: taken from the parameters)."""
+        steps = [int(step)] * len(self.params) if isinstance(step, int) else [int(k) for k in step]
+        if len(steps) != len(self.params) or min(steps) < 0:
+            raise ValueError("step: one count that is not negative, or one per parameter")
+        for name, t, n in (("m", m, self._m.numel()), ("v", v, self._v.numel())) + \
+                ((("master", master, self._master_at[-1]),) if master is not None else ()):
+            if t.numel() != n or t.dtype != torch.float32 or t.device != self.device:
+                raise ValueError(f"{name}: {n} float32 values on {self.device} expected, got {t.dtype} of {t.numel()} on {t.device}")
+        with torch.cuda.device(self.device), torch.no_grad():
+            if self.state_bits == 32:
+                self._m.copy_(m.reshape(-1))
+                self._v.copy_(v.reshape(-1))
+            else:
+                m, v = (t.detach().reshape(-1).clone() for t in (m, v))       # contiguous and aligned
+                L.check(self._lib.srx_adamw_moments_to8(m.data_ptr(), v.data_ptr(), self._m.data_ptr(), self._v.data_ptr(),
+                                                        self._m_scale.data_ptr(), self._v_scale.data_ptr(), self.nblocks,
+                                                        engine.stream_ptr(self.device)), "srx_adamw_moments_to8")
+            self._steps.copy_(torch.tensor(steps, dtype=torch.int32))
+            if self.master is not None:
+                if master is None:
+                    self._copy_masters()
+                else:
+                    self.master.copy_(master.reshape(-1))
+            torch.cuda.current_stream(self.device).synchronize()
+
+    @property
+    def step_counts(self) -> List[int]:
+        """Steps taken by each parameter (reads the device)."""
+        return self._steps[:len(self.params)].tolist()
+
+    def state_dict(self) -> dict:
+        """The ``torch.optim.AdamW.state_dict()`` layout with fp32 moments whatever ``state_bits`` (they load back to the
+        same 8 bits); a bf16 parameter's state also holds its ``master``."""
+        m, v = self.moments()
+        state = {}
+        for i, (n, shp, t) in enumerate(zip(self._n, self._shapes, self.step_counts)):
+            if t == 0 and self.master is None:
+                continue
+            at = L.ADAMW_BLOCK * self._first[i]
+            state[i] = {"step": torch.tensor(float(t)), "exp_avg": m[at:at + n].view(shp).clone(),
+                        "exp_avg_sq": v[at:at + n].view(shp).clone()}
+            if self._dtypes[i] == torch.bfloat16:
+                state[i]["master"] = self.master[self._master_at[i]:self._master_at[i + 1]].view(shp).clone()
+        groups, k = [], 0
+        for g in self.param_groups:
+            groups.append({**{key: g[key] for key in ("lr", "initial_lr", "betas", "eps", "weight_decay")},
+                           "amsgrad": False, "maximize": False, "foreach": None, "capturable": False, "differentiable": False,
+                           "fused": None, "decoupled_weight_decay": True, "params": list(range(k, k + len(g["params"])))})
+            k += len(g["params"])
+        return {"state": state, "param_groups": groups}
+
+    def load_state_dict(self, sd: dict) -> None:
+        """Accepts a state_dict written by this class (any ``state_bits``) or by ``torch.optim.AdamW`` over the same parameters
+        in the same groups."""
+        groups = sd["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError(f"optimizer state_dict does not match: groups of {[len(g['params']) for g in groups]} parameters, "
+                             f"{[len(g['params']) for g in self.param_groups]} here")
+        if any(g.get("amsgrad") or g.get("maximize") for g in groups):
+            raise ValueError("optimizer state_dict with amsgrad or maximize: neither is supported")
+        order = [k for g in groups for k in g["params"]]
+        m = torch.zeros(self._m.numel(), dtype=torch.float32, device=self.device)
+        v, steps = torch.zeros_like(m), []
+        master = None
+        if self.master is not None:
+            master = torch.cat([p.detach().reshape(-1).float() for p in self.params if p.dtype == torch.bfloat16])
+        for i, (k, n, shp) in enumerate(zip(order, self._n, self._shapes)):
+            st = sd["state"].get(k)
+            steps.append(int(float(st["step"])) if st is not None else 0)
+            if st is None:
+                continue
+            if tuple(st["exp_avg"].shape) != tuple(shp):
+                raise ValueError(f"optimizer state for parameter {i} has shape {tuple(st['exp_avg'].shape)}, expected {tuple(shp)}")
+            at = L.ADAMW_BLOCK * self._first[i]
+            m[at:at + n].copy_(st["exp_avg"].reshape(-1))
+            v[at:at + n].copy_(st["exp_avg_sq"].reshape(-1))
+            if "master" in st and self._dtypes[i] == torch.bfloat16:
+                master[self._master_at[i]:self._master_at[i + 1]].copy_(st["master"].reshape(-1))
+        for g, new in zip(self.param_groups, groups):
+            for key in ("lr", "eps", "weight_decay"):
+                g[key] = float(new[key])
+            g["betas"] = tuple(new["betas"])
+            g["initial_lr"] = new.get("initial_lr", g["initial_lr"])
+        self._check_hyper()
+        self.load_moments(m, v, steps, master)

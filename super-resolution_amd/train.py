@@ -158,6 +158,20 @@ def _backward_and_step(plan, opt: "FlatAdam") -> bool:
     return True
 
 
+def _make_optimizer(optimizer: Optional[Callable], module, flat: torch.Tensor, lr: float):
+    """The optimizer of a trainer: ``optimizer(module)`` — for instance ``lambda m: optim.AdamW(optim.decay_groups(m),
+    lr=2e-4, max_grad_norm=1.0, state_bits=8)`` — or FlatAdam.  It is built after the module's parameters
+    have become views of one flat buffer and before the first step, its ``step`` gets the flat gradient, and
+    ``lr`` and ``state_dict`` / ``load_state_dict`` are used as FlatAdam's are."""
+    if optimizer is None:
+        return FlatAdam(flat, lr=lr, shapes=[p.shape for p in module.parameters()])
+    opt = optimizer(module)
+    trained = getattr(opt, "params", None)
+    if trained is not None and sum(p.numel() for p in trained) != flat.numel():
+        raise ValueError("the optimizer must take every parameter of the module: the trainers hand it the whole flat gradient")
+    return opt
+
+
 class GeneratorWarmupTrainer:
     """Generator warm-up: L1 pixel loss, fwd + bwd + Adam.
 
@@ -166,10 +180,12 @@ class GeneratorWarmupTrainer:
     CUs for its whole duration (prologue, epilogue, launch boundary), and two independent
     launch chains in flight hide each other's bubbles.  Sub-batch gradients accumulate
     into one flat buffer.  ``grad_sync`` (optional) is called with that buffer after
-    backward and before the optimizer step (the data-parallel all-reduce hook)."""
+    backward and before the optimizer step (the data-parallel all-reduce hook).
+    ``optimizer`` (optional): called with the module, returns the optimizer to train it with (see
+    ``_make_optimizer``); default ``FlatAdam`` with ``lr``."""
 
     def __init__(self, gen, batch_shape, compute_dtype=torch.bfloat16, lr=2e-4, grad_sync=None,
-                 n_streams: int = 1):
+                 n_streams: int = 1, optimizer: Optional[Callable] = None):
         B, _, h, w = batch_shape
         if B % n_streams:
             n_streams = 1
@@ -192,7 +208,7 @@ class GeneratorWarmupTrainer:
                                                    accumulate_grads=(i > 0), **kw))
         self.plan = self.plans[0]
         self.streams = [torch.cuda.Stream(device=dev) for _ in range(n_streams)] if n_streams > 1 else [None]
-        self.opt = FlatAdam(self.flat, lr=lr, shapes=[p.shape for p in gen.parameters()])
+        self.opt = _make_optimizer(optimizer, gen, self.flat, lr)
         self.loss_acc = torch.zeros(1, dtype=torch.float32, device=dev)
         self.grad_sync = grad_sync
         self.steps = 0
@@ -215,7 +231,8 @@ class GeneratorWarmupTrainer:
                                      p.GY.ptr(), p.GY.img_stride, 1.0 / self.n_streams, Y.B, p.out_ch, Y.H, Y.W,
                                      engine.stream_ptr(p.device)), "srx_l1_c8_nchw")
         if self.n_streams == 1:
-            if self.grad_sync is None and self.step_in_backward and _backward_and_step(p, self.opt):
+            if self.grad_sync is None and self.step_in_backward and isinstance(self.opt, FlatAdam) \
+                    and _backward_and_step(p, self.opt):
                 return "stepped"
             return _backward_with_exchange(p, self.grad_sync)
         p.run_backward_ops()
@@ -278,11 +295,14 @@ class AdversarialTrainer:
     ``losses()`` is the only host synchronisation.
 
     grad_sync_d / grad_sync_g (optional) are called with the flat gradient buffer before the
-    respective optimizer step (data-parallel all-reduce hooks)."""
+    respective optimizer step (data-parallel all-reduce hooks).  optimizer (optional): called once
+    with the generator and once with the discriminator, returns the optimizer to train it with (see
+    ``_make_optimizer``); default ``FlatAdam`` with ``lr`` for both."""
 
     def __init__(self, gen, disc, vgg_loss, batch_shape, compute_dtype=torch.bfloat16, lr: float = 2e-4,
                  lambda_l1: float = 1.0, lambda_adv: float = 5e-3, lambda_percep: float = 1.0,
-                 grad_sync_g: Optional[Callable] = None, grad_sync_d: Optional[Callable] = None):
+                 grad_sync_g: Optional[Callable] = None, grad_sync_d: Optional[Callable] = None,
+                 optimizer: Optional[Callable] = None):
         B, _, h, w = batch_shape
         H, W = 4 * h, 4 * w
         self.gen, self.disc, self.vgg_loss = gen, disc, vgg_loss
@@ -321,8 +341,8 @@ class AdversarialTrainer:
         self.v_real = chain.VGGFeaturePlan(vparams, B, H, W, compute_dtype, need_input_grad=False)
         self.v_fake.run_packing()
         self.v_real.run_packing()                 # frozen weights: packed once
-        self.opt_g = FlatAdam(self.flat_g, lr=lr, shapes=[p.shape for p in gen.parameters()])
-        self.opt_d = FlatAdam(self.flat_d, lr=lr, shapes=[p.shape for p in disc.parameters()])
+        self.opt_g = _make_optimizer(optimizer, gen, self.flat_g, lr)
+        self.opt_d = _make_optimizer(optimizer, disc, self.flat_d, lr)
         self.acc = torch.zeros(4, dtype=torch.float32, device=dev)   # loss_disc, adv, l1, vgg
         self.grad_sync_g, self.grad_sync_d = grad_sync_g, grad_sync_d
         self.steps = 0
@@ -435,7 +455,8 @@ class AdversarialTrainer:
         n = gp.GY.t.numel()
         for src in (dg.gA[0], vf.gA[0]):           # dL/dfake = sum of the three branches
             L.check(lib.srx_axpby(gp.dt, src.ptr(), gp.GY.ptr(), 1.0, 1.0, n, sp), "srx_axpby")
-        if self.grad_sync_g is None and self.step_in_backward and _backward_and_step(gp, self.opt_g):
+        if self.grad_sync_g is None and self.step_in_backward and isinstance(self.opt_g, FlatAdam) \
+                and _backward_and_step(gp, self.opt_g):
             pass                                     # Adam went out range by range beside backward
         else:
             exchanged = _backward_with_exchange(gp, self.grad_sync_g)

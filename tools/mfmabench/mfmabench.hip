@@ -1,6 +1,6 @@
 // Bare MFMA loops, one wave per SIMD on every CU: v_mfma_f32_32x32x16_bf16 against
 // v_mfma_f32_16x16x32_bf16 on random operands — FLOP/s, cycles per instruction and the clock the chip holds.
-// Build:  hipcc -O3 --offload-arch=gfx950 -mllvm -amdgpu-mfma-vgpr-form mfmabench.hip -o mfmabench
+// Build:  hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -mllvm -amdgpu-mfma-vgpr-form mfmabench.hip -o mfmabench
 // The flag matters: without it hipcc keeps the eight 4-register accumulators of the 16x16x32 loop in
 // AGPRs and rotates them through VGPRs every iteration (about sixty v_accvgpr_read / _write / _mov per
 // eight MFMAs), and the loop then measures those moves (23 cycles per instruction) instead of the matrix pipe.
