@@ -38,7 +38,8 @@ const char* srx_last_error(void);
 /* sizeof() of the ABI structs, for binding self-checks: 0 srx_conv_desc, 1 srx_wgrad_task,
  * 2 srx_wgrad_desc, 3 srx_pack_seg, 4 srx_pack_layer, 5 srx_unpack_item, 6 srx_sn_layer,
  * 7 srx_sn_bwd_layer, 8 srx_generic_args, 9 srx_op, 10 srx_tile, 11 srx_crop, 12 srx_rdb_desc,
- * 13 srx_adamw_tensor, 14 srx_adamw_chunk, 15 srx_adamw_group, 16 srx_adamw_desc; -1 for an unknown id. */
+ * 13 srx_adamw_tensor, 14 srx_adamw_chunk, 15 srx_adamw_group, 16 srx_adamw_desc,
+ * 17 srx_resnorm_desc; -1 for an unknown id. */
 int srx_sizeof(int which);
 /* Host-side self-check (no GPU call): kernel attributes such as the dynamic LDS limit are set
  * once per DEVICE a kernel is launched on, not once per process.  0 = ok.  No counterpart in the
@@ -418,6 +419,46 @@ int srx_adamw_moments_to8(const float* m, const float* v, void* m_code, void* v_
                           int64_t nblocks, void* stream);
 int srx_adamw_moments_from8(const void* m_code, const void* v_code, const float* m_scale, const float* v_scale,
                             float* m, float* v, int64_t nblocks, void* stream);
+
+/* ------------------------------------- norms around a gated residual branch */
+/* The reference's residual blocks add a branch scaled by a constant (x5 * 0.2 + x, esrgan/generator.py:23,37) and have
+ * no norm.  These are the same add with a norm over the channels after the branch, a learned gate on it, and the
+ * norm in front of the next branch, in one pass.  For every pixel (row), over its C channels:
+ *     a = N_post(f)      u = act(gate) * a      y = x + scale * u      h = N_pre(y)
+ *     N(z) = z / sqrt(mean z^2 + eps) * w + b  (kind 1)  or  (z - mean z) / sqrt(var z + eps) * w + b  (kind 2);
+ *     kind 0: a = f * w + b;  no h.
+ * w, b: fp32 [C] or NULL (1, 0).  act: the identity (0) or the sigmoid (1).  f == NULL: only h = N_pre(x).
+ * Statistics, products and sums are fp32; y and h are rounded once each.
+ * Layouts: SRX_RESNORM_PLANES, pixels contiguous [B][C][P] (a map of P pixels; *_stride = image stride), C <= 1024;
+ * SRX_RESNORM_ROWS, channels contiguous, row b * P + p at (b * P + p) * *_stride, C <= 16384. */
+#define SRX_RESNORM_PLANES 0
+#define SRX_RESNORM_ROWS 1
+typedef struct srx_resnorm_desc {
+  int32_t dtype, layout;
+  int32_t B, C, P;
+  int32_t post_kind, pre_kind;         /* 0 none, 1 root mean square, 2 mean and variance        */
+  int32_t gate_mode;                   /* 0 none, 1 fp32 [C], 2 fp32 [B][C], 3 a tensor like f    */
+  int32_t gate_act;
+  float scale, post_eps, pre_eps;
+  const void* x; const void* f;
+  void* y; void* h;                    /* outputs of the forward pass; y is an input of the backward pass
+                                          (f == NULL: x as y)                                     */
+  const void* dy; const void* dh;      /* backward: gradients of y and h; NULL: zero              */
+  void* dx; void* df;                  /* backward, each NULL if not wanted                       */
+  const void* gate; void* dgate;       /* dgate as gate                                           */
+  int64_t x_stride, f_stride, y_stride, h_stride, dy_stride, dh_stride, dx_stride, df_stride, gate_stride, dgate_stride;
+  const float* w_post; const float* b_post; const float* w_pre; const float* b_pre;
+  float* dw_post; float* db_post; float* dw_pre; float* db_pre;      /* [C], written, NULL if not wanted  */
+  float* ws;                           /* backward: srx_resnorm_ws_floats(d) floats               */
+} srx_resnorm_desc;
+int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream);
+/* From dy and dh, in one pass over y, f, dy, dh (and a full gate) and a small join of the sums over pixels, which go
+ * in a fixed order (same inputs, same bits):  with n_y, n_f the normalised values and D the whole gradient of y,
+ *     D = dy + N_pre'(y)^T dh,  dx = D,  df = N_post'(f)^T (scale act(gate) D),  dgate = scale act'(gate) sum D a,
+ *     dw_pre = sum dh n_y, db_pre = sum dh, dw_post = sum scale act(gate) D n_f, db_post = sum scale act(gate) D. */
+int srx_resnorm_backward(const srx_resnorm_desc* d, void* stream);
+/* Floats of workspace for the backward pass of d (addresses and strides are not looked at); -1: d is refused. */
+int64_t srx_resnorm_ws_floats(const srx_resnorm_desc* d);
 
 /* -------------------------------------------------------- tiled inference */
 /* Tiling around the generator, reference inference.py:187-230 (_infer_tiled).

@@ -28,6 +28,8 @@ OP_RDB_BWD = 14
 vp, i32, i64, f32, f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_double
 
 ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_GROUPS = 256, 4096, 32
+RESNORM_PLANES, RESNORM_ROWS = 0, 1
+RESNORM_MAX_C = (1024, 16384)          # per layout
 
 
 class PackSeg(C.Structure):
@@ -124,6 +126,17 @@ class AdamwDesc(C.Structure):
                 ("partial", vp), ("norm", vp), ("grad_scale", f64), ("max_norm", f64)]
 
 
+class ResnormDesc(C.Structure):
+    _fields_ = [("dtype", i32), ("layout", i32), ("B", i32), ("C", i32), ("P", i32), ("post_kind", i32), ("pre_kind", i32),
+                ("gate_mode", i32), ("gate_act", i32), ("scale", f32), ("post_eps", f32), ("pre_eps", f32),
+                ("x", vp), ("f", vp), ("y", vp), ("h", vp), ("dy", vp), ("dh", vp), ("dx", vp), ("df", vp),
+                ("gate", vp), ("dgate", vp),
+                ("x_stride", i64), ("f_stride", i64), ("y_stride", i64), ("h_stride", i64), ("dy_stride", i64),
+                ("dh_stride", i64), ("dx_stride", i64), ("df_stride", i64), ("gate_stride", i64), ("dgate_stride", i64),
+                ("w_post", vp), ("b_post", vp), ("w_pre", vp), ("b_pre", vp),
+                ("dw_post", vp), ("db_post", vp), ("dw_pre", vp), ("db_pre", vp), ("ws", vp)]
+
+
 class _OpU(C.Union):
     _fields_ = [("conv", ConvDesc), ("wgrad", WgradDesc), ("g", GenericArgs), ("rdb", RdbDesc)]
 
@@ -171,6 +184,9 @@ _SIGS = {
     "srx_adamw_step": (C.c_int, [C.POINTER(AdamwDesc), vp]),
     "srx_adamw_moments_to8": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, vp]),
     "srx_adamw_moments_from8": (C.c_int, [vp, vp, vp, vp, vp, vp, i64, vp]),
+    "srx_resnorm_forward": (C.c_int, [C.POINTER(ResnormDesc), vp]),
+    "srx_resnorm_backward": (C.c_int, [C.POINTER(ResnormDesc), vp]),
+    "srx_resnorm_ws_floats": (i64, [C.POINTER(ResnormDesc)]),
     "srx_run_ops": (C.c_int, [vp, C.c_int, vp]),
     "srx_stream_create": (C.c_int, [C.c_int, C.POINTER(vp)]),
     "srx_stream_destroy": (C.c_int, [vp]),
@@ -200,7 +216,7 @@ def lib():
             fn.argtypes = args
         structs = (ConvDesc, WgradTask, WgradDesc, PackSeg, PackLayer, UnpackItem, SnLayer,
                    SnBwdLayer, GenericArgs, Op, Tile, Crop, RdbDesc,
-                   AdamwTensor, AdamwChunk, AdamwGroup, AdamwDesc)
+                   AdamwTensor, AdamwChunk, AdamwGroup, AdamwDesc, ResnormDesc)
         for i, st in enumerate(structs):
             if l.srx_sizeof(i) != C.sizeof(st):
                 raise RuntimeError(f"libsrx ABI mismatch: sizeof({st.__name__}) is {C.sizeof(st)} in "

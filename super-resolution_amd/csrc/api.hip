@@ -39,6 +39,7 @@ int srx_sizeof(int which) {
     case 14: return (int)sizeof(srx_adamw_chunk);
     case 15: return (int)sizeof(srx_adamw_group);
     case 16: return (int)sizeof(srx_adamw_desc);
+    case 17: return (int)sizeof(srx_resnorm_desc);
     default: return -1;
   }
 }
