@@ -430,7 +430,7 @@ int srx_adamw_moments_from8(const void* m_code, const void* v_code, const float*
  * w, b: fp32 [C] or NULL (1, 0).  act: the identity (0) or the sigmoid (1).  f == NULL: only h = N_pre(x).
  * Statistics, products and sums are fp32; y and h are rounded once each.
  * Layouts: SRX_RESNORM_PLANES, pixels contiguous [B][C][P] (a map of P pixels; *_stride = image stride), C <= 1024;
- * SRX_RESNORM_ROWS, channels contiguous, row b * P + p at (b * P + p) * *_stride, C <= 16384. */
+ * SRX_RESNORM_ROWS, channels contiguous, row b * P + p at (b * P + p) * *_stride, C <= 8192. */
 #define SRX_RESNORM_PLANES 0
 #define SRX_RESNORM_ROWS 1
 typedef struct srx_resnorm_desc {
@@ -441,8 +441,7 @@ typedef struct srx_resnorm_desc {
   int32_t gate_act;
   float scale, post_eps, pre_eps;
   const void* x; const void* f;
-  void* y; void* h;                    /* outputs of the forward pass; y is an input of the backward pass
-                                          (f == NULL: x as y)                                     */
+  void* y; void* h;                    /* outputs of the forward pass (the backward pass reads x and f)  */
   const void* dy; const void* dh;      /* backward: gradients of y and h; NULL: zero              */
   void* dx; void* df;                  /* backward, each NULL if not wanted                       */
   const void* gate; void* dgate;       /* dgate as gate                                           */
@@ -452,7 +451,7 @@ typedef struct srx_resnorm_desc {
   float* ws;                           /* backward: srx_resnorm_ws_floats(d) floats               */
 } srx_resnorm_desc;
 int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream);
-/* From dy and dh, in one pass over y, f, dy, dh (and a full gate) and a small join of the sums over pixels, which go
+/* From dy and dh, in one pass over x, f, dy, dh (and a full gate) and a small join of the sums over pixels, which go
  * in a fixed order (same inputs, same bits):  with n_y, n_f the normalised values and D the whole gradient of y,
  *     D = dy + N_pre'(y)^T dh,  dx = D,  df = N_post'(f)^T (scale act(gate) D),  dgate = scale act'(gate) sum D a,
  *     dw_pre = sum dh n_y, db_pre = sum dh, dw_post = sum scale act(gate) D n_f, db_post = sum scale act(gate) D. */

@@ -5,21 +5,22 @@
 //   rows   (channels contiguous): V neighbouring channels, K times, of ONE row; `lanes` threads share a row.
 //   planes (pixels contiguous):   V neighbouring pixels of K channels; `lanes` threads of a wave sit side by side
 //                                 along the pixels, the others hold other channels of the same pixels.
-// Every tensor is read once: statistics, norm and gradients come out of the registers, in fp32.  The sums over the pixels
-// (gradients of weights, biases and gates) stay in registers while a workgroup walks its share of the pixels; their
-// partial sums are joined by a second small kernel in a fixed order (no atomics: same inputs, same bits).
+// Every tensor is read once: statistics, norm and gradients come out of the registers, in fp32.  The backward pass takes
+// x and f and forms y again: the same traffic as reading y, and not y's rounding to bf16 (which would put 2^-9 of
+// error into every weight gradient).  The sums over the pixels (gradients of weights, biases and gates) stay in registers
+// while a workgroup walks its share of the pixels; their partial sums are joined by a second small kernel in a fixed
+// order (no atomics: same inputs, same bits).
 #include "srx_common.h"
 
 namespace {
 
-constexpr int MAX_THREADS = 1024;
 constexpr int MAX_Q = 2;          // quantities reduced together
 enum { KIND_NONE = 0, KIND_RMS = 1, KIND_LAYER = 2 };
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_IMAGE = 2, GATE_FULL = 3 };
 
 struct Args {
   srx_resnorm_desc d;
-  int lanes;            // rows: threads per row (a power of two); planes: lanes along the pixels (64, 32 or 16)
+  int lanes;            // rows: threads per row (a power of two); planes: lanes along the pixels (64 down to 4)
   int slices;           // shares of an image's pixels
   int64_t len;          // pixels of a share
   int64_t items;        // images * slices
@@ -28,98 +29,160 @@ struct Args {
   float* part_post;     // [workgroups or items][2][C]
 };
 
-template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T e[V]; };
-template <typename T, int V> __device__ __forceinline__ void load(const T* p, float* out) {
-  const Vec<T, V> t = *reinterpret_cast<const Vec<T, V>*>(p);
-#pragma unroll
-  for (int j = 0; j < V; ++j) out[j] = (float)t.e[j];
-}
-template <typename T, int V> __device__ __forceinline__ void store(T* p, const float* v) {
-  Vec<T, V> t;
-#pragma unroll
-  for (int j = 0; j < V; ++j) t.e[j] = (T)v[j];
-  *reinterpret_cast<Vec<T, V>*>(p) = t;
-}
+// V elements, at any address that is a multiple of the element's size: global memory takes wide accesses there (a row
+// of an odd number of channels, a map of an odd number of pixels), so there is no second, narrow form of the kernels.
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Vec { T e[V]; };
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
 
-template <typename T, bool ROWS, int K, int V> struct Thread {
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+// sum over the lanes whose numbers differ in the bits lo, 2 lo, ... hi / 2 (every lane gets it)
+__device__ __forceinline__ float lanes_sum(float v, int lo, int hi) {
+  if (lo <= 1 && hi > 1) v = dpp_add<0xB1>(v);          // quad_perm 1,0,3,2
+  if (lo <= 2 && hi > 2) v = dpp_add<0x4E>(v);          // quad_perm 2,3,0,1
+  if (lo <= 4 && hi > 4) v += __shfl_xor(v, 4, 64);
+  if (lo <= 8 && hi > 8) v = dpp_add<0x128>(v);         // row_ror 8
+  if (lo <= 16 && hi > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (lo <= 32 && hi > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+// UNI: all lanes of a wave hold the same channels (planes with 64 lanes along the pixels): weights in scalar registers
+template <typename T, bool ROWS, int K, int V, bool UNI> struct Thread {
   static constexpr int E = K * V;                     // elements of each tensor
   static constexpr int NP = ROWS ? 1 : V;             // pixels
   static constexpr int NW = ROWS ? E : K;             // channels
   static __device__ __forceinline__ constexpr int pix(int e) { return ROWS ? 0 : e % V; }
   static __device__ __forceinline__ constexpr int wi(int e) { return ROWS ? e : e / V; }
+  typedef Vec<T, V> Raw;
 
   const Args& a;
   float* lds;
   int round;
   int lane, wave, l, grp;     // rows: l = thread within the row, grp = row of the workgroup; planes: l = lane along the pixels
-  bool chan_ok[K];            // this k's channels exist
-  bool ok;                    // the row / the pixels exist
-  int64_t pixel;              // first pixel within the image
-  int64_t image;
+  int have;                   // elements of a vector that exist: planes, along the pixels; rows: 0 where the row does not exist
+  bool full;                  // every element of the wave exists
+  int64_t image, base;        // first pixel of the workgroup's tile within the image
 
   __device__ __forceinline__ Thread(const Args& a_, float* lds_) : a(a_), lds(lds_), round(0) {
     lane = threadIdx.x & 63;
-    wave = threadIdx.x >> 6;
-    if (ROWS) { l = threadIdx.x & (a.lanes - 1); grp = threadIdx.x / a.lanes; }
-    else { l = lane & (a.lanes - 1); grp = threadIdx.x / a.lanes; }
-#pragma unroll
-    for (int k = 0; k < K; ++k) chan_ok[k] = chan(k) < a.d.C;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    l = ROWS ? threadIdx.x & (a.lanes - 1) : lane & (a.lanes - 1);
+    grp = UNI ? wave : threadIdx.x / a.lanes;
   }
   __device__ __forceinline__ int chan(int k) const { return ROWS ? (k * a.lanes + l) * V : grp * K + k; }
+  // elements of step k that exist
+  __device__ __forceinline__ int exist(int k) const {
+    const int left = a.d.C - chan(k);
+    if (ROWS) return !have || left < 0 ? 0 : left < V ? left : V;
+    return left > 0 ? have : 0;
+  }
+  // whether an element's channel exists (its pixel need not)
+  __device__ __forceinline__ bool chan_ok(int e) const { return chan(e / V) + (ROWS ? e % V : 0) < a.d.C; }
   // pixels that a workgroup takes at a time
   __device__ __forceinline__ int tile() const { return ROWS ? (int)blockDim.x / a.lanes : a.lanes * V; }
-  __device__ __forceinline__ void at(int64_t img, int64_t base, int64_t end) {
+  __device__ __forceinline__ void at(int64_t img, int64_t base_, int64_t end) {
     image = img;
-    pixel = base + (ROWS ? grp : l * V);
-    ok = pixel < end;
+    base = base_;
+    const int64_t left = end - base - (ROWS ? grp : l * V);
+    have = left <= 0 ? 0 : ROWS || left >= V ? V : (int)left;
+    full = __all(have == V && (ROWS ? chan(K - 1) + V : chan(K - 1) + 1) <= a.d.C);
   }
-  // image / row stride -> offset of element 0 of step k
-  __device__ __forceinline__ int64_t offset(int64_t stride, int k) const {
-    return ROWS ? (image * a.P + pixel) * stride + chan(k) : image * stride + (int64_t)chan(k) * a.P + pixel;
+  // address of step 0, and elements from one step to the next: a uniform part and an offset within the workgroup's tile
+  template <typename P> __device__ __forceinline__ P* first(P* p, int64_t stride) const {
+    if (ROWS) return p + (image * a.P + base) * stride + ((int64_t)grp * stride + l * V);
+    if (UNI) return p + image * stride + (int64_t)(wave * K) * a.P + base;
+    return p + image * stride + base + ((int64_t)(grp * K) * a.P + l * V);
   }
-  __device__ __forceinline__ void read(const void* p, int64_t stride, float* z) const {
+  __device__ __forceinline__ int64_t step() const { return ROWS ? a.lanes * V : a.P; }
+  __device__ __forceinline__ void read(const void* p, int64_t stride, Raw* z) const {
+    const T* q = first(static_cast<const T*>(p), stride);
+    const unsigned off = UNI ? l * V : 0;
+    if (full) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) z[k] = *reinterpret_cast<const Raw*>(q + k * step() + off);
+      return;
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (ok && chan_ok[k]) load<T, V>(static_cast<const T*>(p) + offset(stride, k), z + k * V);
+      const T* w = q + k * step() + off;
+      const int n = exist(k);
+      if (n == V) z[k] = *reinterpret_cast<const Raw*>(w);
       else
 #pragma unroll
-        for (int j = 0; j < V; ++j) z[k * V + j] = 0.f;
+        for (int j = 0; j < V; ++j) z[k].e[j] = j < n ? w[j] : (T)0.f;
     }
   }
-  __device__ __forceinline__ void write(void* p, int64_t stride, const float* z) const {
+  __device__ __forceinline__ void write(void* p, int64_t stride, const float* v) const {
+    T* q = first(static_cast<T*>(p), stride);
+    const unsigned off = UNI ? l * V : 0;
+    if (full) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (ok && chan_ok[k]) store<T, V>(static_cast<T*>(p) + offset(stride, k), z + k * V);
+      for (int k = 0; k < K; ++k) {
+        Raw z;
+#pragma unroll
+        for (int j = 0; j < V; ++j) z.e[j] = (T)v[k * V + j];
+        *reinterpret_cast<Raw*>(q + k * step() + off) = z;
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      T* w = q + k * step() + off;
+      const int n = exist(k);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < n) w[j] = (T)v[k * V + j];
+    }
   }
   // per-channel fp32 values (NULL: `missing`); channels that do not exist get 0
-  __device__ __forceinline__ void weights(const float* w, float missing, float* out) const {
+  __device__ __forceinline__ float weight(const float* w, float missing, int i) const {
+    const int c = ROWS ? chan(i / V) + i % V : chan(i);
+    return c >= a.d.C ? 0.f : w ? w[c] : missing;
+  }
+  static __device__ __forceinline__ float uniform(float v) {
+    return UNI ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))) : v;
+  }
+  // the branch's factor and offset: u = gw n + gb (a full gate multiplies that per element)
+  __device__ __forceinline__ void branch(int64_t img, float* gw, float* gb) const {
+    const srx_resnorm_desc& d = a.d;
+    const float* gate = d.gate_mode == GATE_CHANNEL || d.gate_mode == GATE_IMAGE
+                            ? static_cast<const float*>(d.gate) + (d.gate_mode == GATE_IMAGE ? img * d.C : 0) : nullptr;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-      const int k = ROWS ? i / V : i, c = chan(k) + (ROWS ? i % V : 0);
-      out[i] = !chan_ok[k] ? 0.f : w ? w[c] : missing;
+      float G = weight(gate, 1.f, i);
+      if (gate && d.gate_act) G = sigmoid(G);
+      G *= d.scale;
+      gw[i] = uniform(G * weight(d.w_post, 1.f, i));
+      gb[i] = uniform(G * weight(d.b_post, 0.f, i));
     }
   }
   // sums over the channels: of Q quantities, one value for each of the thread's pixels
   template <int Q> __device__ __forceinline__ void reduce(float (&s)[Q][NP]) {
     static_assert(Q <= MAX_Q, "");
     const int lo = ROWS ? 1 : a.lanes, hi = ROWS ? (a.lanes < 64 ? a.lanes : 64) : 64;
-    for (int o = lo; o < hi; o <<= 1)
+    if (!UNI)
 #pragma unroll
       for (int q = 0; q < Q; ++q)
 #pragma unroll
-        for (int j = 0; j < NP; ++j) s[q][j] += __shfl_xor(s[q][j], o, 64);
+        for (int j = 0; j < NP; ++j) s[q][j] = lanes_sum(s[q][j], lo, hi);
     const int waves = ROWS ? a.lanes >> 6 : (int)blockDim.x >> 6;      // that share a pixel
     if (waves <= 1) return;
     // two buffers in turn: the barrier of one round keeps the next but one from overwriting what is still being read
-    const int per = ROWS ? 1 : a.lanes * NP, all = (int)blockDim.x >> 6;
-    float* buf = lds + (round & 1) * (all * MAX_Q * per);
-    const int slot = ROWS ? 0 : l * NP;
-    if (ROWS ? lane == 0 : lane < a.lanes)
+    const int per = (ROWS ? 1 : a.lanes) * Q * NP, all = (int)blockDim.x >> 6;
+    float* buf = lds + (round & 1) * (all * (ROWS ? 1 : a.lanes) * MAX_Q * NP) + (ROWS ? 0 : l * Q * NP);
+    if (ROWS ? lane == 0 : UNI || lane < a.lanes)
 #pragma unroll
       for (int q = 0; q < Q; ++q)
 #pragma unroll
-        for (int j = 0; j < NP; ++j) buf[(wave * Q + q) * per + slot + j] = s[q][j];
+        for (int j = 0; j < NP; ++j) buf[wave * per + q * NP + j] = s[q][j];
     __syncthreads();
     const int first = ROWS ? wave & ~(waves - 1) : 0;
 #pragma unroll
@@ -130,7 +193,7 @@ template <typename T, bool ROWS, int K, int V> struct Thread {
 #pragma unroll
       for (int q = 0; q < Q; ++q)
 #pragma unroll
-        for (int j = 0; j < NP; ++j) s[q][j] += buf[(w * Q + q) * per + slot + j];
+        for (int j = 0; j < NP; ++j) s[q][j] += buf[w * per + q * NP + j];
     ++round;
   }
   // z -> (z - mean) / sqrt(var + eps) or z / sqrt(mean square + eps); returns the factor.  The variance is summed about the
@@ -144,9 +207,12 @@ template <typename T, bool ROWS, int K, int V> struct Thread {
 #pragma unroll
       for (int e = 0; e < E; ++e) s[0][pix(e)] += z[e];
       reduce<1>(s);
+      if (full)
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (chan_ok[e / V]) z[e] -= s[0][pix(e)] * inv;
+        for (int e = 0; e < E; ++e) z[e] -= s[0][pix(e)] * inv;
+      else
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[e] -= chan_ok(e) ? s[0][pix(e)] * inv : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < NP; ++j) s[0][j] = 0;
@@ -168,26 +234,26 @@ template <typename T, bool ROWS, int K, int V> struct Thread {
     for (int e = 0; e < E; ++e) { s[0][pix(e)] += dn[e] * n[e]; s[1][pix(e)] += dn[e]; }
     reduce<2>(s);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int j = pix(e);
-      dn[e] = r[j] * (dn[e] - n[e] * (s[0][j] * inv) - (kind == KIND_LAYER ? s[1][j] * inv : 0.f));
+    for (int j = 0; j < NP; ++j) {
+      s[0][j] *= inv;
+      s[1][j] = kind == KIND_LAYER ? s[1][j] * inv : 0.f;
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) dn[e] = r[pix(e)] * (dn[e] - n[e] * s[0][pix(e)] - s[1][pix(e)]);
   }
   // sum the thread's per-channel values over the workgroup and write them to out[C]
   __device__ __forceinline__ void flush(float* acc, float* out) {
     if (!ROWS) {
-      for (int o = 1; o < a.lanes; o <<= 1)
 #pragma unroll
-        for (int i = 0; i < NW; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+      for (int i = 0; i < NW; ++i) acc[i] = lanes_sum(acc[i], 1, a.lanes);
       if (l == 0)
 #pragma unroll
         for (int k = 0; k < K; ++k)
-          if (chan_ok[k]) out[chan(k)] = acc[k];
+          if (chan(k) < a.d.C) out[chan(k)] = acc[k];
       return;
     }
-    for (int o = a.lanes; o < 64; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < NW; ++i) acc[i] += __shfl_xor(acc[i], o, 64);
+    for (int i = 0; i < NW; ++i) acc[i] = lanes_sum(acc[i], a.lanes, 64);
     // waves that hold the same channels: every (lanes / 64)-th
     const int per_row = a.lanes > 64 ? a.lanes >> 6 : 1, waves = (int)blockDim.x >> 6;
     const bool first = wave < per_row && lane < a.lanes;
@@ -205,49 +271,51 @@ template <typename T, bool ROWS, int K, int V> struct Thread {
     }
     if (first)
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (chan_ok[k])
-#pragma unroll
-          for (int j = 0; j < V; ++j) out[chan(k) + j] = acc[k * V + j];
+      for (int i = 0; i < NW; ++i)
+        if (chan_ok(i)) out[chan(i / V) + i % V] = acc[i];
   }
 };
 
-template <typename T, bool ROWS, int K, int V, int THREADS>
+template <typename T, bool ROWS, int K, int V, bool UNI, bool FULL, int THREADS>
 __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
   extern __shared__ float lds[];
-  typedef Thread<T, ROWS, K, V> Th;
+  typedef Thread<T, ROWS, K, V, UNI> Th;
   Th t(a, lds);
   const srx_resnorm_desc& d = a.d;
-  float w2[Th::NW], b2[Th::NW], g[Th::NW], w1[Th::NW], b1[Th::NW];
-  if (d.f) { t.weights(d.w_post, 1.f, w2); t.weights(d.b_post, 0.f, b2); }
-  if (d.pre_kind) { t.weights(d.w_pre, 1.f, w1); t.weights(d.b_pre, 0.f, b1); }
+  float gw[Th::NW], gb[Th::NW], w1[Th::NW], b1[Th::NW];
+  if (d.pre_kind)
+#pragma unroll
+    for (int i = 0; i < Th::NW; ++i) { w1[i] = Th::uniform(t.weight(d.w_pre, 1.f, i)); b1[i] = Th::uniform(t.weight(d.b_pre, 0.f, i)); }
+  if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0, gw, gb);
   for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
     const int64_t img = item / a.slices, lo = item % a.slices * a.len;
     const int64_t hi = lo + a.len < a.P ? lo + a.len : a.P;
-    if (d.f && d.gate_mode != GATE_FULL) {
-      t.weights(d.gate_mode == GATE_NONE ? nullptr : static_cast<const float*>(d.gate) + (d.gate_mode == GATE_IMAGE ? img * d.C : 0), 1.f, g);
-#pragma unroll
-      for (int i = 0; i < Th::NW; ++i) g[i] = d.scale * (d.gate_mode && d.gate_act ? sigmoid(g[i]) : g[i]);
-    }
+    if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img, gw, gb);
     for (int64_t base = lo; base < hi; base += t.tile()) {
       t.at(img, base, hi);
+      typename Th::Raw xr[K], fr[K], qr[K];
+      t.read(d.x, d.x_stride, xr);
+      if (d.f) t.read(d.f, d.f_stride, fr);
+      if (FULL) t.read(d.gate, d.gate_stride, qr);
       float y[Th::E], r[Th::NP];
-      t.read(d.x, d.x_stride, y);
+#pragma unroll
+      for (int e = 0; e < Th::E; ++e) y[e] = (float)xr[e / V].e[e % V];
       if (d.f) {
         float n[Th::E];
-        t.read(d.f, d.f_stride, n);
-        if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r);
-        if (d.gate_mode == GATE_FULL) {
-          float q[Th::E];
-          t.read(d.gate, d.gate_stride, q);
 #pragma unroll
-          for (int e = 0; e < Th::E; ++e)
-            y[e] += d.scale * (d.gate_act ? sigmoid(q[e]) : q[e]) * (n[e] * w2[Th::wi(e)] + b2[Th::wi(e)]);
+        for (int e = 0; e < Th::E; ++e) n[e] = (float)fr[e / V].e[e % V];
+        if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r);
+        if (FULL) {
+#pragma unroll
+          for (int e = 0; e < Th::E; ++e) {
+            const float q = (float)qr[e / V].e[e % V];
+            y[e] += (d.gate_act ? sigmoid(q) : q) * (gw[Th::wi(e)] * n[e] + gb[Th::wi(e)]);
+          }
         } else {
 #pragma unroll
-          for (int e = 0; e < Th::E; ++e) y[e] += g[Th::wi(e)] * (n[e] * w2[Th::wi(e)] + b2[Th::wi(e)]);
+          for (int e = 0; e < Th::E; ++e) y[e] += gw[Th::wi(e)] * n[e] + gb[Th::wi(e)];
         }
-        if (d.y) t.write(d.y, d.y_stride, y);
+        t.write(d.y, d.y_stride, y);
       }
       if (d.pre_kind) {
         t.normalise(y, d.pre_kind, d.pre_eps, r);
@@ -262,70 +330,86 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
 // With D the gradient of y, the branch's per-channel sums are
 //   d w_post = s sum G D n,   d b_post = s sum G D,   d G = s sum D (w n + b),
 // and where G is the same for all pixels of an image (or is 1) all three follow from sum D n and sum D: two
-// accumulators a channel instead of three.  A full gate takes s G D in D's place and writes its own gradient.
-template <typename T, bool ROWS, int K, int V, int THREADS>
+// accumulators a channel instead of three.  A full gate takes G D in D's place and writes its own gradient.
+template <typename T, bool ROWS, int K, int V, bool UNI, bool FULL, int THREADS>
 __global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
   extern __shared__ float lds[];
-  typedef Thread<T, ROWS, K, V> Th;
+  typedef Thread<T, ROWS, K, V, UNI> Th;
   Th t(a, lds);
   const srx_resnorm_desc& d = a.d;
-  float w2[Th::NW], b2[Th::NW], g[Th::NW], w1[Th::NW];
+  float gw[Th::NW], gb[Th::NW], w1[Th::NW];
   float s_dhn[Th::NW] = {}, s_dh[Th::NW] = {}, s_dn[Th::NW] = {}, s_d[Th::NW] = {};
-  if (d.f) { t.weights(d.w_post, 1.f, w2); t.weights(d.b_post, 0.f, b2); }
-  if (d.dh) t.weights(d.w_pre, 1.f, w1);
+  if (d.dh)
+#pragma unroll
+    for (int i = 0; i < Th::NW; ++i) w1[i] = Th::uniform(t.weight(d.w_pre, 1.f, i));
+  if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0, gw, gb);
   for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
     const int64_t img = item / a.slices, lo = item % a.slices * a.len;
     const int64_t hi = lo + a.len < a.P ? lo + a.len : a.P;
-    if (d.f && d.gate_mode != GATE_FULL) {
-      t.weights(d.gate_mode == GATE_NONE ? nullptr : static_cast<const float*>(d.gate) + (d.gate_mode == GATE_IMAGE ? img * d.C : 0), 1.f, g);
-#pragma unroll
-      for (int i = 0; i < Th::NW; ++i) g[i] = d.scale * (d.gate_mode && d.gate_act ? sigmoid(g[i]) : g[i]);
-    }
+    if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img, gw, gb);
     for (int64_t base = lo; base < hi; base += t.tile()) {
       t.at(img, base, hi);
-      float D[Th::E], r[Th::NP];
-      if (d.dy) t.read(d.dy, d.dy_stride, D);
-      else
+      typename Th::Raw xr[K], fr[K], qr[K], dyr[K], dhr[K];
+      if (d.f) t.read(d.f, d.f_stride, fr);
+      if (d.dh) t.read(d.x, d.x_stride, xr);
+      if (FULL) t.read(d.gate, d.gate_stride, qr);
+      if (d.dh) t.read(d.dh, d.dh_stride, dhr);
+      if (d.dy) t.read(d.dy, d.dy_stride, dyr);
+      float D[Th::E], n[Th::E], r[Th::NP], r2[Th::NP];
+      if (d.f) {
 #pragma unroll
-        for (int e = 0; e < Th::E; ++e) D[e] = 0;
+        for (int e = 0; e < Th::E; ++e) n[e] = (float)fr[e / V].e[e % V];
+        if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r2);
+      }
+#pragma unroll
+      for (int e = 0; e < Th::E; ++e) D[e] = d.dy ? (float)dyr[e / V].e[e % V] : 0.f;
       if (d.dh) {
-        float n[Th::E], dn[Th::E];
-        t.read(d.y, d.y_stride, n);
-        t.read(d.dh, d.dh_stride, dn);
-        t.normalise(n, d.pre_kind, d.pre_eps, r);
+        float y[Th::E], dn[Th::E];
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) {
-          s_dhn[Th::wi(e)] += dn[e] * n[e];
-          s_dh[Th::wi(e)] += dn[e];
-          dn[e] *= w1[Th::wi(e)];
+          y[e] = (float)xr[e / V].e[e % V];
+          if (d.f) {
+            float u = gw[Th::wi(e)] * n[e] + gb[Th::wi(e)];
+            if (FULL) {
+              const float q = (float)qr[e / V].e[e % V];
+              u *= d.gate_act ? sigmoid(q) : q;
+            }
+            y[e] += u;
+          }
         }
-        t.normalise_back(dn, n, d.pre_kind, r);
+        t.normalise(y, d.pre_kind, d.pre_eps, r);
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) {
+          const float g = (float)dhr[e / V].e[e % V];
+          s_dhn[Th::wi(e)] += g * y[e];
+          s_dh[Th::wi(e)] += g;
+          dn[e] = g * w1[Th::wi(e)];
+        }
+        t.normalise_back(dn, y, d.pre_kind, r);
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) D[e] += dn[e];
       }
       if (d.dx) t.write(d.dx, d.dx_stride, D);
       if (d.f) {
-        float n[Th::E];
-        t.read(d.f, d.f_stride, n);
-        if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r);
-        if (d.gate_mode == GATE_FULL) {
-          float q[Th::E];
-          t.read(d.gate, d.gate_stride, q);
+        if (FULL) {
+          float dq[Th::E];
 #pragma unroll
           for (int e = 0; e < Th::E; ++e) {
-            const float G = d.gate_act ? sigmoid(q[e]) : q[e];
-            q[e] = d.scale * D[e] * (n[e] * w2[Th::wi(e)] + b2[Th::wi(e)]) * (d.gate_act ? G * (1.f - G) : 1.f);
-            D[e] *= d.scale * G;
+            const float q = (float)qr[e / V].e[e % V], G = d.gate_act ? sigmoid(q) : q;
+            dq[e] = D[e] * (gw[Th::wi(e)] * n[e] + gb[Th::wi(e)]) * (d.gate_act ? G * (1.f - G) : 1.f);
+            D[e] *= G;
           }
-          if (d.dgate) t.write(d.dgate, d.dgate_stride, q);
+          if (d.dgate) t.write(d.dgate, d.dgate_stride, dq);
         }
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) {
-          s_dn[Th::wi(e)] += D[e] * n[e];
-          s_d[Th::wi(e)] += D[e];
-          D[e] *= d.gate_mode == GATE_FULL ? w2[Th::wi(e)] : g[Th::wi(e)] * w2[Th::wi(e)];
+          // pixels that do not exist have D = 0 but for the offset that a mean takes off: they are left out here
+          const float De = ROWS || t.have == V || Th::pix(e) < t.have ? D[e] : 0.f;
+          s_dn[Th::wi(e)] += De * n[e];
+          s_d[Th::wi(e)] += De;
+          D[e] *= gw[Th::wi(e)];
         }
-        if (d.post_kind) t.normalise_back(D, n, d.post_kind, r);
+        if (d.post_kind) t.normalise_back(D, n, d.post_kind, r2);
         if (d.df) t.write(d.df, d.df_stride, D);
       }
     }
@@ -349,13 +433,14 @@ __global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
   }
 }
 
-// Joins the partial sums: 64 channels a workgroup, 16 threads a channel that take every 16th partial.
-constexpr int JOIN_X = 64, JOIN_Y = 16;
+// Joins the partial sums: 16 channels a workgroup, 64 threads a channel that take every 64th partial.
+constexpr int JOIN_X = 16, JOIN_Y = 64;
 __device__ __forceinline__ float join(float v, float (*lds)[JOIN_X]) {
   __syncthreads();
   lds[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
   float s = 0;
+#pragma unroll
   for (int i = 0; i < JOIN_Y; ++i) s += lds[i][threadIdx.x];
   return s;
 }
@@ -367,6 +452,7 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
   if (d.dh && (d.dw_pre || d.db_pre)) {
     float sn = 0, s = 0;
     if (ok)
+#pragma unroll 4
       for (int i = threadIdx.y; i < workgroups; i += JOIN_Y) {
         sn += a.part_pre[(int64_t)i * 2 * d.C + c];
         s += a.part_pre[((int64_t)i * 2 + 1) * d.C + c];
@@ -387,6 +473,7 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
     if (ok)
       for (int i = threadIdx.y; i < images; i += JOIN_Y) {
         float sn = 0, s = 0;
+#pragma unroll 4
         for (int k = 0; k < a.slices; ++k) {
           const float* p = a.part_post + ((int64_t)i * a.slices + k) * 2 * d.C + c;
           sn += p[0];
@@ -401,18 +488,17 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
     db = join(db, lds);
   } else {
     if (ok)
+#pragma unroll 4
       for (int i = threadIdx.y; i < workgroups; i += JOIN_Y) {
         dw += a.part_post[(int64_t)i * 2 * d.C + c];
         db += a.part_post[((int64_t)i * 2 + 1) * d.C + c];
       }
     dw = join(dw, lds);
     db = join(db, lds);
-    if (d.gate_mode != GATE_FULL) {
-      const float q = gate && ok ? gate[c] : 1.f, G = gate && d.gate_act ? sigmoid(q) : q;
-      if (dgate && ok && threadIdx.y == 0) dgate[c] = d.scale * (w * dw + b * db) * (d.gate_act ? G * (1.f - G) : 1.f);
-      dw *= d.scale * G;
-      db *= d.scale * G;
-    }
+    const float q = gate && ok ? gate[c] : 1.f, G = gate && d.gate_act ? sigmoid(q) : q;
+    if (dgate && ok && threadIdx.y == 0) dgate[c] = d.scale * (w * dw + b * db) * (d.gate_act ? G * (1.f - G) : 1.f);
+    dw *= d.scale * G;
+    db *= d.scale * G;
   }
   if (ok && threadIdx.y == 0) {
     if (d.dw_post) d.dw_post[c] = dw;
@@ -423,12 +509,14 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
 // ------------------------------------------------------------------------------------------------ host side
 struct Plan {
   Args a;
-  int threads, workgroups, v, images;
+  int threads, workgroups, images;
+  int elems;               // rows: elements a thread holds
   int lds_bytes;
 };
 
-constexpr int KV = 16;            // elements of a tensor that a thread holds
-constexpr int MAX_ROWS_C = KV * MAX_THREADS, MAX_PLANES_C = KV * MAX_THREADS / 16;
+constexpr int PLANES_K = 8, PLANES_V = 2;
+constexpr int MAX_THREADS = 512;
+constexpr int MAX_ROWS_C = 16 * MAX_THREADS, MAX_PLANES_C = 1024;
 
 int pow2_at_least(int64_t n) {
   int p = 1;
@@ -437,26 +525,25 @@ int pow2_at_least(int64_t n) {
 }
 
 // The decomposition of a call: workspace size and launch use the same one.
-void make_plan(const srx_resnorm_desc& d, int backward, bool vector, Plan& p) {
+void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
   const bool rows = d.layout == SRX_RESNORM_ROWS;
   p.a.d = d;
-  int tile;
-  if (rows) {
-    p.v = vector ? (d.dtype == SRX_BF16 ? 8 : 4) : 1;
-    p.a.lanes = pow2_at_least((d.C + KV - 1) / KV);
-    p.threads = p.a.lanes > 256 ? p.a.lanes : 256;
-    tile = p.threads / p.a.lanes;
-  } else {
-    p.v = vector ? 2 : 1;
-    const int k = KV / p.v;
-    const int groups = (d.C + k - 1) / k;
-    p.a.lanes = groups <= 16 ? 64 : groups <= 32 ? 32 : 16;
-    p.threads = 64 * ((groups * p.a.lanes + 63) / 64);
-    tile = p.a.lanes * p.v;
-  }
   const bool image_gate = d.f && d.gate_mode == GATE_IMAGE;
   p.images = rows && !image_gate ? 1 : d.B;
   p.a.P = rows && !image_gate ? (int64_t)d.B * d.P : d.P;
+  int tile;
+  if (rows) {
+    p.elems = d.C <= 512 ? 8 : 16;
+    p.a.lanes = pow2_at_least((d.C + p.elems - 1) / p.elems);
+    p.threads = p.a.lanes > 256 ? p.a.lanes : 256;
+    tile = p.threads / p.a.lanes;
+  } else {
+    const int groups = (d.C + PLANES_K - 1) / PLANES_K;
+    p.a.lanes = 64;
+    while (groups * p.a.lanes > MAX_THREADS) p.a.lanes /= 2;
+    p.threads = 64 * ((groups * p.a.lanes + 63) / 64);
+    tile = p.a.lanes * PLANES_V;
+  }
   const int64_t tiles = (p.a.P + tile - 1) / tile;
   const int64_t target = backward ? 512 : 4096;
   int64_t s = p.images > 0 ? (target + p.images - 1) / p.images : 1;
@@ -468,26 +555,9 @@ void make_plan(const srx_resnorm_desc& d, int backward, bool vector, Plan& p) {
   p.a.items = p.a.P > 0 ? (int64_t)p.images * p.a.slices : 0;
   p.workgroups = (int)(p.a.items < target ? p.a.items : target);
   const int waves = p.threads / 64;
-  const int np = rows ? 1 : p.v;
-  int bytes = 2 * waves * MAX_Q * (rows ? 1 : p.a.lanes * np) * 4;            // two buffers; at most 32 KB
-  if (backward && rows && p.threads == 256 && bytes < waves * KV * 64 * 4) bytes = waves * KV * 64 * 4;     // flush: 16 KB
+  int bytes = 2 * waves * MAX_Q * (rows ? 1 : p.a.lanes * PLANES_V) * 4;            // two buffers; at most 32 KB
+  if (backward && rows && p.threads == 256 && bytes < waves * p.elems * 64 * 4) bytes = waves * p.elems * 64 * 4;     // flush: 16 KB
   p.lds_bytes = bytes;
-}
-
-// Vector accesses need every tensor's elements to line up: channels (rows) or pixels (planes) a multiple of the vector, and
-// strides and addresses too.
-bool can_vector(const srx_resnorm_desc& d) {
-  const bool rows = d.layout == SRX_RESNORM_ROWS;
-  const int v = rows ? (d.dtype == SRX_BF16 ? 8 : 4) : 2;
-  const int esize = d.dtype == SRX_BF16 ? 2 : 4;
-  if ((rows ? d.C : d.P) % v || (!rows && d.C > MAX_PLANES_C / v)) return false;
-  const void* ptrs[] = {d.x, d.f, d.y, d.h, d.dy, d.dh, d.dx, d.df, d.gate_mode == GATE_FULL ? d.gate : nullptr,
-                        d.gate_mode == GATE_FULL ? d.dgate : nullptr};
-  const int64_t strides[] = {d.x_stride, d.f_stride, d.y_stride, d.h_stride, d.dy_stride, d.dh_stride, d.dx_stride, d.df_stride,
-                             d.gate_stride, d.dgate_stride};
-  for (int i = 0; i < 10; ++i)
-    if (ptrs[i] && ((uintptr_t)ptrs[i] % (v * esize) || strides[i] % v)) return false;
-  return true;
 }
 
 int check(const char* what, const srx_resnorm_desc* d) {
@@ -519,24 +589,23 @@ int check(const char* what, const srx_resnorm_desc* d) {
   return SRX_OK;
 }
 
-template <typename T, bool ROWS, int K, int V, int THREADS> int launch_with(const Plan& p, int backward, hipStream_t s) {
+template <typename T, bool ROWS, int K, int V, bool UNI, bool FULL> int launch_with(const Plan& p, int backward, hipStream_t s) {
   if (backward)
-    hipLaunchKernelGGL((resnorm_bwd_kernel<T, ROWS, K, V, THREADS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
+    hipLaunchKernelGGL((resnorm_bwd_kernel<T, ROWS, K, V, UNI, FULL, MAX_THREADS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
   else
-    hipLaunchKernelGGL((resnorm_fwd_kernel<T, ROWS, K, V, THREADS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
+    hipLaunchKernelGGL((resnorm_fwd_kernel<T, ROWS, K, V, UNI, FULL, MAX_THREADS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
   return srx_check_launch(backward ? "resnorm_bwd" : "resnorm_fwd");
 }
-
-template <typename T, bool ROWS, int K, int V> int launch(const Plan& p, int backward, hipStream_t s) {
-  return p.threads <= 256 ? launch_with<T, ROWS, K, V, 256>(p, backward, s)
-         : p.threads <= 512 ? launch_with<T, ROWS, K, V, 512>(p, backward, s) : launch_with<T, ROWS, K, V, 1024>(p, backward, s);
+template <typename T, bool ROWS, int K, int V, bool UNI> int launch(const Plan& p, int backward, hipStream_t s) {
+  return p.a.d.gate_mode == GATE_FULL ? launch_with<T, ROWS, K, V, UNI, true>(p, backward, s) : launch_with<T, ROWS, K, V, UNI, false>(p, backward, s);
 }
 
 template <typename T> int dispatch(const Plan& p, int backward, hipStream_t s) {
-  constexpr int VR = sizeof(T) == 2 ? 8 : 4;
+  constexpr int V = 16 / sizeof(T);
   if (p.a.d.layout == SRX_RESNORM_ROWS)
-    return p.v == 1 ? launch<T, true, KV, 1>(p, backward, s) : launch<T, true, KV / VR, VR>(p, backward, s);
-  return p.v == 1 ? launch<T, false, KV, 1>(p, backward, s) : launch<T, false, KV / 2, 2>(p, backward, s);
+    return p.elems == 8 ? launch<T, true, 8 / V, V, false>(p, backward, s) : launch<T, true, 16 / V, V, false>(p, backward, s);
+  return p.a.lanes == 64 ? launch<T, false, PLANES_K, PLANES_V, true>(p, backward, s)
+                         : launch<T, false, PLANES_K, PLANES_V, false>(p, backward, s);
 }
 
 }  // namespace
@@ -545,11 +614,9 @@ extern "C" {
 
 int64_t srx_resnorm_ws_floats(const srx_resnorm_desc* d) {
   if (check("srx_resnorm_ws_floats", d)) return -1;
-  Plan p = {}, q = {};
-  make_plan(*d, 1, true, p);
-  make_plan(*d, 1, false, q);
-  const int64_t items = p.a.items > q.a.items ? p.a.items : q.a.items, wgs = p.workgroups > q.workgroups ? p.workgroups : q.workgroups;
-  return 2 * (int64_t)d->C * (wgs + (d->f && d->gate_mode == GATE_IMAGE ? items : wgs)) + 1;
+  Plan p = {};
+  make_plan(*d, 1, p);
+  return 2 * (int64_t)d->C * (p.workgroups + (d->f && d->gate_mode == GATE_IMAGE ? p.a.items : p.workgroups)) + 1;
 }
 
 int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream) {
@@ -557,7 +624,7 @@ int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream) {
   if ((int64_t)d->B * d->P == 0) return SRX_OK;
   SRX_CHECK_ARG(d->x && (!d->f || d->y) && (!d->pre_kind || d->h), "srx_resnorm_forward: null tensor");
   Plan p = {};
-  make_plan(*d, 0, can_vector(*d), p);
+  make_plan(*d, 0, p);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return d->dtype == SRX_BF16 ? dispatch<bf16>(p, 0, s) : dispatch<float>(p, 0, s);
 }
@@ -566,10 +633,10 @@ int srx_resnorm_backward(const srx_resnorm_desc* d, void* stream) {
   if (int rc = check("srx_resnorm_backward", d)) return rc;
   const bool empty = (int64_t)d->B * d->P == 0;
   SRX_CHECK_ARG(empty || d->dy || d->dh, "srx_resnorm_backward: neither dy nor dh");
-  SRX_CHECK_ARG(!d->dh || (d->pre_kind && (d->y || empty)), "srx_resnorm_backward: dh needs the norm before the next branch, and y");
+  SRX_CHECK_ARG(!d->dh || (d->pre_kind && (d->x || empty)), "srx_resnorm_backward: dh needs the norm before the next branch, and x");
   SRX_CHECK_ARG(empty || d->ws, "srx_resnorm_backward: null workspace");
   Plan p = {};
-  make_plan(*d, 1, can_vector(*d), p);
+  make_plan(*d, 1, p);
   if (empty) p.a.slices = 0;            // the gradients of weights and gates are zeros
   p.a.part_pre = d->ws;
   p.a.part_post = d->ws + 2 * (int64_t)d->C * p.workgroups;

@@ -10,7 +10,7 @@ branch, in one pass over the data, forward and backward::
 ``GatedResidualStack`` chains branches (this package's dense blocks, or any module that keeps its input's shape).
 
 Tensors: float32 or bfloat16 on a GPU, channels at dim 1 (``[B, C, ...]`` maps, ``channel_dim=1``) or last (tokens,
-``channel_dim=-1``); at most 1024 channels in maps, 16384 in channels-last tensors.  Memory order is kept: a
+``channel_dim=-1``); at most 1024 channels in maps, 8192 in channels-last tensors.  Memory order is kept: a
 channels-last map gives channels-last results.  Statistics and sums are float32 whatever the type.
 """
 from __future__ import annotations
@@ -196,14 +196,14 @@ class _ResNormFn(torch.autograd.Function):
         y, h = call.forward(x, f, gate, w_post, b_post, w_pre, b_pre)
         ctx.call = call
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if f is None else y if h is not None else None, f, gate, w_post, b_post, w_pre, b_pre)
+        ctx.save_for_backward(x if h is not None else None, f, gate, w_post, b_post, w_pre, b_pre)
         return h if f is None else y if h is None else (y, h)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         call, geo = ctx.call, ctx.call.geo
-        y, f, gate, w_post, b_post, w_pre, b_pre = ctx.saved_tensors
+        x, f, gate, w_post, b_post, w_pre, b_pre = ctx.saved_tensors
         dy = grads[0] if call.branch else None
         dh = grads[-1] if call.desc.pre_kind else None
         if dy is None and dh is None:
@@ -229,14 +229,9 @@ class _ResNormFn(torch.autograd.Function):
             if need:
                 out[at] = new(name, vec())
         if nf or ng or nwp or nbp or dh is not None:
-            call.put(d, keep, "y", y if dh is not None else None)
-            # the branch's part is left out where nothing of it is wanted
-            branch = nf or ng or nwp or nbp
-            if branch:
-                call.put(d, keep, "f", f)
-            call.common(d, keep, gate if branch else None, w_post, b_post, w_pre, b_pre)
-            if not branch:
-                d.post_kind = d.gate_mode = 0
+            call.put(d, keep, "x", x if dh is not None else None)
+            call.put(d, keep, "f", f)                 # y is formed again from x and f
+            call.common(d, keep, gate, w_post, b_post, w_pre, b_pre)
             if dh is None:
                 d.pre_kind = 0
             call.put(d, keep, "dy", dy)

@@ -20,7 +20,7 @@ def _desc(L, **kw):
 
 REFUSED = [
     (dict(dtype=3), b"dtype"), (dict(layout=2), b"layout"), (dict(C=0), b"sizes"), (dict(B=-1), b"sizes"), (dict(P=-1), b"sizes"),
-    (dict(C=1025), b"at most 1024"), (dict(layout=1, C=16385), b"at most 16384"), (dict(post_kind=3), b"norm kind"),
+    (dict(C=1025), b"at most 1024"), (dict(layout=1, C=8193), b"at most 8192"), (dict(post_kind=3), b"norm kind"),
     (dict(pre_kind=-1), b"norm kind"), (dict(gate_mode=4), b"gate mode"), (dict(gate_act=2), b"gate mode"),
     (dict(pre_eps=0.0), b"eps"), (dict(post_eps=float("nan")), b"eps"), (dict(f=None), b"without a branch"),
     (dict(f=None, post_kind=0, gate_mode=0, pre_kind=0), b"neither"), (dict(gate=None), b"null gate"),
@@ -35,7 +35,7 @@ def test_forward_refusals(kw, msg):
     assert msg in L.lib().srx_last_error(), L.lib().srx_last_error()
 
 
-@pytest.mark.parametrize("kw,msg", REFUSED + [(dict(), b"neither dy nor dh"), (dict(dh=256, y=None), b"and y"),
+@pytest.mark.parametrize("kw,msg", REFUSED + [(dict(), b"neither dy nor dh"), (dict(dh=256, x=None), b"and x"),
                                               (dict(dh=256, pre_kind=0), b"needs the norm"), (dict(dy=256), b"workspace"),
                                               (dict(dy=256, ws=256, dx=256, dx_stride=5), b"stride 5")])
 def test_backward_refusals(kw, msg):
