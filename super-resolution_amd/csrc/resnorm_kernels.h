@@ -1,0 +1,622 @@
+// Norms over the channels before and after a residual branch, fused with the branch's gate, the residual scale and the
+// residual add (include/srx.h, srx_resnorm_forward / _backward, has the formulas): the kernels, included by one translation
+// unit per element type.
+//
+// One kernel body serves both layouts.  A thread holds K x V elements of each tensor in registers:
+//   rows   (channels contiguous): V neighbouring channels, K times, of ONE row; `lanes` threads share a row.
+//   planes (pixels contiguous):   V neighbouring pixels of K channels; `lanes` threads of a wave sit side by side
+//                                 along the pixels, the others hold other channels of the same pixels.
+// Every tensor is read once: statistics, norm and gradients come out of the registers, in fp32.  The backward pass takes
+// x and f and forms y again: the same traffic as reading y, and not y's rounding to bf16 (which would put 2^-9 of
+// error into every weight gradient).  The sums over the pixels (gradients of weights, biases and gates) stay in registers
+// while a workgroup walks its share of the pixels; their partial sums are joined by a second small kernel in a fixed
+// order (no atomics: same inputs, same bits).
+#pragma once
+#include <type_traits>
+#include "srx_common.h"
+
+namespace resnorm {
+
+constexpr int MAX_Q = 2;          // quantities reduced together
+constexpr int THREADS = 512;      // most threads of a workgroup
+enum { KIND_NONE = 0, KIND_RMS = 1, KIND_LAYER = 2 };
+enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_IMAGE = 2, GATE_FULL = 3 };
+
+struct Args {
+  srx_resnorm_desc d;
+  int lanes;            // rows: threads per row (a power of two); planes: lanes along the pixels (64 down to 4)
+  int slices;           // shares of an image's pixels
+  int items;            // images * slices
+  int64_t len;          // pixels of a share
+  int64_t P;            // pixels of an "image" (rows without per-image gate: all rows are one image)
+  float* part_pre;      // [workgroups][2][C]
+  float* part_post;     // [workgroups or items][2][C]
+};
+struct Plan {
+  Args a;
+  int threads, workgroups, images;
+  int elems;               // rows: elements a thread holds
+  int lds_bytes;
+};
+constexpr int PLANES_K = 8, PLANES_V = 2;
+int launch_bf16(const Plan& p, int backward, hipStream_t s);
+int launch_f32(const Plan& p, int backward, hipStream_t s);
+
+// V elements, at any address that is a multiple of the element's size: global memory takes wide accesses there (a row
+// of an odd number of channels, a map of an odd number of pixels), so there is no second, narrow form of the kernels.
+// Kept as 32-bit words: the compiler would give every bf16 element a register of its own.
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Vec { uint32_t w[V * sizeof(T) / 4]; };
+template <> struct Vec<bf16, 1> { uint16_t w; };
+template <int V> __device__ __forceinline__ float element(const Vec<float, V>& z, int j) { return __uint_as_float(z.w[j]); }
+template <int V> __device__ __forceinline__ float element(const Vec<bf16, V>& z, int j) {
+  if constexpr (V == 1) return __uint_as_float((uint32_t)z.w << 16);
+  else return __uint_as_float(j & 1 ? z.w[j / 2] & 0xFFFF0000u : z.w[j / 2] << 16);
+}
+// zeros in place of the first n elements
+template <int V> __device__ __forceinline__ void drop(Vec<float, V>& z, int n) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) z.w[j] = j < n ? 0u : z.w[j];
+}
+template <int V> __device__ __forceinline__ void drop(Vec<bf16, V>& z, int n) {
+  if constexpr (V == 1) z.w = n > 0 ? 0 : z.w;
+  else
+#pragma unroll
+    for (int j = 0; j < V; j += 2) z.w[j / 2] = j + 1 < n ? 0u : j < n ? z.w[j / 2] & 0xFFFF0000u : z.w[j / 2];
+}
+template <int V> __device__ __forceinline__ Vec<float, V> packed(const float* v, const float*) {
+  Vec<float, V> z;
+#pragma unroll
+  for (int j = 0; j < V; ++j) z.w[j] = __float_as_uint(v[j]);
+  return z;
+}
+template <int V> __device__ __forceinline__ Vec<bf16, V> packed(const float* v, const bf16*) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  Vec<bf16, V> z;
+  if constexpr (V == 1) z.w = __builtin_bit_cast(uint16_t, (bf16)v[0]);
+  else
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const bf16x2 p = {(bf16)v[j], (bf16)v[j + 1]};
+      z.w[j / 2] = __builtin_bit_cast(uint32_t, p);
+    }
+  return z;
+}
+__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
+
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+// sums over the lanes whose numbers differ in the bits lo, 2 lo, ... hi / 2 (every lane gets them)
+template <int N> __device__ __forceinline__ void lanes_sum(float* v, int lo, int hi) {
+  if (lo <= 1 && hi > 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = dpp_add<0xB1>(v[i]);          // quad_perm 1,0,3,2
+  if (lo <= 2 && hi > 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = dpp_add<0x4E>(v[i]);          // quad_perm 2,3,0,1
+  if (lo <= 4 && hi > 4) {
+    if (lo <= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = dpp_add<0x141>(v[i]);       // row_half_mirror: lane ^ 7, and quads are uniform by now
+    else
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], 4, 64);
+  }
+  if (lo <= 8 && hi > 8)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = dpp_add<0x128>(v[i]);         // row_ror 8
+  if (lo <= 16 && hi > 16)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+  if (lo <= 32 && hi > 32)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+}
+
+// Every load is a whole vector that lies inside the tensor, without a branch: one that would pass the end (of a row; of
+// a plane; a row or channel that does not exist) starts earlier, and the elements in front of the thread's own, `dup` of
+// them, are zeros from then on.  BIAS: some norm has a bias (else: no offsets, and no sums for them).
+// UNI (planes with 64 lanes along the pixels): a wave's lanes hold the same channels, so that channels, their addresses
+// and their weights are scalars.
+template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Thread {
+  static constexpr int E = K * V;                     // elements of each tensor
+  static constexpr int NP = ROWS ? 1 : V;             // pixels
+  static constexpr int NW = ROWS ? E : K;             // channels
+  static constexpr int NL = ROWS ? E : 1;             // channels whose weights a thread keeps (planes: they lie in LDS)
+  static __device__ __forceinline__ constexpr int pix(int e) { return ROWS ? 0 : e % V; }
+  static __device__ __forceinline__ constexpr int wi(int e) { return ROWS ? e : e / V; }
+  typedef Vec<T, V> Raw;
+
+  const Args& a;
+  float* lds;                 // reductions
+  float* lw;                  // planes: weights by channel: gw, gb, w1, b1 (BIAS) or gw, w1
+  int round;
+  int lane, wave, l;          // l = thread within the row / lane along the pixels
+  int grp;                    // the thread's row of the workgroup / group of K channels
+  int cb;                     // planes: first channel read (64 lanes: the group's own; else as a vector's, all K exist)
+  int rdup[ROWS ? K : 1];     // rows: elements of step k that are not the thread's; planes: channels of the group that are not
+  int pdup;                   // planes: pixels that are not the lane's; rows: V where there is no such row
+  bool cfull, full;           // nothing is dropped in this wave: of the channels; at all
+  unsigned off;               // planes: bytes from `base` (and the wave's channel, if it has one) to the lane's first element
+  int64_t row;                // rows: the thread's row
+  int64_t image, base;        // first pixel of the workgroup's tile within the image
+  float gw_[NL], gb_[NL], w1_[NL], b1_[NL];
+
+  __device__ __forceinline__ Thread(const Args& a_, float* lds_) : a(a_), lds(lds_), round(0) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    l = UNI ? lane : threadIdx.x & (a.lanes - 1);
+    grp = UNI ? wave : threadIdx.x / a.lanes;
+    bool ok = true;
+    if (ROWS) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int over = (k * a.lanes + l) * V - (a.d.C - V);
+        rdup[k] = over < 0 ? 0 : over < V ? over : V;
+        ok = ok && over <= 0;
+      }
+    } else {
+      const int last = a.d.C - K;
+      cb = UNI || grp * K < last ? grp * K : last;
+      rdup[0] = grp * K - cb;
+      ok = cb + K <= a.d.C && rdup[0] == 0;
+    }
+    cfull = __all(ok);
+    lw = lds + 2 * (int)(blockDim.x >> 6) * MAX_Q * (ROWS ? 1 : lanes() * V);
+  }
+  __device__ __forceinline__ int lanes() const { return UNI ? 64 : a.lanes; }
+  // first channel of step k
+  __device__ __forceinline__ int ch(int k) const {
+    if (ROWS) {
+      const int c = (k * a.lanes + l) * V;
+      return c < a.d.C - V ? c : a.d.C - V;
+    }
+    return !UNI ? cb + k : cb + k < a.d.C ? cb + k : a.d.C - 1;
+  }
+  // elements of step k that are not the thread's because of its channels
+  __device__ __forceinline__ int cdup(int k) const { return ROWS ? rdup[k % (ROWS ? K : 1)] : (UNI ? cb + k >= a.d.C : k < rdup[0]) ? V : 0; }
+  __device__ __forceinline__ int dropped(int k) const { return cdup(k) > pdup ? cdup(k) : pdup; }
+  // whether an element's channel is the thread's (its pixel need not be)
+  __device__ __forceinline__ bool chan_ok(int e) const { return ROWS ? e % V >= cdup(e / V) : cdup(e / V) == 0; }
+  __device__ __forceinline__ int chan(int e) const { return ch(e / V) + (ROWS ? e % V : 0); }
+  // pixels that a workgroup takes at a time
+  __device__ __forceinline__ int tile() const { return ROWS ? (int)blockDim.x / a.lanes : lanes() * V; }
+  __device__ __forceinline__ void at(int64_t img, int64_t base_, int64_t end) {
+    image = img;
+    base = base_;
+    const int64_t want = base + (ROWS ? grp : l * V), last = end - (ROWS ? 1 : V);
+    if (ROWS) {
+      row = image * a.P + (want < last ? want : last);
+      pdup = want > last ? V : 0;
+    } else {
+      // where less than a vector is left behind the tile's start, the tile starts earlier
+      const int64_t from = want < last ? want : last;
+      pdup = want - from < V ? (int)(want - from) : V;
+      if (base > last) base = last;
+      off = ((unsigned)(from - base) + (UNI ? 0u : (unsigned)cb * (unsigned)a.P)) * (unsigned)sizeof(T);
+    }
+    full = cfull && __all(pdup == 0);
+  }
+  template <typename P> __device__ __forceinline__ P* address(P* p, int64_t stride, int k) const {
+    if (ROWS) return p + row * stride + ch(k);
+    // a scalar base and 32 bits of bytes, in one register for all of the kernel's accesses
+    typedef typename std::conditional<std::is_const<P>::value, const char, char>::type Byte;
+    return reinterpret_cast<P*>(reinterpret_cast<Byte*>(p + (image * stride + base + (UNI ? ch(k) : k) * a.P)) + off);
+  }
+  __device__ __forceinline__ void read(const void* p, int64_t stride, Raw* z) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) z[k] = *reinterpret_cast<const Raw*>(address(static_cast<const T*>(p), stride, k));
+    if (!full)
+#pragma unroll
+      for (int k = 0; k < K; ++k) drop<V>(z[k], dropped(k));
+  }
+  __device__ __forceinline__ void write(void* p, int64_t stride, const float* v) const {
+    if (full) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        T* w = address(static_cast<T*>(p), stride, k);
+        *reinterpret_cast<Raw*>(w) = packed<V>(v + k * V, w);
+      }
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      T* w = address(static_cast<T*>(p), stride, k);
+      const int n = dropped(k);
+      if (n == 0) *reinterpret_cast<Raw*>(w) = packed<V>(v + k * V, w);
+      else if (n < V)
+#pragma unroll
+        for (int j = 1; j < V; ++j)
+          if (j >= n) w[j] = (T)v[k * V + j];
+    }
+  }
+
+  // ---- weights: the branch's factor and offset (u = gw n + gb; a full gate multiplies that per element) and the norm's after it
+  template <int N> __device__ __forceinline__ static void weights(const float* w, float missing, int c, float* out) {
+    if (w) {
+      const Vec<float, N> z = *reinterpret_cast<const Vec<float, N>*>(w + c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) out[j] = element<N>(z, j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) out[j] = missing;
+    }
+  }
+  // of N neighbouring channels
+  template <int N> __device__ __forceinline__ void branch_weights(int64_t img, int c, float* gw, float* gb) const {
+    const srx_resnorm_desc& d = a.d;
+    const bool gated = d.gate_mode == GATE_CHANNEL || d.gate_mode == GATE_IMAGE;
+    float G[N], w[N], b[N];
+    weights<N>(gated ? static_cast<const float*>(d.gate) + (d.gate_mode == GATE_IMAGE ? img * d.C : 0) : nullptr, 1.f, c, G);
+    weights<N>(d.w_post, 1.f, c, w);
+    if (BIAS) weights<N>(d.b_post, 0.f, c, b);
+    if (gated && d.gate_act)
+#pragma unroll
+      for (int j = 0; j < N; ++j) G[j] = sigmoid(G[j]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      gw[j] = d.scale * G[j] * w[j];
+      if (BIAS) gb[j] = d.scale * G[j] * b[j];
+    }
+  }
+  // (an element that is not the thread's has n = 0 and dh = 0; its weights count only through offsets)
+  __device__ __forceinline__ void branch(int64_t img) {
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) branch_weights<V>(img, ch(k), gw_ + k * V, gb_ + k * V);
+      if (BIAS && !cfull)
+#pragma unroll
+        for (int e = 0; e < E; ++e) gb_[e] = chan_ok(e) ? gb_[e] : 0.f;
+    } else {
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.d.C; c += blockDim.x) {
+        float g, b;
+        branch_weights<1>(img, c, &g, &b);
+        lw[c * (BIAS ? 4 : 2)] = g;
+        if (BIAS) lw[c * 4 + 1] = b;
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ void norm_weights() {
+    const srx_resnorm_desc& d = a.d;
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        weights<V>(d.w_pre, 1.f, ch(k), w1_ + k * V);
+        if (BIAS) weights<V>(d.b_pre, 0.f, ch(k), b1_ + k * V);
+      }
+    } else {
+      for (int c = threadIdx.x; c < d.C; c += blockDim.x) {
+        lw[c * (BIAS ? 4 : 2) + (BIAS ? 2 : 1)] = d.w_pre ? d.w_pre[c] : 1.f;
+        if (BIAS) lw[c * 4 + 3] = d.b_pre ? d.b_pre[c] : 0.f;
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ float gw(int e) const { return ROWS ? gw_[e % NL] : lw[ch(e / V) * (BIAS ? 4 : 2)]; }
+  __device__ __forceinline__ float gb(int e) const { return !BIAS ? 0.f : ROWS ? gb_[e % NL] : cdup(e / V) ? 0.f : lw[ch(e / V) * 4 + 1]; }
+  __device__ __forceinline__ float w1(int e) const { return ROWS ? w1_[e % NL] : lw[ch(e / V) * (BIAS ? 4 : 2) + (BIAS ? 2 : 1)]; }
+  __device__ __forceinline__ float b1(int e) const { return !BIAS ? 0.f : ROWS ? b1_[e % NL] : lw[ch(e / V) * 4 + 3]; }
+
+  // ---- sums over the channels: of Q quantities, one value for each of the thread's pixels
+  template <int Q> __device__ __forceinline__ void reduce(float (&s)[Q][NP]) {
+    static_assert(Q <= MAX_Q, "");
+    const int lo = ROWS ? 1 : lanes(), hi = ROWS ? (a.lanes < 64 ? a.lanes : 64) : 64;
+    if (lo < hi) lanes_sum<Q * NP>(&s[0][0], lo, hi);
+    const int waves = ROWS ? a.lanes >> 6 : (int)blockDim.x >> 6;      // that share a pixel
+    if (waves <= 1) return;
+    // two buffers in turn: the barrier of one round keeps the next but one from overwriting what is still being read
+    const int per = (ROWS ? 1 : lanes()) * Q * NP, all = (int)blockDim.x >> 6;
+    float* buf = lds + (round & 1) * (all * (ROWS ? 1 : lanes()) * MAX_Q * NP) + (ROWS ? 0 : l * Q * NP);
+    if (ROWS ? lane == 0 : lane < lanes())
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int j = 0; j < NP; ++j) buf[wave * per + q * NP + j] = s[q][j];
+    __syncthreads();
+    const int first = ROWS ? wave & ~(waves - 1) : 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+      for (int j = 0; j < NP; ++j) s[q][j] = 0;
+    for (int w = first; w < first + waves; ++w)
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int j = 0; j < NP; ++j) s[q][j] += buf[w * per + q * NP + j];
+    ++round;
+  }
+  __device__ __forceinline__ void centre(float* z, const float* mean) const {
+    if (cfull)
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] -= mean[pix(e)];
+    else
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] -= chan_ok(e) ? mean[pix(e)] : 0.f;
+  }
+  // z -> (z - mean) / sqrt(var + eps) or z / sqrt(mean square + eps); returns the factor.  The variance is summed about the
+  // mean, in a second round: E[z^2] - mean^2 would lose it for channels that sit far from zero.
+  __device__ __forceinline__ void normalise(float* z, int kind, float eps, float* r) {
+    const float inv = 1.f / (float)a.d.C;
+    float s[1][NP];
+    if (kind == KIND_LAYER) {
+#pragma unroll
+      for (int j = 0; j < NP; ++j) s[0][j] = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[0][pix(e)] += z[e];
+      reduce<1>(s);
+#pragma unroll
+      for (int j = 0; j < NP; ++j) s[0][j] *= inv;
+      centre(z, s[0]);
+    }
+#pragma unroll
+    for (int j = 0; j < NP; ++j) s[0][j] = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[0][pix(e)] += z[e] * z[e];
+    reduce<1>(s);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) r[j] = 1.f / sqrtf(s[0][j] * inv + eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] *= r[pix(e)];
+  }
+  // u of one element; q: the full gate's raw values
+  template <bool FULL> __device__ __forceinline__ float branch_value(int e, float n, const Raw* q) const {
+    float u = BIAS ? gw(e) * n + gb(e) : gw(e) * n;
+    if (FULL) {
+      const float g = element<V>(q[e / V], e % V);
+      u *= a.d.gate_act ? sigmoid(g) : g;
+    }
+    return u;
+  }
+  // sum the thread's per-channel values over the workgroup and write them to out[C]
+  __device__ __forceinline__ void flush(float* acc, float* out) {
+    if (!ROWS) {
+      lanes_sum<NW>(acc, 1, lanes());
+      if (l == 0)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (cdup(k) == 0) out[ch(k)] = acc[k];
+      return;
+    }
+    if (a.lanes < 64) lanes_sum<NW>(acc, a.lanes, 64);
+    // waves that hold the same channels: every (lanes / 64)-th
+    const int per_row = a.lanes > 64 ? a.lanes >> 6 : 1, waves = (int)blockDim.x >> 6;
+    const bool first = wave < per_row && lane < a.lanes;
+    if (waves > per_row) {
+      __syncthreads();                   // the buffer may still be read as a reduction's
+      if (lane < a.lanes)
+#pragma unroll
+        for (int i = 0; i < NW; ++i) lds[(wave * NW + i) * 64 + lane] = acc[i];
+      __syncthreads();
+      if (first)
+        for (int w = wave + per_row; w < waves; w += per_row)
+#pragma unroll
+          for (int i = 0; i < NW; ++i) acc[i] += lds[(w * NW + i) * 64 + lane];
+      __syncthreads();
+    }
+    if (first) {
+      if (cfull) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) *reinterpret_cast<Vec<float, V>*>(out + ch(k)) = packed<V>(acc + k * V, out);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+          if (chan_ok(i)) out[chan(i)] = acc[i];
+      }
+    }
+  }
+};
+
+template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS>
+__global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
+  extern __shared__ float lds[];
+  typedef Thread<T, ROWS, UNI, K, V, BIAS> Th;
+  Th t(a, lds);
+  const srx_resnorm_desc& d = a.d;
+  if (d.pre_kind) t.norm_weights();
+  if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0);
+  for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
+    const int img = item / a.slices;
+    const int64_t lo = (item - img * a.slices) * a.len;
+    const int64_t hi = lo + a.len < a.P ? lo + a.len : a.P;
+    if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img);
+    for (int64_t base = lo; base < hi; base += t.tile()) {
+      t.at(img, base, hi);
+      typename Th::Raw xr[K], fr[K], qr[K];
+      float y[Th::E], r[Th::NP];
+      if (d.f) {
+        t.read(d.f, d.f_stride, fr);
+        t.read(d.x, d.x_stride, xr);
+        if (FULL) t.read(d.gate, d.gate_stride, qr);
+        float n[Th::E];
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) n[e] = element<V>(fr[e / V], e % V);
+        if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r);
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) y[e] = element<V>(xr[e / V], e % V) + t.template branch_value<FULL>(e, n[e], qr);
+        t.write(d.y, d.y_stride, y);
+      } else {
+        t.read(d.x, d.x_stride, xr);
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) y[e] = element<V>(xr[e / V], e % V);
+      }
+      if (d.pre_kind) {
+        t.normalise(y, d.pre_kind, d.pre_eps, r);
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) y[e] = BIAS ? y[e] * t.w1(e) + t.b1(e) : y[e] * t.w1(e);
+        t.write(d.h, d.h_stride, y);
+      }
+    }
+  }
+}
+
+// With n the normalised y and g = dh w:  D = dy + r (g - n mean(g n) - [mean g]); as n = (y - mu) r, sum g n comes out of the
+// same round of reductions as the variance.
+// The branch's per-channel sums are
+//   d w_post = s sum G D n,   d b_post = s sum G D,   d G = s sum D (w n + b),
+// and where G is the same for all pixels of an image (or is 1) all three follow from sum D n and sum D: two
+// accumulators a channel instead of three.  A full gate takes G D in D's place and writes its own gradient.
+template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS>
+__global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
+  extern __shared__ float lds[];
+  typedef Thread<T, ROWS, UNI, K, V, BIAS> Th;
+  Th t(a, lds);
+  const srx_resnorm_desc& d = a.d;
+  const float inv = 1.f / (float)d.C;
+  float s_dhn[Th::NW] = {}, s_dh[Th::NW] = {}, s_dn[Th::NW] = {}, s_d[Th::NW] = {};
+  if (d.dh) t.norm_weights();
+  if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0);
+  for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
+    const int img = item / a.slices;
+    const int64_t lo = (item - img * a.slices) * a.len;
+    const int64_t hi = lo + a.len < a.P ? lo + a.len : a.P;
+    if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img);
+    for (int64_t base = lo; base < hi; base += t.tile()) {
+      t.at(img, base, hi);
+      typename Th::Raw xr[K], fr[K], qr[K], dyr[K], dhr[K];
+      if (d.f) t.read(d.f, d.f_stride, fr);
+      if (d.dh) t.read(d.x, d.x_stride, xr);
+      if (FULL) t.read(d.gate, d.gate_stride, qr);
+      if (d.dh) t.read(d.dh, d.dh_stride, dhr);
+      if (d.dy) t.read(d.dy, d.dy_stride, dyr);
+      float D[Th::E], n[Th::E], r[Th::NP], r2[Th::NP];
+      float s[2][Th::NP];
+      if (d.f) {
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) n[e] = element<V>(fr[e / V], e % V);
+        if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r2);
+      }
+      if (d.dh) {
+        float mean_g[Th::NP] = {};
+        // y, in D's place for now
+        if (d.f)
+#pragma unroll
+          for (int e = 0; e < Th::E; ++e) D[e] = element<V>(xr[e / V], e % V) + t.template branch_value<FULL>(e, n[e], qr);
+        else
+#pragma unroll
+          for (int e = 0; e < Th::E; ++e) D[e] = element<V>(xr[e / V], e % V);
+        if (d.pre_kind == KIND_LAYER) {
+#pragma unroll
+          for (int j = 0; j < Th::NP; ++j) s[0][j] = s[1][j] = 0;
+#pragma unroll
+          for (int e = 0; e < Th::E; ++e) { s[0][Th::pix(e)] += D[e]; s[1][Th::pix(e)] += element<V>(dhr[e / V], e % V) * t.w1(e); }
+          t.template reduce<2>(s);
+#pragma unroll
+          for (int j = 0; j < Th::NP; ++j) { s[0][j] *= inv; mean_g[j] = s[1][j] * inv; }
+          t.centre(D, s[0]);
+        }
+#pragma unroll
+        for (int j = 0; j < Th::NP; ++j) s[0][j] = s[1][j] = 0;
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) {
+          s[0][Th::pix(e)] += D[e] * D[e];
+          s[1][Th::pix(e)] += element<V>(dhr[e / V], e % V) * t.w1(e) * D[e];
+        }
+        t.template reduce<2>(s);
+#pragma unroll
+        for (int j = 0; j < Th::NP; ++j) {
+          r[j] = 1.f / sqrtf(s[0][j] * inv + d.pre_eps);
+          s[1][j] *= inv * r[j];
+        }
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) {
+          const float g = element<V>(dhr[e / V], e % V), ny = D[e] * r[Th::pix(e)];
+          s_dhn[Th::wi(e)] += g * ny;
+          if (BIAS) s_dh[Th::wi(e)] += g;
+          D[e] = r[Th::pix(e)] * (g * t.w1(e) - ny * s[1][Th::pix(e)] - mean_g[Th::pix(e)]);
+        }
+        if (!t.full)                  // what a mean's offset leaves where there is nothing
+#pragma unroll
+          for (int e = 0; e < Th::E; ++e) D[e] = e % V < t.dropped(e / V) ? 0.f : D[e];
+        if (d.dy)
+#pragma unroll
+          for (int e = 0; e < Th::E; ++e) D[e] += element<V>(dyr[e / V], e % V);
+      } else {
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) D[e] = element<V>(dyr[e / V], e % V);
+      }
+      if (d.dx) t.write(d.dx, d.dx_stride, D);
+      if (d.f) {
+        if (FULL) {
+          float dq[Th::E];
+#pragma unroll
+          for (int e = 0; e < Th::E; ++e) {
+            const float q = element<V>(qr[e / V], e % V), G = d.gate_act ? sigmoid(q) : q;
+            dq[e] = D[e] * (BIAS ? t.gw(e) * n[e] + t.gb(e) : t.gw(e) * n[e]) * (d.gate_act ? G * (1.f - G) : 1.f);
+            D[e] *= G;
+          }
+          if (d.dgate) t.write(d.dgate, d.dgate_stride, dq);
+        }
+#pragma unroll
+        for (int e = 0; e < Th::E; ++e) {
+          s_dn[Th::wi(e)] += D[e] * n[e];
+          if (BIAS) s_d[Th::wi(e)] += D[e];
+          D[e] *= t.gw(e);
+        }
+        if (d.df) {
+          if (d.post_kind) {
+#pragma unroll
+            for (int j = 0; j < Th::NP; ++j) s[0][j] = s[1][j] = 0;
+#pragma unroll
+            for (int e = 0; e < Th::E; ++e) { s[0][Th::pix(e)] += D[e] * n[e]; s[1][Th::pix(e)] += D[e]; }
+            t.template reduce<2>(s);
+#pragma unroll
+            for (int j = 0; j < Th::NP; ++j) { s[0][j] *= inv; s[1][j] = d.post_kind == KIND_LAYER ? s[1][j] * inv : 0.f; }
+#pragma unroll
+            for (int e = 0; e < Th::E; ++e) D[e] = r2[Th::pix(e)] * (D[e] - n[e] * s[0][Th::pix(e)] - s[1][Th::pix(e)]);
+          }
+          t.write(d.df, d.df_stride, D);
+        }
+      }
+    }
+    if (d.f && d.gate_mode == GATE_IMAGE) {
+      float* out = a.part_post + (int64_t)item * 2 * d.C;
+      t.flush(s_dn, out);
+      if (BIAS) t.flush(s_d, out + d.C);
+#pragma unroll
+      for (int i = 0; i < Th::NW; ++i) s_dn[i] = s_d[i] = 0;
+    }
+  }
+  if (d.dh) {
+    float* out = a.part_pre + (int64_t)blockIdx.x * 2 * d.C;
+    t.flush(s_dhn, out);
+    if (BIAS) t.flush(s_dh, out + d.C);
+  }
+  if (d.f && d.gate_mode != GATE_IMAGE) {
+    float* out = a.part_post + (int64_t)blockIdx.x * 2 * d.C;
+    t.flush(s_dn, out);
+    if (BIAS) t.flush(s_d, out + d.C);
+  }
+}
+
+template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS> int launch_with(const Plan& p, int backward, hipStream_t s) {
+  if (backward)
+    hipLaunchKernelGGL((resnorm_bwd_kernel<T, ROWS, UNI, K, V, FULL, BIAS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
+  else
+    hipLaunchKernelGGL((resnorm_fwd_kernel<T, ROWS, UNI, K, V, FULL, BIAS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
+  return srx_check_launch(backward ? "resnorm_bwd" : "resnorm_fwd");
+}
+// whether any offsets, or sums for them, are wanted
+inline bool has_bias(const srx_resnorm_desc& d) { return d.b_post || d.b_pre || d.db_post || d.db_pre; }
+template <typename T, bool ROWS, bool UNI, int K, int V> int launch_for(const Plan& p, int backward, hipStream_t s) {
+  const bool bias = has_bias(p.a.d);
+  if (p.a.d.gate_mode == GATE_FULL)
+    return bias ? launch_with<T, ROWS, UNI, K, V, true, true>(p, backward, s) : launch_with<T, ROWS, UNI, K, V, true, false>(p, backward, s);
+  return bias ? launch_with<T, ROWS, UNI, K, V, false, true>(p, backward, s) : launch_with<T, ROWS, UNI, K, V, false, false>(p, backward, s);
+}
+template <typename T> int launch(const Plan& p, int backward, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  if (p.a.d.layout == SRX_RESNORM_PLANES)
+    return p.a.lanes == 64 ? launch_for<T, false, true, PLANES_K, PLANES_V>(p, backward, s) : launch_for<T, false, false, PLANES_K, PLANES_V>(p, backward, s);
+  if (p.a.d.C < V) return launch_for<T, true, false, V, 1>(p, backward, s);           // rows shorter than a vector: one thread a row
+  return p.elems == 8 ? launch_for<T, true, false, 8 / V, V>(p, backward, s) : launch_for<T, true, false, 16 / V, V>(p, backward, s);
+}
+
+}  // namespace resnorm
