@@ -8,6 +8,21 @@ namespace {
 
 // Joins the partial sums: 16 channels a workgroup, 64 threads a channel that take every 64th partial, in a fixed order.
 constexpr int JOIN_X = 16, JOIN_Y = 64, JOIN_WAVES = JOIN_X * JOIN_Y / 64;
+// sums of p[i step] and, where second > 0, of p[i step + second] over i = y, y + 64, ... < n: eight loads of each in flight (a
+// partial sum was written on another die: a load takes the better part of a microsecond)
+__device__ __forceinline__ void join_sum(const float* p, int y, int n, int step, int second, float& s0, float& s1) {
+  for (int i0 = y; i0 < n; i0 += 8 * JOIN_Y) {
+    float v[8], u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * JOIN_Y;
+      v[j] = i < n ? p[(int64_t)i * step] : 0.f;
+      u[j] = second && i < n ? p[(int64_t)i * step + second] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { s0 += v[j]; s1 += u[j]; }
+  }
+}
 __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args a, int workgroups, int images, bool bias) {
   __shared__ float lds[4][JOIN_WAVES][JOIN_X];
   const srx_resnorm_desc& d = a.d;
@@ -18,14 +33,7 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
   const float w = ok && d.w_post ? d.w_post[c] : 1.f, b = ok && d.b_post ? d.b_post[c] : 0.f;
   const float q = ok && d.gate_mode == GATE_CHANNEL ? gate[c] : 1.f;
   float s[4] = {};                       // sum dh n, sum dh, sum D n (image gates: times s G), sum D
-  if (ok && pre) {
-    const float* p = a.part_pre + c;
-#pragma unroll 4
-    for (int i = y; i < workgroups; i += JOIN_Y) {
-      s[0] += p[(int64_t)i * 2 * d.C];
-      if (bias) s[1] += p[((int64_t)i * 2 + 1) * d.C];
-    }
-  }
+  if (ok && pre) join_sum(a.part_pre + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[0], s[1]);
   if (ok && d.f && d.gate_mode == GATE_IMAGE) {
     for (int i = y; i < images; i += JOIN_Y) {
       float sn = 0, sd = 0;
@@ -41,12 +49,7 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
       s[3] += d.scale * G * sd;
     }
   } else if (ok && d.f) {
-    const float* p = a.part_post + c;
-#pragma unroll 4
-    for (int i = y; i < workgroups; i += JOIN_Y) {
-      s[2] += p[(int64_t)i * 2 * d.C];
-      if (bias) s[3] += p[((int64_t)i * 2 + 1) * d.C];
-    }
+    join_sum(a.part_post + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[2], s[3]);
   }
   lanes_sum<4>(s, JOIN_X, 64);
   if ((threadIdx.x & 63) < JOIN_X)
@@ -97,7 +100,7 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     p.threads = backward || p.a.lanes > 256 ? THREADS : 256;
     tile = p.threads / p.a.lanes;
   } else {
-    const int groups = (d.C + PLANES_K - 1) / PLANES_K;
+    const int groups = d.C < PLANES_K ? d.C : (d.C + PLANES_K - 1) / PLANES_K;        // few channels: one a wave
     p.a.lanes = 64;
     while (groups * p.a.lanes > THREADS) p.a.lanes /= 2;
     p.threads = 64 * ((groups * p.a.lanes + 63) / 64);

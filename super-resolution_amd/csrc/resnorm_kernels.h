@@ -139,7 +139,7 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
   int round;
   int lane, wave, l;          // l = thread within the row / lane along the pixels
   int grp;                    // the thread's row of the workgroup / group of K channels
-  int cb;                     // planes: first channel read (64 lanes: the group's own; else as a vector's, all K exist)
+  int cb;                     // planes: first channel that is read: of the last group, like a vector's, such that all K exist
   int rdup[ROWS ? K : 1];     // rows: elements of step k that are not the thread's; planes: channels of the group that are not
   int pdup;                   // planes: pixels that are not the lane's; rows: V where there is no such row
   bool cfull, full;           // nothing is dropped in this wave: of the channels; at all
@@ -163,9 +163,9 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
       }
     } else {
       const int last = a.d.C - K;
-      cb = UNI || grp * K < last ? grp * K : last;
+      cb = grp * K < last ? grp * K : last;
       rdup[0] = grp * K - cb;
-      ok = cb + K <= a.d.C && rdup[0] == 0;
+      ok = rdup[0] == 0;
     }
     cfull = __all(ok);
     lw = lds + 2 * (int)(blockDim.x >> 6) * MAX_Q * (ROWS ? 1 : lanes() * V);
@@ -177,10 +177,10 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
       const int c = (k * a.lanes + l) * V;
       return c < a.d.C - V ? c : a.d.C - V;
     }
-    return !UNI ? cb + k : cb + k < a.d.C ? cb + k : a.d.C - 1;
+    return cb + k;
   }
   // elements of step k that are not the thread's because of its channels
-  __device__ __forceinline__ int cdup(int k) const { return ROWS ? rdup[k % (ROWS ? K : 1)] : (UNI ? cb + k >= a.d.C : k < rdup[0]) ? V : 0; }
+  __device__ __forceinline__ int cdup(int k) const { return ROWS ? rdup[k % (ROWS ? K : 1)] : k < rdup[0] ? V : 0; }
   __device__ __forceinline__ int dropped(int k) const { return cdup(k) > pdup ? cdup(k) : pdup; }
   // whether an element's channel is the thread's (its pixel need not be)
   __device__ __forceinline__ bool chan_ok(int e) const { return ROWS ? e % V >= cdup(e / V) : cdup(e / V) == 0; }
@@ -203,33 +203,35 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
     }
     full = cfull && __all(pdup == 0);
   }
-  template <typename P> __device__ __forceinline__ P* address(P* p, int64_t stride, int k) const {
-    if (ROWS) return p + row * stride + ch(k);
-    // a scalar base and 32 bits of bytes, in one register for all of the kernel's accesses
+  // planes: a scalar base for each step, and 32 bits of bytes in one register for all of the kernel's accesses
+  template <typename P> __device__ __forceinline__ P* first(P* p, int64_t stride) const {
+    return ROWS ? p + row * stride : p + (image * stride + base + (UNI ? cb * a.P : 0));
+  }
+  template <typename P> __device__ __forceinline__ P* address(P* q, int k) const {
+    if (ROWS) return q + ch(k);
     typedef typename std::conditional<std::is_const<P>::value, const char, char>::type Byte;
-    return reinterpret_cast<P*>(reinterpret_cast<Byte*>(p + (image * stride + base + (UNI ? ch(k) : k) * a.P)) + off);
+    return reinterpret_cast<P*>(reinterpret_cast<Byte*>(q + k * a.P) + off);
   }
   __device__ __forceinline__ void read(const void* p, int64_t stride, Raw* z) const {
+    const T* q = first(static_cast<const T*>(p), stride);
 #pragma unroll
-    for (int k = 0; k < K; ++k) z[k] = *reinterpret_cast<const Raw*>(address(static_cast<const T*>(p), stride, k));
+    for (int k = 0; k < K; ++k) z[k] = *reinterpret_cast<const Raw*>(address(q, k));
     if (!full)
 #pragma unroll
       for (int k = 0; k < K; ++k) drop<V>(z[k], dropped(k));
   }
   __device__ __forceinline__ void write(void* p, int64_t stride, const float* v) const {
+    T* q = first(static_cast<T*>(p), stride);
     if (full) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        T* w = address(static_cast<T*>(p), stride, k);
-        *reinterpret_cast<Raw*>(w) = packed<V>(v + k * V, w);
-      }
+      for (int k = 0; k < K; ++k) *reinterpret_cast<Raw*>(address(q, k)) = packed<V>(v + k * V, q);
       return;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      T* w = address(static_cast<T*>(p), stride, k);
+      T* w = address(q, k);
       const int n = dropped(k);
-      if (n == 0) *reinterpret_cast<Raw*>(w) = packed<V>(v + k * V, w);
+      if (n == 0) *reinterpret_cast<Raw*>(w) = packed<V>(v + k * V, q);
       else if (n < V)
 #pragma unroll
         for (int j = 1; j < V; ++j)
@@ -464,7 +466,10 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
 // and where G is the same for all pixels of an image (or is 1) all three follow from sum D n and sum D: two
 // accumulators a channel instead of three.  A full gate takes G D in D's place and writes its own gradient.
 template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS>
-__global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
+#ifndef BWD_ATTR
+#define BWD_ATTR
+#endif
+__global__ __launch_bounds__(THREADS) BWD_ATTR void resnorm_bwd_kernel(const Args a) {
   extern __shared__ float lds[];
   typedef Thread<T, ROWS, UNI, K, V, BIAS> Th;
   Th t(a, lds);
@@ -613,6 +618,7 @@ template <typename T, bool ROWS, bool UNI, int K, int V> int launch_for(const Pl
 }
 template <typename T> int launch(const Plan& p, int backward, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
+  if (p.a.d.layout == SRX_RESNORM_PLANES && p.a.d.C < PLANES_K) return launch_for<T, false, true, 1, PLANES_V>(p, backward, s);
   if (p.a.d.layout == SRX_RESNORM_PLANES)
     return p.a.lanes == 64 ? launch_for<T, false, true, PLANES_K, PLANES_V>(p, backward, s) : launch_for<T, false, false, PLANES_K, PLANES_V>(p, backward, s);
   if (p.a.d.C < V) return launch_for<T, true, false, V, 1>(p, backward, s);           // rows shorter than a vector: one thread a row
