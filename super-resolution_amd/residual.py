@@ -98,8 +98,11 @@ class _Geometry:
             t = t.contiguous()
         return t, n
 
-    def empty(self) -> torch.Tensor:
-        """A new tensor in this order, as the caller sees it."""
+    def empty(self, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """A new tensor in this order, as the caller sees it; like: a tensor of this shape and type, to copy the order of where it
+        fits (half the host time of a fresh description)."""
+        if like is not None and not self.moved and like.is_contiguous():
+            return torch.empty_like(like)
         if self.moved:
             return torch.empty(self.shape[:1] + self.shape[2:] + self.shape[1:2], dtype=self.dtype, device=self.device).movedim(-1, 1)
         return torch.empty(self.shape, dtype=self.dtype, device=self.device)
@@ -146,11 +149,11 @@ class _Call:
         d.b_pre = b_pre.data_ptr() if b_pre is not None else None
 
     def launch(self, name: str, d) -> None:
-        dev = self.geo.device
-        if torch.cuda.current_device() != dev.index:
-            with torch.cuda.device(dev):
+        index = self.geo.device.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
                 return self.launch(name, d)
-        L.check(getattr(L.lib(), name)(C.byref(d), engine.stream_ptr(dev)), name)
+        L.check(getattr(L.lib(), name)(C.byref(d), torch.cuda.current_stream().cuda_stream), name)
 
     def forward(self, x, f, gate, w_post, b_post, w_pre, b_pre):
         d, keep, geo = self.fresh(), [], self.geo
@@ -159,10 +162,10 @@ class _Call:
         self.common(d, keep, gate, w_post, b_post, w_pre, b_pre)
         y = h = None
         if f is not None:
-            y = geo.empty()
+            y = geo.empty(x)
             d.y, d.y_stride = y.data_ptr() or 16, geo.out_stride()
         if d.pre_kind:
-            h = geo.empty()
+            h = geo.empty(x)
             d.h, d.h_stride = h.data_ptr() or 16, geo.out_stride()
         self.launch("srx_resnorm_forward", d)
         return y, h
@@ -176,17 +179,15 @@ def _note_graph(ctx, tensors, device) -> None:
     """Autograd keeps one accumulator per leaf for as long as any graph of that leaf lives, bound to the stream it was
     first used on.  A backward pass captured on another stream would then make the capture wait for that stream, and
     ROCm's runtime ends the process when such a capture closes.  So the forward call is refused instead."""
-    leaves = [id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf]
-    if not leaves:
-        return
-    stream = engine.stream_ptr(device)
-    if torch.cuda.is_current_stream_capturing():
-        if any(g.srx_stream != stream and not set(leaves).isdisjoint(g.srx_leaves) for g in list(_EAGER)):
+    leaves = [id(t) for t in tensors if t is not None and t.is_leaf and t.requires_grad]
+    if leaves:
+        stream = engine.stream_ptr(device)
+        if not torch.cuda.is_current_stream_capturing():
+            ctx.srx_leaves, ctx.srx_stream = leaves, stream
+            _EAGER.add(ctx)
+        elif any(g.srx_stream != stream and not set(leaves).isdisjoint(g.srx_leaves) for g in list(_EAGER)):
             raise RuntimeError("a graph that was recorded before this capture, on another stream, still holds one of these leaves "
                                "(an output of an earlier call is alive): delete it, or capture on the stream that it was recorded on")
-        return
-    ctx.srx_leaves, ctx.srx_stream = leaves, stream
-    _EAGER.add(ctx)
 
 
 class _ResNormFn(torch.autograd.Function):
@@ -212,22 +213,28 @@ class _ResNormFn(torch.autograd.Function):
         d, keep, out = call.fresh(), [], [None] * 8
         nw, nb = nw and dh is not None, nb and dh is not None
 
-        def new(name, t):
+        def new(at, name, t, stride=0):
+            out[at] = t
             setattr(d, name, t.data_ptr())
-            if name in ("dx", "df") or (name == "dgate" and call.gate_mode == 3):
-                setattr(d, name + "_stride", geo.out_stride())
-            return t
+            if stride:
+                setattr(d, name + "_stride", stride)
 
-        vec = lambda: torch.empty(geo.C, dtype=torch.float32, device=geo.device)  # noqa: E731
+        like, stride = f if f is not None else x, geo.out_stride()
         if nx:
-            out[1] = new("dx", geo.empty()) if dh is not None else dy        # without h, y's gradient is x's
+            if dh is not None:
+                new(1, "dx", geo.empty(like), stride)
+            else:
+                out[1] = dy                                               # without h, y's gradient is x's
         if nf:
-            out[2] = new("df", geo.empty())
-        if ng:
-            out[3] = new("dgate", geo.empty() if call.gate_mode == 3 else torch.empty_like(gate))
-        for at, name, need in ((4, "dw_post", nwp), (5, "db_post", nbp), (6, "dw_pre", nw), (7, "db_pre", nb)):
-            if need:
-                out[at] = new(name, vec())
+            new(2, "df", geo.empty(like), stride)
+        if ng and call.gate_mode != 1:
+            new(3, "dgate", geo.empty(like) if call.gate_mode == 3 else torch.empty_like(gate), stride if call.gate_mode == 3 else 0)
+        vectors = [(at, name) for at, name, need in ((3, "dgate", ng and call.gate_mode == 1), (4, "dw_post", nwp), (5, "db_post", nbp),
+                                                     (6, "dw_pre", nw), (7, "db_pre", nb)) if need]
+        if vectors:
+            rows = torch.empty((len(vectors), geo.C), dtype=torch.float32, device=geo.device)
+            for (at, name), t in zip(vectors, rows.unbind()):
+                new(at, name, t)
         if nf or ng or nwp or nbp or dh is not None:
             call.put(d, keep, "x", x if dh is not None else None)
             call.put(d, keep, "f", f)                 # y is formed again from x and f
