@@ -65,8 +65,55 @@ template <int NG> __device__ __forceinline__ Grad grad_of(const StepArgs<NG>& a,
   }
   return r;
 }
-__device__ __forceinline__ float grad_at(const Grad& g, int64_t i) {
-  return g.bf ? (float)static_cast<const bf16*>(g.p)[i] : static_cast<const float*>(g.p)[i];
+// Four elements at any address that is a multiple of the element's size (views of a flat buffer start anywhere): global
+// memory takes wide accesses there.
+struct __attribute__((packed, aligned(4))) F4 { float e[4]; };
+struct __attribute__((packed, aligned(2))) H4 { uint16_t e[4]; };
+__device__ __forceinline__ float from_bf16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
+__device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (bf16)f); }
+// elements i .. i + 3 of a tensor (i < n; `full`: all of a wave's are there); zeros behind the end
+__device__ __forceinline__ F4 load4(const float* p, int64_t i, int64_t n, bool full) {
+  if (full) return *reinterpret_cast<const F4*>(p + i);
+  F4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r.e[j] = i + j < n ? p[i + j] : 0.f;
+  return r;
+}
+__device__ __forceinline__ F4 load4(const uint16_t* p, int64_t i, int64_t n, bool full) {
+  F4 r;
+  if (full) {
+    const H4 h = *reinterpret_cast<const H4*>(p + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.e[j] = from_bf16(h.e[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.e[j] = i + j < n ? from_bf16(p[i + j]) : 0.f;
+  }
+  return r;
+}
+__device__ __forceinline__ F4 grad4(const Grad& g, int64_t i, int64_t n, bool full) {
+  return g.bf ? load4(static_cast<const uint16_t*>(g.p), i, n, full) : load4(static_cast<const float*>(g.p), i, n, full);
+}
+__device__ __forceinline__ void store4(float* p, int64_t i, int64_t n, bool full, const F4& v) {
+  if (full) {
+    *reinterpret_cast<F4*>(p + i) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) p[i + j] = v.e[j];
+  }
+}
+__device__ __forceinline__ void store4(uint16_t* p, int64_t i, int64_t n, bool full, const F4& v) {
+  if (full) {
+    H4 h;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h.e[j] = to_bf16(v.e[j]);
+    *reinterpret_cast<H4*>(p + i) = h;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < n) p[i + j] = to_bf16(v.e[j]);
+  }
 }
 
 __device__ __forceinline__ double wave_sum_d(double v) {
@@ -76,13 +123,19 @@ __device__ __forceinline__ double wave_sum_d(double v) {
 }
 // Non-negative floats order like their bits, and a NaN's bits are above every number's: one NaN or infinity in a
 // block makes its scale, and with it the whole block, NaN, as it would make the 32-bit moments it touches.
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
+  const unsigned w = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+  return w > v ? w : v;
+}
 __device__ __forceinline__ unsigned wave_max_u(unsigned v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const unsigned w = (unsigned)__shfl_xor((int)v, o, 64);
-    v = w > v ? w : v;
-  }
-  return v;
+  v = dpp_max<0xB1>(v);          // quad_perm 1,0,3,2
+  v = dpp_max<0x4E>(v);          // quad_perm 2,3,0,1
+  v = dpp_max<0x141>(v);         // row_half_mirror
+  v = dpp_max<0x140>(v);         // row_mirror
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = r[0] > r[1] ? r[0] : r[1];
+  const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return q[0] > q[1] ? q[0] : q[1];
 }
 
 __device__ __forceinline__ float decode(unsigned k, unsigned base) { return k ? __uint_as_float((k + base) << 20) : 0.f; }
@@ -95,12 +148,6 @@ __device__ __forceinline__ unsigned encode(float t, unsigned base, unsigned leas
   return c < (int)least ? least : (unsigned)c;
 }
 
-// a first moment that rounds to 0 loses its sign: one code for each value
-__device__ __forceinline__ unsigned encode_signed(float x, float s) {
-  const unsigned c = encode(fabsf(x) / s, M_BASE, 0);
-  return c && x < 0 ? c | 128u : c;
-}
-
 // sum of squares of one chunk of gradients, in 64 bits (a square can leave 32 bits' range, and the sum runs over
 // millions of terms); a fixed order, so the norm is the same every time
 template <int NG> __global__ __launch_bounds__(TPB) void adamw_norm_kernel(const StepArgs<NG> a) {
@@ -110,12 +157,15 @@ template <int NG> __global__ __launch_bounds__(TPB) void adamw_norm_kernel(const
   const Grad g = grad_of<NG>(a, t, ch.tensor);
   double s = 0;
   if (g.p) {
-    const int64_t lo = (int64_t)ch.index * CHUNK;
-    const int64_t hi = lo + CHUNK < t.n ? lo + CHUNK : t.n;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += TPB) {
-      const double x = grad_at(g, i);
-      s += x * x;
-    }
+    const int64_t lo = (int64_t)ch.index * CHUNK + threadIdx.x * 4;
+    const bool full = (int64_t)(ch.index + 1) * CHUNK <= t.n;
+    F4 x[CHUNK / TPB / 4];
+#pragma unroll
+    for (int k = 0; k < CHUNK / TPB / 4; ++k) x[k] = grad4(g, lo + k * TPB * 4, t.n, full);
+#pragma unroll
+    for (int k = 0; k < CHUNK / TPB / 4; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s = fma((double)x[k].e[j], (double)x[k].e[j], s);
   }
   __shared__ double part[TPB / 64];
   s = wave_sum_d(s);
@@ -197,10 +247,40 @@ __device__ __forceinline__ void moments(float& m, float& v, float g, const Coef&
   v = v * c.b2;
   v = v + vg;
 }
-__device__ __forceinline__ float updated(float w, float m, float v, const Coef& c) {
-  return w * c.decay - c.step_size * (m / (sqrtf(v) * c.root + c.eps));
+// The hardware's square root and reciprocal are within 2^-23 of the value: 2^-21 of the update at most, which is itself
+// far below the parameter.  They take a denormal for zero, so an eps that does not cover such a root gets the exact forms.
+__device__ __forceinline__ float updated(float w, float m, float v, const Coef& c, bool fast) {
+  const float u = fast ? m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * c.root + c.eps) : m / (sqrtf(v) * c.root + c.eps);
+  return w * c.decay - c.step_size * u;
+}
+// Codes of four values x against a block's largest, s: the nearest code of the correctly rounded quotient |x| / s.  The
+// reciprocal's product is within 3 units of it, so it gives the same code unless it lies that close to the middle
+// between two codes: then the division is made.
+template <bool SIGNED> __device__ __forceinline__ uint32_t encode4(const float* x, float s) {
+  constexpr unsigned base = SIGNED ? M_BASE : V_BASE, least = SIGNED ? 0 : 1;
+  const float r = __builtin_amdgcn_rcpf(s);
+  float t[4];
+  bool near = !(s > 1e-30f && s < 1e30f);           // (a reciprocal that is no normal number)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    t[j] = fabsf(x[j]) * r;
+    near = near || ((__float_as_uint(t[j]) + 0x80004u) & 0xFFFFFu) < 8u;
+  }
+  if (__any(near))
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = fabsf(x[j]) / s;
+  uint32_t out = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    unsigned c = encode(t[j], base, least);
+    if (SIGNED) c |= c && x[j] < 0 ? 128u : 0u;     // a first moment that rounds to 0 loses its sign: one code for each value
+    out |= c << (8 * j);
+  }
+  return out;
 }
 
+// A wave takes whole blocks of 256, four elements a lane, so that a block's largest is a wave's.  All of a wave's four
+// blocks are read before the first is computed: a workgroup's only other wait is for the tables in front of them.
 template <int BITS, int NG> __global__ __launch_bounds__(TPB) void adamw_step_kernel(const StepArgs<NG> a) {
   const Ctl* ctl = reinterpret_cast<const Ctl*>(a.coef);
   if (ctl->skip) return;
@@ -210,68 +290,80 @@ template <int BITS, int NG> __global__ __launch_bounds__(TPB) void adamw_step_ke
   if (!g.p) return;
   const Coef c = reinterpret_cast<const Coef*>(a.coef + 4)[ch.tensor];
   const float factor = ctl->factor;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int b = wave; b < CHUNK / BLOCK; b += TPB / 64) {
-    const int64_t lo = (int64_t)ch.index * CHUNK + b * BLOCK;      // first element of the block in its tensor
-    if (lo >= t.n) break;
-    const int64_t blk = t.first_block + lo / BLOCK;
-    float m[4], v[4];
-    float ms = 0, vs = 0;
-    if constexpr (BITS == 8) { ms = a.m_scale[blk]; vs = a.v_scale[blk]; }
+  const bool fast = c.eps >= 1e-15f;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int NB = CHUNK / BLOCK / (TPB / 64);
+  const int64_t lo = (int64_t)ch.index * CHUNK + wave * NB * BLOCK;        // the wave's first element in its tensor
+  const int64_t blk = t.first_block + lo / BLOCK;
+  F4 w[NB], gr[NB], m[NB], v[NB];
+  uint32_t mc[NB], vc[NB];
+  float ms[NB], vs[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t i = lo + b * BLOCK + lane * 4, s = (blk + b) * BLOCK + lane * 4;
+    if (lo + b * BLOCK >= t.n) break;
+    const bool full = lo + (b + 1) * BLOCK <= t.n;
+    gr[b] = grad4(g, i, t.n, full);
+    if (t.master) w[b] = load4(t.master, i, t.n, full);
+    else w[b] = load4(static_cast<const float*>(t.p), i, t.n, full);
+    if constexpr (BITS == 8) {
+      mc[b] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + s);
+      vc[b] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + s);
+      ms[b] = a.m_scale[blk + b];
+      vs[b] = a.v_scale[blk + b];
+    } else {
+      m[b] = *reinterpret_cast<const F4*>(static_cast<const float*>(a.m) + s);
+      v[b] = *reinterpret_cast<const F4*>(static_cast<const float*>(a.v) + s);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int64_t i = lo + b * BLOCK + lane * 4, s = (blk + b) * BLOCK + lane * 4;
+    if (lo + b * BLOCK >= t.n) break;
+    const bool full = lo + (b + 1) * BLOCK <= t.n;
+    if (t.master) {
+      // the parameter is what the user sees and may have written: where it is not the master's rounding, it wins
+      const F4 p = load4(static_cast<const uint16_t*>(t.p), i, t.n, full);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[b].e[j] = from_bf16(to_bf16(w[b].e[j])) == p.e[j] ? w[b].e[j] : p.e[j];
+    }
     unsigned mmax = 0, vmax = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int e = lane + 64 * j;
-      const int64_t i = lo + e, s = blk * BLOCK + e;
-      m[j] = v[j] = 0;
-      if (i >= t.n) continue;
       if constexpr (BITS == 8) {
-        const unsigned mc = static_cast<const uint8_t*>(a.m)[s], vc = static_cast<const uint8_t*>(a.v)[s];
-        m[j] = decode(mc & 127, M_BASE) * ms;
-        if (mc & 128) m[j] = -m[j];
-        v[j] = decode(vc, V_BASE) * vs;
-      } else {
-        m[j] = static_cast<const float*>(a.m)[s];
-        v[j] = static_cast<const float*>(a.v)[s];
+        const unsigned mk = (mc[b] >> (8 * j)) & 255, vk = (vc[b] >> (8 * j)) & 255;
+        const float x = decode(mk & 127, M_BASE) * ms[b];
+        m[b].e[j] = mk & 128 ? -x : x;
+        v[b].e[j] = decode(vk, V_BASE) * vs[b];
       }
       float gi;
       {
 #pragma clang fp contract(off)
-        gi = grad_at(g, i) * factor;
+        gi = gr[b].e[j] * factor;
       }
-      moments(m[j], v[j], gi, c);
-      if (t.master) {
-        // the parameter is what the user sees and may have written: where it is not the master's rounding, it wins
-        bf16* p = static_cast<bf16*>(t.p) + i;
-        const float w0 = t.master[i];
-        const float w = updated((float)(bf16)w0 == (float)*p ? w0 : (float)*p, m[j], v[j], c);
-        t.master[i] = w;
-        *p = (bf16)w;
-      } else {
-        float* p = static_cast<float*>(t.p) + i;
-        *p = updated(*p, m[j], v[j], c);
-      }
-      if constexpr (BITS == 32) {
-        static_cast<float*>(a.m)[s] = m[j];
-        static_cast<float*>(a.v)[s] = v[j];
-      } else {
-        const unsigned mb = __float_as_uint(m[j]) & 0x7FFFFFFFu, vb = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+      moments(m[b].e[j], v[b].e[j], gi, c);
+      w[b].e[j] = updated(w[b].e[j], m[b].e[j], v[b].e[j], c, fast);
+      if constexpr (BITS == 8) {
+        // (behind the tensor's end everything is zero and stays zero, unless the block is not finite)
+        const unsigned mb = __float_as_uint(m[b].e[j]) & 0x7FFFFFFFu, vb = __float_as_uint(v[b].e[j]) & 0x7FFFFFFFu;
         mmax = mb > mmax ? mb : mmax;
         vmax = vb > vmax ? vb : vmax;
       }
     }
-    if constexpr (BITS == 8) {
-      ms = __uint_as_float(wave_max_u(mmax));
-      vs = __uint_as_float(wave_max_u(vmax));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int e = lane + 64 * j;
-        if (lo + e >= t.n) continue;
-        const int64_t s = blk * BLOCK + e;
-        static_cast<uint8_t*>(a.m)[s] = (uint8_t)encode_signed(m[j], ms);
-        static_cast<uint8_t*>(a.v)[s] = (uint8_t)encode(v[j] / vs, V_BASE, 1);
-      }
-      if (lane == 0) { a.m_scale[blk] = ms; a.v_scale[blk] = vs; }
+    if (t.master) {
+      store4(t.master, i, t.n, full, w[b]);
+      store4(static_cast<uint16_t*>(t.p), i, t.n, full, w[b]);
+    } else {
+      store4(static_cast<float*>(t.p), i, t.n, full, w[b]);
+    }
+    if constexpr (BITS == 32) {
+      *reinterpret_cast<F4*>(static_cast<float*>(a.m) + s) = m[b];
+      *reinterpret_cast<F4*>(static_cast<float*>(a.v) + s) = v[b];
+    } else {
+      const float nm = __uint_as_float(wave_max_u(mmax)), nv = __uint_as_float(wave_max_u(vmax));
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s) = encode4<true>(m[b].e, nm);
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s) = encode4<false>(v[b].e, nv);
+      if (lane == 0) { a.m_scale[blk + b] = nm; a.v_scale[blk + b] = nv; }
     }
   }
 }
@@ -292,12 +384,8 @@ __global__ __launch_bounds__(TPB) void moments_to8_kernel(const float* m, const 
     bm = y > bm ? y : bm;
   }
   const float sm = __uint_as_float(wave_max_u(am)), sv = __uint_as_float(wave_max_u(bm));
-  uint32_t cm = 0, cv = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    cm |= encode_signed(a[j], sm) << (8 * j);
-    cv |= encode(b[j] / sv, V_BASE, 1) << (8 * j);
-  }
+  const float xm[4] = {a[0], a[1], a[2], a[3]}, xv[4] = {b[0], b[1], b[2], b[3]};
+  const uint32_t cm = encode4<true>(xm, sm), cv = encode4<false>(xv, sv);
   *reinterpret_cast<uint32_t*>(mc + s) = cm;
   *reinterpret_cast<uint32_t*>(vc + s) = cv;
   if (lane == 0) { ms[blk] = sm; vs[blk] = sv; }
