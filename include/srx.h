@@ -433,6 +433,8 @@ int srx_adamw_moments_from8(const void* m_code, const void* v_code, const float*
  * SRX_RESNORM_ROWS, channels contiguous, row b * P + p at (b * P + p) * *_stride, C <= 8192. */
 #define SRX_RESNORM_PLANES 0
 #define SRX_RESNORM_ROWS 1
+#define SRX_RESNORM_MAX_PLANES_C 1024
+#define SRX_RESNORM_MAX_ROWS_C 8192
 typedef struct srx_resnorm_desc {
   int32_t dtype, layout;
   int32_t B, C, P;

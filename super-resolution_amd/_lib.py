@@ -6,6 +6,7 @@ fails, a RuntimeError is raised.
 from __future__ import annotations
 
 import ctypes as C
+import importlib
 import os
 
 # PyTorch's ROCm wheel bundles its own HIP runtime (torch/lib/libamdhip64.so).  It must be the
@@ -29,7 +30,6 @@ vp, i32, i64, f32, f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_double
 
 ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_GROUPS = 256, 4096, 32
 RESNORM_PLANES, RESNORM_ROWS = 0, 1
-RESNORM_MAX_C = (1024, 8192)          # per layout
 
 
 class PackSeg(C.Structure):
@@ -223,6 +223,29 @@ def lib():
                                    f"the binding but {l.srx_sizeof(i)} in {LIB_PATH}")
         _lib = l
     return _lib
+
+
+_host = None
+
+
+def host():
+    """The host module (csrc/host.cpp, once), bound to the library that lib() has loaded.  Raises RuntimeError if it has
+    not been built."""
+    global _host
+    if _host is None:
+        l = lib()
+        try:
+            m = importlib.import_module(__package__ + "._srxhost")
+        except ImportError as e:
+            raise RuntimeError(f"{os.path.join(_HERE, '_srxhost.so')} cannot be loaded ({e}): build it with "
+                               f"`make -C {os.path.join(_HERE, 'csrc')}` (or python -c 'import __graft_entry__ as g; g.build()'). "
+                               "There is no fallback path.") from e
+        if m.desc_bytes != C.sizeof(ResnormDesc):
+            raise RuntimeError(f"_srxhost was built against another srx.h (descriptor of {m.desc_bytes} bytes, {C.sizeof(ResnormDesc)} here)")
+        m.bind(*(C.cast(getattr(l, n), C.c_void_p).value for n in
+                 ("srx_resnorm_forward", "srx_resnorm_backward", "srx_resnorm_ws_floats", "srx_last_error")))
+        _host = m
+    return _host
 
 
 def check(rc: int, what: str = "") -> None:

@@ -77,7 +77,8 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-constexpr int MAX_ROWS_C = 16 * THREADS, MAX_PLANES_C = 1024;
+constexpr int MAX_ROWS_C = SRX_RESNORM_MAX_ROWS_C, MAX_PLANES_C = SRX_RESNORM_MAX_PLANES_C;
+static_assert(MAX_ROWS_C == 16 * THREADS, "");
 
 int pow2_at_least(int64_t n) {
   int p = 1;

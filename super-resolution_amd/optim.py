@@ -8,10 +8,8 @@ decisions are taken on the device: a step never waits for the host and can be ca
 """
 from __future__ import annotations
 
-import array
 import ctypes as C
 import math
-from operator import attrgetter
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -21,10 +19,7 @@ from . import _lib as L
 from . import engine
 
 _ptr = torch.Tensor.data_ptr
-_numel = torch.Tensor.numel
-_contiguous = torch.Tensor.is_contiguous
-_device = torch.Tensor.get_device
-_dtype, _grad = attrgetter("dtype"), attrgetter("grad")
+_MOVED, _ODD, _BF16 = 1, 2, 4              # flags of the host module's gather()
 _DTYPE_ID = {torch.bfloat16: L.BF16, torch.float32: L.F32}
 
 
@@ -123,8 +118,11 @@ class AdamW:
                 self._master_at.append(self._master_at[-1] + n)
             #: fp32 masters of the bf16 parameters, one after the other (None: there are none)
             self.master = zeros(self._master_at[-1]) if sum(half) else None
-            self._ptrs: List[int] = []
+            self._tensors: Optional[torch.Tensor] = None
             self._bind()
+            self._addresses, self._types = np.zeros(len(self.params), np.uint64), np.zeros(len(self.params), np.uint8)
+            self._addresses_at, self._types_at = self._addresses.ctypes.data, self._types.ctypes.data
+            self._gather = L.host().gather
             self._copy_masters()
             d = self._desc = L.AdamwDesc()
             d.state_bits, d.ntensors, d.ngroups = state_bits, len(self.params), len(self.param_groups)
@@ -189,10 +187,10 @@ class AdamW:
                 t.g_off = (ptrs[i] - base) // esize if self._flat and self._n[i] else 0
                 i += 1
         raw = torch.frombuffer(bytearray(C.string_at(C.addressof(arr), C.sizeof(arr))), dtype=torch.uint8)
-        if self._ptrs:
+        if self._tensors is not None:
             torch.cuda.synchronize(self.device)      # steps in flight still read the old table
         self._tensors = raw.to(self.device)
-        self._ptrs = ptrs
+        self._ptrs = np.array(ptrs, dtype=np.uint64)
 
     def _copy_masters(self) -> None:
         for i, p in enumerate(self.params):
@@ -212,10 +210,10 @@ class AdamW:
                 return self.step(grads, grad_scale)
         if not math.isfinite(grad_scale):
             raise ValueError(f"grad_scale must be finite, got {grad_scale}")
-        if list(map(_ptr, self.params)) != self._ptrs:
-            self._bind()
-        d, keep = self._desc, None
+        d = self._desc
         if isinstance(grads, torch.Tensor):
+            if list(map(_ptr, self.params)) != self._ptrs.tolist():
+                self._bind()
             if not self._flat:
                 raise ValueError("a flat gradient needs parameters of one type that are views covering one flat buffer")
             if grads.device != self.device or grads.dtype not in _DTYPE_ID or grads.numel() != sum(self._n) or not grads.is_contiguous():
@@ -226,8 +224,18 @@ class AdamW:
             if grads.numel() == 0:
                 return self._empty_norm()
         else:
-            addresses, types, keep = self._addresses(grads)
-            d.grads, d.grad_dtypes, d.flat_grad = addresses.buffer_info()[0], types, None
+            # one pass over both lists: addresses, types, and whether anything is not as it should be
+            if grads is not None and type(grads) is not list:
+                grads = list(grads)
+            index = self.device.index
+            flags = self._gather(self.params, grads, self._ptrs, self._addresses, self._types, index)
+            if flags & _MOVED:
+                self._bind()
+            if flags & _ODD:
+                grads = self._taken(grads)
+                flags = self._gather(self.params, grads, self._ptrs, self._addresses, self._types, index)
+            d.grads, d.flat_grad = self._addresses_at, None
+            d.grad_dtypes = self._types_at if flags & _BF16 else None
         self._check_hyper()
         for q, g in zip(self._groups, self.param_groups):
             q.lr, (q.beta1, q.beta2), q.eps, q.weight_decay = g["lr"], g["betas"], g["eps"], g["weight_decay"]
@@ -238,43 +246,22 @@ class AdamW:
             norm = torch.empty((), dtype=torch.float32, device=self.device)
             d.norm = norm.data_ptr()
         L.check(self._lib.srx_adamw_step(C.byref(d), engine.stream_ptr(self.device)), "srx_adamw_step")
-        del keep
         return norm
 
     def _empty_norm(self):
         return torch.zeros((), device=self.device) if self.max_grad_norm or self.skip_nonfinite else None
 
-    def _addresses(self, grads):
-        """(addresses, C array of dtypes or None, what has to live until the launch) of a list of gradients."""
-        given = grads is not None
-        grads = list(grads) if given else list(map(_grad, self.params))
-        if len(grads) != len(self.params):
-            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        some = grads if all(g is not None for g in grads) else [g for g in grads if g is not None]
-        # whole lists are compared in C: 702 tensors cost tens of microseconds here, not hundreds
-        index = self.device.index
-        n = self._n if some is grads else [k for k, g in zip(self._n, grads) if g is not None]
-        if list(map(_numel, some)) != n or any(i != index for i in map(_device, some)) or \
-                (given and any(g.shape != p.shape for g, p in zip(grads, self.params) if g is not None)):
-            for i, (g, p) in enumerate(zip(grads, self.params)):
-                if g is not None and (g.shape != p.shape or g.device != p.device):
-                    raise ValueError(f"gradient {i} has shape {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {p.device}")
-        types = list(map(_dtype, some))
-        if not set(types) <= set(_DTYPE_ID):
-            raise ValueError(f"gradients must be float32 or bfloat16, got {sorted(str(t) for t in set(types) - set(_DTYPE_ID))}")
-        if not all(map(_contiguous, some)):
-            grads = [g if g is None else g.contiguous() for g in grads]
-            some = [g for g in grads if g is not None]
-        ptrs = list(map(_ptr, some))
-        if 0 in ptrs:                     # an empty tensor has no address, but it takes its step: any that is not 0 will do
-            ptrs = [p or self._steps.data_ptr() for p in ptrs]
-        if some is not grads:
-            left = iter(ptrs)
-            ptrs = [0 if g is None else next(left) for g in grads]
-        ids = None
-        if torch.bfloat16 in types:
-            ids = bytes(L.F32 if g is None else _DTYPE_ID[g.dtype] for g in grads)
-        return array.array("Q", ptrs), (C.cast(C.c_char_p(ids), C.c_void_p) if ids is not None else None), (grads, ids)
+    def _taken(self, grads) -> list:
+        """Gradients that gather() cannot take as they are: brought into order, or refused."""
+        grads = [p.grad for p in self.params] if grads is None else grads
+        for i, (g, p) in enumerate(zip(grads, self.params)):
+            if g is None:
+                continue
+            if g.shape != p.shape or g.device != p.device:
+                raise ValueError(f"gradient {i} has shape {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {p.device}")
+            if g.dtype not in _DTYPE_ID or g.layout != torch.strided:
+                raise ValueError(f"gradient {i}: a dense float32 or bfloat16 tensor expected, got {g.dtype}, {g.layout}")
+        return [g if g is None else g.contiguous() for g in grads]
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         for p in self.params:
