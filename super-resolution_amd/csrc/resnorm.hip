@@ -107,18 +107,19 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     p.threads = 64 * ((groups * p.a.lanes + 63) / 64);
     tile = p.a.lanes * PLANES_V;
   }
-  const int64_t tiles = (p.a.P + tile - 1) / tile;
-  const int64_t target = backward ? 512 : 4096;
-  int64_t s = p.images > 0 ? (target + p.images - 1) / p.images : 1;
-  s = s < 1 ? 1 : s > tiles ? tiles : s;
-  if (s < 1) s = 1;
-  p.a.len = (tiles + s - 1) / s * tile;
-  p.a.slices = p.a.len > 0 ? (int)((p.a.P + p.a.len - 1) / p.a.len) : 1;
-  if (p.a.slices < 1) p.a.slices = 1;
+  // Workgroups walk the tiles side by side: neighbours in time are neighbours in memory.  (Shares of consecutive tiles, each
+  // a power of two apart, keep all workgroups on the same few memory channels: 64 x 64 x 128 x 128 bf16 maps ran backward
+  // in WALK_BEFORE us that way, in WALK_AFTER us this way.)  With a gate for each image an item stays within its image, so that its sums
+  // are the image's.
+  const int64_t tiles = (p.a.P + tile - 1) / tile, most = backward ? 512 : 4096;
+  int64_t s = tiles;
+  if (image_gate && p.images > 0 && s > (most + p.images - 1) / p.images) s = (most + p.images - 1) / p.images;
+  if (p.images > 0 && s > (1LL << 30) / p.images) s = (1LL << 30) / p.images;
+  p.a.slices = s < 1 ? 1 : (int)s;
   p.a.items = p.a.P > 0 ? p.images * p.a.slices : 0;
-  p.workgroups = (int)(p.a.items < target ? p.a.items : target);
+  p.workgroups = (int)(p.a.items < most ? p.a.items : most);
   const int waves = p.threads / 64;
-  int bytes = 2 * waves * MAX_Q * (rows ? 1 : p.a.lanes * PLANES_V) * 4;            // two buffers of a reduction: at most 16 KB
+  int bytes = 2 * WAVES * MAX_Q * (rows ? 1 : p.a.lanes * PLANES_V) * 4;            // two buffers of a reduction: at most 16 KB
   if (!rows) bytes += p.threads / p.a.lanes * PLANES_K * 16;                        // weights: at most 16 KB
   if (backward && rows && p.a.lanes < p.threads && bytes < waves * p.elems * 64 * 4) bytes = waves * p.elems * 64 * 4;     // flush: at most 32 KB
   p.lds_bytes = bytes;

@@ -19,15 +19,15 @@ namespace resnorm {
 
 constexpr int MAX_Q = 2;          // quantities reduced together
 constexpr int THREADS = 512;      // most threads of a workgroup
+constexpr int WAVES = THREADS / 64;
 enum { KIND_NONE = 0, KIND_RMS = 1, KIND_LAYER = 2 };
 enum { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_IMAGE = 2, GATE_FULL = 3 };
 
 struct Args {
   srx_resnorm_desc d;
   int lanes;            // rows: threads per row (a power of two); planes: lanes along the pixels (64 down to 4)
-  int slices;           // shares of an image's pixels
-  int items;            // images * slices
-  int64_t len;          // pixels of a share
+  int slices;           // shares of an image's tiles: share s takes tiles s, s + slices, ...
+  int items;            // images * slices; workgroup w takes items w, w + workgroups, ...
   int64_t P;            // pixels of an "image" (rows without per-image gate: all rows are one image)
   float* part_pre;      // [workgroups][2][C]
   float* part_post;     // [workgroups or items][2][C]
@@ -83,6 +83,14 @@ template <int V> __device__ __forceinline__ Vec<bf16, V> packed(const float* v, 
 }
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
 
+// A barrier for what waves hand each other through LDS, and only that: __syncthreads() would also wait for every global load
+// and store in flight, the last tile's results and the next one's inputs among them.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
   return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
 }
@@ -133,6 +141,14 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
   static __device__ __forceinline__ constexpr int wi(int e) { return ROWS ? e : e / V; }
   typedef Vec<T, V> Raw;
 
+  // a tile of the workgroup
+  struct Pos {
+    int64_t image, base;      // its first pixel within the image
+    int64_t row;              // rows: the thread's row
+    unsigned off;             // planes: bytes from `base` (and the wave's channel, if it has one) to the lane's first element
+    int pdup;                 // planes: pixels that are not the lane's; rows: V where there is no such row
+    bool full;                // nothing is dropped in this wave
+  };
   const Args& a;
   float* lds;                 // reductions
   float* lw;                  // planes: weights by channel: gw, gb, w1, b1 (BIAS) or gw, w1
@@ -141,11 +157,7 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
   int grp;                    // the thread's row of the workgroup / group of K channels
   int cb;                     // planes: first channel that is read: of the last group, like a vector's, such that all K exist
   int rdup[ROWS ? K : 1];     // rows: elements of step k that are not the thread's; planes: channels of the group that are not
-  int pdup;                   // planes: pixels that are not the lane's; rows: V where there is no such row
-  bool cfull, full;           // nothing is dropped in this wave: of the channels; at all
-  unsigned off;               // planes: bytes from `base` (and the wave's channel, if it has one) to the lane's first element
-  int64_t row;                // rows: the thread's row
-  int64_t image, base;        // first pixel of the workgroup's tile within the image
+  bool cfull;                 // nothing is dropped in this wave because of the channels
   float gw_[NL], gb_[NL], w1_[NL], b1_[NL];
 
   __device__ __forceinline__ Thread(const Args& a_, float* lds_) : a(a_), lds(lds_), round(0) {
@@ -168,7 +180,12 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
       ok = rdup[0] == 0;
     }
     cfull = __all(ok);
-    lw = lds + 2 * (int)(blockDim.x >> 6) * MAX_Q * (ROWS ? 1 : lanes() * V);
+    const int floats = 2 * WAVES * MAX_Q * (ROWS ? 1 : lanes() * V);
+    lw = lds + floats;
+    if (!ROWS && (int)blockDim.x < THREADS) {
+      for (int i = threadIdx.x; i < floats; i += blockDim.x) lds[i] = 0;
+      lds_barrier();
+    }
   }
   __device__ __forceinline__ int lanes() const { return UNI ? 64 : a.lanes; }
   // first channel of step k
@@ -181,56 +198,59 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
   }
   // elements of step k that are not the thread's because of its channels
   __device__ __forceinline__ int cdup(int k) const { return ROWS ? rdup[k % (ROWS ? K : 1)] : k < rdup[0] ? V : 0; }
-  __device__ __forceinline__ int dropped(int k) const { return cdup(k) > pdup ? cdup(k) : pdup; }
+  __device__ __forceinline__ int dropped(int k, const Pos& o) const { return cdup(k) > o.pdup ? cdup(k) : o.pdup; }
   // whether an element's channel is the thread's (its pixel need not be)
   __device__ __forceinline__ bool chan_ok(int e) const { return ROWS ? e % V >= cdup(e / V) : cdup(e / V) == 0; }
   __device__ __forceinline__ int chan(int e) const { return ch(e / V) + (ROWS ? e % V : 0); }
   // pixels that a workgroup takes at a time
   __device__ __forceinline__ int tile() const { return ROWS ? (int)blockDim.x / a.lanes : lanes() * V; }
-  __device__ __forceinline__ void at(int64_t img, int64_t base_, int64_t end) {
-    image = img;
-    base = base_;
+  __device__ __forceinline__ Pos at(int64_t img, int64_t base, int64_t end) const {
+    Pos o;
+    o.image = img;
     const int64_t want = base + (ROWS ? grp : l * V), last = end - (ROWS ? 1 : V);
     if (ROWS) {
-      row = image * a.P + (want < last ? want : last);
-      pdup = want > last ? V : 0;
+      o.row = img * a.P + (want < last ? want : last);
+      o.pdup = want > last ? V : 0;
+      o.base = base;
     } else {
       // where less than a vector is left behind the tile's start, the tile starts earlier
       const int64_t from = want < last ? want : last;
-      pdup = want - from < V ? (int)(want - from) : V;
-      if (base > last) base = last;
-      off = ((unsigned)(from - base) + (UNI ? 0u : (unsigned)cb * (unsigned)a.P)) * (unsigned)sizeof(T);
+      o.pdup = want - from < V ? (int)(want - from) : V;
+      o.base = base < last ? base : last;
+      o.off = ((unsigned)(from - o.base) + (UNI ? 0u : (unsigned)cb * (unsigned)a.P)) * (unsigned)sizeof(T);
     }
-    full = cfull && __all(pdup == 0);
+    o.full = cfull && __all(o.pdup == 0);
+    return o;
   }
   // planes: a scalar base for each step, and 32 bits of bytes in one register for all of the kernel's accesses
-  template <typename P> __device__ __forceinline__ P* first(P* p, int64_t stride) const {
-    return ROWS ? p + row * stride : p + (image * stride + base + (UNI ? cb * a.P : 0));
+  template <typename P> __device__ __forceinline__ P* first(P* p, int64_t stride, const Pos& o) const {
+    return ROWS ? p + o.row * stride : p + (o.image * stride + o.base + (UNI ? cb * a.P : 0));
   }
-  template <typename P> __device__ __forceinline__ P* address(P* q, int k) const {
+  template <typename P> __device__ __forceinline__ P* address(P* q, int k, const Pos& o) const {
     if (ROWS) return q + ch(k);
     typedef typename std::conditional<std::is_const<P>::value, const char, char>::type Byte;
-    return reinterpret_cast<P*>(reinterpret_cast<Byte*>(q + k * a.P) + off);
+    return reinterpret_cast<P*>(reinterpret_cast<Byte*>(q + k * a.P) + o.off);
   }
-  __device__ __forceinline__ void read(const void* p, int64_t stride, Raw* z) const {
-    const T* q = first(static_cast<const T*>(p), stride);
+  __device__ __forceinline__ void read(const void* p, int64_t stride, Raw* z, const Pos& o) const {
+    const T* q = first(static_cast<const T*>(p), stride, o);
 #pragma unroll
-    for (int k = 0; k < K; ++k) z[k] = *reinterpret_cast<const Raw*>(address(q, k));
-    if (!full)
-#pragma unroll
-      for (int k = 0; k < K; ++k) drop<V>(z[k], dropped(k));
+    for (int k = 0; k < K; ++k) z[k] = *reinterpret_cast<const Raw*>(address(q, k, o));
   }
-  __device__ __forceinline__ void write(void* p, int64_t stride, const float* v) const {
-    T* q = first(static_cast<T*>(p), stride);
-    if (full) {
+  __device__ __forceinline__ void drop_dups(Raw* z, const Pos& o) const {
 #pragma unroll
-      for (int k = 0; k < K; ++k) *reinterpret_cast<Raw*>(address(q, k)) = packed<V>(v + k * V, q);
+    for (int k = 0; k < K; ++k) drop<V>(z[k], dropped(k, o));
+  }
+  __device__ __forceinline__ void write(void* p, int64_t stride, const float* v, const Pos& o) const {
+    T* q = first(static_cast<T*>(p), stride, o);
+    if (o.full) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) *reinterpret_cast<Raw*>(address(q, k, o)) = packed<V>(v + k * V, q);
       return;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      T* w = address(q, k);
-      const int n = dropped(k);
+      T* w = address(q, k, o);
+      const int n = dropped(k, o);
       if (n == 0) *reinterpret_cast<Raw*>(w) = packed<V>(v + k * V, q);
       else if (n < V)
 #pragma unroll
@@ -276,14 +296,14 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
 #pragma unroll
         for (int e = 0; e < E; ++e) gb_[e] = chan_ok(e) ? gb_[e] : 0.f;
     } else {
-      __syncthreads();
+      lds_barrier();
       for (int c = threadIdx.x; c < a.d.C; c += blockDim.x) {
         float g, b;
         branch_weights<1>(img, c, &g, &b);
         lw[c * (BIAS ? 4 : 2)] = g;
         if (BIAS) lw[c * 4 + 1] = b;
       }
-      __syncthreads();
+      lds_barrier();
     }
   }
   __device__ __forceinline__ void norm_weights() {
@@ -299,7 +319,7 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
         lw[c * (BIAS ? 4 : 2) + (BIAS ? 2 : 1)] = d.w_pre ? d.w_pre[c] : 1.f;
         if (BIAS) lw[c * 4 + 3] = d.b_pre ? d.b_pre[c] : 0.f;
       }
-      __syncthreads();
+      lds_barrier();
     }
   }
   __device__ __forceinline__ float gw(int e) const { return ROWS ? gw_[e % NL] : lw[ch(e / V) * (BIAS ? 4 : 2)]; }
@@ -312,28 +332,41 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
     static_assert(Q <= MAX_Q, "");
     const int lo = ROWS ? 1 : lanes(), hi = ROWS ? (a.lanes < 64 ? a.lanes : 64) : 64;
     if (lo < hi) lanes_sum<Q * NP>(&s[0][0], lo, hi);
+    // two buffers in turn: the barrier of one round keeps the next but one from overwriting what is still being read
     const int waves = ROWS ? a.lanes >> 6 : (int)blockDim.x >> 6;      // that share a pixel
     if (waves <= 1) return;
-    // two buffers in turn: the barrier of one round keeps the next but one from overwriting what is still being read
-    const int per = (ROWS ? 1 : lanes()) * Q * NP, all = (int)blockDim.x >> 6;
-    float* buf = lds + (round & 1) * (all * (ROWS ? 1 : lanes()) * MAX_Q * NP) + (ROWS ? 0 : l * Q * NP);
-    if (ROWS ? lane == 0 : lane < lanes())
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-#pragma unroll
-        for (int j = 0; j < NP; ++j) buf[wave * per + q * NP + j] = s[q][j];
-    __syncthreads();
-    const int first = ROWS ? wave & ~(waves - 1) : 0;
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-#pragma unroll
-      for (int j = 0; j < NP; ++j) s[q][j] = 0;
-    for (int w = first; w < first + waves; ++w)
-#pragma unroll
-      for (int q = 0; q < Q; ++q)
-#pragma unroll
-        for (int j = 0; j < NP; ++j) s[q][j] += buf[w * per + q * NP + j];
+    constexpr int N = Q * NP;
+    float* buf = lds + (round & 1) * (WAVES * (ROWS ? 1 : lanes()) * MAX_Q * NP);
     ++round;
+    if (ROWS) {
+      if (lane == 0)
+#pragma unroll
+        for (int q = 0; q < Q; ++q) buf[wave * N + q] = s[q][0];
+      lds_barrier();
+      const int w = (wave & ~(waves - 1)) + (lane & (waves - 1));
+#pragma unroll
+      for (int q = 0; q < Q; ++q) s[q][0] = buf[w * N + q];
+      lanes_sum<N>(&s[0][0], 1, waves);
+    } else {
+      // slots of waves that the workgroup does not have hold zeros: all eight reads go out together
+      const int per = lanes() * N;
+      if (UNI || lane < lanes())
+#pragma unroll
+        for (int i = 0; i < N; ++i) buf[wave * per + l * N + i] = s[i / NP][i % NP];
+      lds_barrier();
+      float v[WAVES][N];
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[w][i] = buf[w * per + l * N + i];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float sum = v[0][i];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sum += v[w][i];
+        s[i / NP][i % NP] = sum;
+      }
+    }
   }
   __device__ __forceinline__ void centre(float* z, const float* mean) const {
     if (cfull)
@@ -392,16 +425,16 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
     const int per_row = a.lanes > 64 ? a.lanes >> 6 : 1, waves = (int)blockDim.x >> 6;
     const bool first = wave < per_row && lane < a.lanes;
     if (waves > per_row) {
-      __syncthreads();                   // the buffer may still be read as a reduction's
+      lds_barrier();                   // the buffer may still be read as a reduction's
       if (lane < a.lanes)
 #pragma unroll
         for (int i = 0; i < NW; ++i) lds[(wave * NW + i) * 64 + lane] = acc[i];
-      __syncthreads();
+      lds_barrier();
       if (first)
         for (int w = wave + per_row; w < waves; w += per_row)
 #pragma unroll
           for (int i = 0; i < NW; ++i) acc[i] += lds[(w * NW + i) * 64 + lane];
-      __syncthreads();
+      lds_barrier();
     }
     if (first) {
       if (cfull) {
@@ -426,26 +459,31 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
   if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0);
   for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
     const int img = item / a.slices;
-    const int64_t lo = (item - img * a.slices) * a.len;
-    const int64_t hi = lo + a.len < a.P ? lo + a.len : a.P;
+    const int64_t first = (int64_t)(item - img * a.slices) * t.tile(), step = (int64_t)a.slices * t.tile();
     if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img);
-    for (int64_t base = lo; base < hi; base += t.tile()) {
-      t.at(img, base, hi);
+    for (int64_t base = first; base < a.P; base += step) {
+      const typename Th::Pos o = t.at(img, base, a.P);
       typename Th::Raw xr[K], fr[K], qr[K];
       float y[Th::E], r[Th::NP];
       if (d.f) {
-        t.read(d.f, d.f_stride, fr);
-        t.read(d.x, d.x_stride, xr);
-        if (FULL) t.read(d.gate, d.gate_stride, qr);
+        t.read(d.f, d.f_stride, fr, o);
+        t.read(d.x, d.x_stride, xr, o);
+        if (FULL) t.read(d.gate, d.gate_stride, qr, o);
+        if (!o.full) {
+          t.drop_dups(fr, o);
+          t.drop_dups(xr, o);
+          if (FULL) t.drop_dups(qr, o);
+        }
         float n[Th::E];
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) n[e] = element<V>(fr[e / V], e % V);
         if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r);
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) y[e] = element<V>(xr[e / V], e % V) + t.template branch_value<FULL>(e, n[e], qr);
-        t.write(d.y, d.y_stride, y);
+        t.write(d.y, d.y_stride, y, o);
       } else {
-        t.read(d.x, d.x_stride, xr);
+        t.read(d.x, d.x_stride, xr, o);
+        if (!o.full) t.drop_dups(xr, o);
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) y[e] = element<V>(xr[e / V], e % V);
       }
@@ -453,7 +491,7 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
         t.normalise(y, d.pre_kind, d.pre_eps, r);
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) y[e] = BIAS ? y[e] * t.w1(e) + t.b1(e) : y[e] * t.w1(e);
-        t.write(d.h, d.h_stride, y);
+        t.write(d.h, d.h_stride, y, o);
       }
     }
   }
@@ -466,10 +504,7 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
 // and where G is the same for all pixels of an image (or is 1) all three follow from sum D n and sum D: two
 // accumulators a channel instead of three.  A full gate takes G D in D's place and writes its own gradient.
 template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS>
-#ifndef BWD_ATTR
-#define BWD_ATTR
-#endif
-__global__ __launch_bounds__(THREADS) BWD_ATTR void resnorm_bwd_kernel(const Args a) {
+__global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
   extern __shared__ float lds[];
   typedef Thread<T, ROWS, UNI, K, V, BIAS> Th;
   Th t(a, lds);
@@ -480,17 +515,23 @@ __global__ __launch_bounds__(THREADS) BWD_ATTR void resnorm_bwd_kernel(const Arg
   if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0);
   for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
     const int img = item / a.slices;
-    const int64_t lo = (item - img * a.slices) * a.len;
-    const int64_t hi = lo + a.len < a.P ? lo + a.len : a.P;
+    const int64_t first = (int64_t)(item - img * a.slices) * t.tile(), step = (int64_t)a.slices * t.tile();
     if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img);
-    for (int64_t base = lo; base < hi; base += t.tile()) {
-      t.at(img, base, hi);
+    for (int64_t base = first; base < a.P; base += step) {
+      const typename Th::Pos o = t.at(img, base, a.P);
       typename Th::Raw xr[K], fr[K], qr[K], dyr[K], dhr[K];
-      if (d.f) t.read(d.f, d.f_stride, fr);
-      if (d.dh) t.read(d.x, d.x_stride, xr);
-      if (FULL) t.read(d.gate, d.gate_stride, qr);
-      if (d.dh) t.read(d.dh, d.dh_stride, dhr);
-      if (d.dy) t.read(d.dy, d.dy_stride, dyr);
+      if (d.f) t.read(d.f, d.f_stride, fr, o);
+      if (d.dh) t.read(d.x, d.x_stride, xr, o);
+      if (FULL) t.read(d.gate, d.gate_stride, qr, o);
+      if (d.dh) t.read(d.dh, d.dh_stride, dhr, o);
+      if (d.dy) t.read(d.dy, d.dy_stride, dyr, o);
+      if (!o.full) {
+        t.drop_dups(fr, o);
+        t.drop_dups(xr, o);
+        if (FULL) t.drop_dups(qr, o);
+        t.drop_dups(dhr, o);
+        t.drop_dups(dyr, o);
+      }
       float D[Th::E], n[Th::E], r[Th::NP], r2[Th::NP];
       float s[2][Th::NP];
       if (d.f) {
@@ -537,9 +578,9 @@ __global__ __launch_bounds__(THREADS) BWD_ATTR void resnorm_bwd_kernel(const Arg
           if (BIAS) s_dh[Th::wi(e)] += g;
           D[e] = r[Th::pix(e)] * (g * t.w1(e) - ny * s[1][Th::pix(e)] - mean_g[Th::pix(e)]);
         }
-        if (!t.full)                  // what a mean's offset leaves where there is nothing
+        if (!o.full)                  // what a mean's offset leaves where there is nothing
 #pragma unroll
-          for (int e = 0; e < Th::E; ++e) D[e] = e % V < t.dropped(e / V) ? 0.f : D[e];
+          for (int e = 0; e < Th::E; ++e) D[e] = e % V < t.dropped(e / V, o) ? 0.f : D[e];
         if (d.dy)
 #pragma unroll
           for (int e = 0; e < Th::E; ++e) D[e] += element<V>(dyr[e / V], e % V);
@@ -547,7 +588,7 @@ __global__ __launch_bounds__(THREADS) BWD_ATTR void resnorm_bwd_kernel(const Arg
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) D[e] = element<V>(dyr[e / V], e % V);
       }
-      if (d.dx) t.write(d.dx, d.dx_stride, D);
+      if (d.dx) t.write(d.dx, d.dx_stride, D, o);
       if (d.f) {
         if (FULL) {
           float dq[Th::E];
@@ -557,7 +598,7 @@ __global__ __launch_bounds__(THREADS) BWD_ATTR void resnorm_bwd_kernel(const Arg
             dq[e] = D[e] * (BIAS ? t.gw(e) * n[e] + t.gb(e) : t.gw(e) * n[e]) * (d.gate_act ? G * (1.f - G) : 1.f);
             D[e] *= G;
           }
-          if (d.dgate) t.write(d.dgate, d.dgate_stride, dq);
+          if (d.dgate) t.write(d.dgate, d.dgate_stride, dq, o);
         }
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) {
@@ -577,7 +618,7 @@ __global__ __launch_bounds__(THREADS) BWD_ATTR void resnorm_bwd_kernel(const Arg
 #pragma unroll
             for (int e = 0; e < Th::E; ++e) D[e] = r2[Th::pix(e)] * (D[e] - n[e] * s[0][Th::pix(e)] - s[1][Th::pix(e)]);
           }
-          t.write(d.df, d.df_stride, D);
+          t.write(d.df, d.df_stride, D, o);
         }
       }
     }
