@@ -1,5 +1,6 @@
 // Norms around a gated residual branch: argument checks, decomposition, and the join of the sums over pixels.  The kernels
 // are in resnorm_kernels.h.
+#include <float.h>
 #include "resnorm_kernels.h"
 
 using namespace resnorm;
@@ -107,21 +108,24 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     p.threads = 64 * ((groups * p.a.lanes + 63) / 64);
     tile = p.a.lanes * PLANES_V;
   }
-  // Workgroups walk the tiles side by side: neighbours in time are neighbours in memory.  (Shares of consecutive tiles, each
-  // a power of two apart, keep all workgroups on the same few memory channels: 64 x 64 x 128 x 128 bf16 maps ran backward
-  // in WALK_BEFORE us that way, in WALK_AFTER us this way.)  With a gate for each image an item stays within its image, so that its sums
-  // are the image's.
-  const int64_t tiles = (p.a.P + tile - 1) / tile, most = backward ? 512 : 4096;
+  // Workgroups walk the tiles side by side, neighbours in time being neighbours in memory.  With a gate for each image an item
+  // stays within its image, so that its sums are the image's.
+  // Backward: as many workgroups as run at once, since each pays for its start, its sums over the lanes and its partial sums
+  // (about 9 us): 16 waves a compute unit for rows of root mean squares (113 registers), 8 otherwise.
+  const int64_t tiles = (p.a.P + tile - 1) / tile;
+  const int64_t most = !backward ? 4096 : 256 * (rows && p.elems == 8 && !general(d) && d.gate_mode != GATE_FULL ? 1024 : 512) / p.threads;
   int64_t s = tiles;
   if (image_gate && p.images > 0 && s > (most + p.images - 1) / p.images) s = (most + p.images - 1) / p.images;
   if (p.images > 0 && s > (1LL << 30) / p.images) s = (1LL << 30) / p.images;
   p.a.slices = s < 1 ? 1 : (int)s;
   p.a.items = p.a.P > 0 ? p.images * p.a.slices : 0;
   p.workgroups = (int)(p.a.items < most ? p.a.items : most);
+  p.a.jump_images = p.workgroups / p.a.slices;
+  p.a.jump_shares = p.workgroups % p.a.slices;
   const int waves = p.threads / 64;
   int bytes = 2 * WAVES * MAX_Q * (rows ? 1 : p.a.lanes * PLANES_V) * 4;            // two buffers of a reduction: at most 16 KB
   if (!rows) bytes += p.threads / p.a.lanes * PLANES_K * 16;                        // weights: at most 16 KB
-  if (backward && rows && p.a.lanes < p.threads && bytes < waves * p.elems * 64 * 4) bytes = waves * p.elems * 64 * 4;     // flush: at most 32 KB
+  if (backward && rows && p.a.lanes < p.threads && bytes < waves * p.elems * 128 * 4) bytes = waves * p.elems * 128 * 4;   // flush: at most 64 KB
   p.lds_bytes = bytes;
 }
 
@@ -134,7 +138,7 @@ int check(const char* what, const srx_resnorm_desc* d) {
   SRX_CHECK_ARG(d->C <= most, "%s: %d channels, at most %d in this layout", what, d->C, most);
   SRX_CHECK_ARG(d->post_kind >= 0 && d->post_kind <= 2 && d->pre_kind >= 0 && d->pre_kind <= 2, "%s: bad norm kind", what);
   SRX_CHECK_ARG(d->gate_mode >= 0 && d->gate_mode <= 3 && (d->gate_act == 0 || d->gate_act == 1), "%s: bad gate mode", what);
-  SRX_CHECK_ARG((!d->post_kind || d->post_eps > 0) && (!d->pre_kind || d->pre_eps > 0), "%s: eps must be positive", what);
+  SRX_CHECK_ARG((!d->post_kind || d->post_eps >= FLT_MIN) && (!d->pre_kind || d->pre_eps >= FLT_MIN), "%s: eps must be positive (a normal number)", what);
   SRX_CHECK_ARG(d->f || (!d->post_kind && !d->gate_mode), "%s: a norm after the branch or a gate without a branch", what);
   SRX_CHECK_ARG(d->f || d->pre_kind, "%s: neither a branch nor a norm", what);
   SRX_CHECK_ARG(!d->gate_mode || d->gate, "%s: null gate", what);
@@ -193,7 +197,7 @@ int srx_resnorm_backward(const srx_resnorm_desc* d, void* stream) {
     if (int rc = d->dtype == SRX_BF16 ? launch_bf16(p, 1, s) : launch_f32(p, 1, s)) return rc;
   const bool sums = d->dw_pre || d->db_pre || (d->f && (d->dw_post || d->db_post || (d->dgate && d->gate_mode && d->gate_mode != GATE_FULL)));
   if (!sums) return SRX_OK;
-  hipLaunchKernelGGL(resnorm_join_kernel, dim3((d->C + JOIN_X - 1) / JOIN_X), dim3(JOIN_X * JOIN_Y), 0, s, p.a, p.workgroups, p.images, has_bias(*d));
+  hipLaunchKernelGGL(resnorm_join_kernel, dim3((d->C + JOIN_X - 1) / JOIN_X), dim3(JOIN_X * JOIN_Y), 0, s, p.a, p.workgroups, p.images, general(*d));
   return srx_check_launch("resnorm_join");
 }
 

@@ -31,6 +31,15 @@ struct Args {
   int64_t P;            // pixels of an "image" (rows without per-image gate: all rows are one image)
   float* part_pre;      // [workgroups][2][C]
   float* part_post;     // [workgroups or items][2][C]
+  int jump_images, jump_shares;       // from a workgroup's item to its next: workgroups / slices, workgroups % slices
+  __device__ __forceinline__ void next(int& image, int& share) const {
+    image += jump_images;
+    share += jump_shares;
+    if (share >= slices) {
+      share -= slices;
+      ++image;
+    }
+  }
 };
 struct Plan {
   Args a;
@@ -81,6 +90,8 @@ template <int V> __device__ __forceinline__ Vec<bf16, V> packed(const float* v, 
     }
   return z;
 }
+// within 2^-22 of the value; eps is a normal number, so the argument is one too
+__device__ __forceinline__ float rsqrt_hw(float x) { return __builtin_amdgcn_rsqf(x); }
 __device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
 
 // A barrier for what waves hand each other through LDS, and only that: __syncthreads() would also wait for every global load
@@ -129,10 +140,10 @@ template <int N> __device__ __forceinline__ void lanes_sum(float* v, int lo, int
 
 // Every load is a whole vector that lies inside the tensor, without a branch: one that would pass the end (of a row; of
 // a plane; a row or channel that does not exist) starts earlier, and the elements in front of the thread's own, `dup` of
-// them, are zeros from then on.  BIAS: some norm has a bias (else: no offsets, and no sums for them).
+// them, are zeros from then on.  GEN: some norm has a bias (else: no offsets, and no sums for them).
 // UNI (planes with 64 lanes along the pixels): a wave's lanes hold the same channels, so that channels, their addresses
 // and their weights are scalars.
-template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Thread {
+template <typename T, bool ROWS, bool UNI, int K, int V, bool GEN> struct Thread {
   static constexpr int E = K * V;                     // elements of each tensor
   static constexpr int NP = ROWS ? 1 : V;             // pixels
   static constexpr int NW = ROWS ? E : K;             // channels
@@ -151,13 +162,14 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
   };
   const Args& a;
   float* lds;                 // reductions
-  float* lw;                  // planes: weights by channel: gw, gb, w1, b1 (BIAS) or gw, w1
+  float* lw;                  // planes: weights by channel: gw, gb, w1, b1 (GEN) or gw, w1
   int round;
   int lane, wave, l;          // l = thread within the row / lane along the pixels
   int grp;                    // the thread's row of the workgroup / group of K channels
   int cb;                     // planes: first channel that is read: of the last group, like a vector's, such that all K exist
   int rdup[ROWS ? K : 1];     // rows: elements of step k that are not the thread's; planes: channels of the group that are not
   bool cfull;                 // nothing is dropped in this wave because of the channels
+  unsigned off0;              // planes: Pos::off within a whole tile
   float gw_[NL], gb_[NL], w1_[NL], b1_[NL];
 
   __device__ __forceinline__ Thread(const Args& a_, float* lds_) : a(a_), lds(lds_), round(0) {
@@ -180,6 +192,7 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
       ok = rdup[0] == 0;
     }
     cfull = __all(ok);
+    off0 = ((unsigned)(l * V) + (ROWS || UNI ? 0u : (unsigned)cb * (unsigned)a.P)) * (unsigned)sizeof(T);
     const int floats = 2 * WAVES * MAX_Q * (ROWS ? 1 : lanes() * V);
     lw = lds + floats;
     if (!ROWS && (int)blockDim.x < THREADS) {
@@ -207,16 +220,23 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
   __device__ __forceinline__ Pos at(int64_t img, int64_t base, int64_t end) const {
     Pos o;
     o.image = img;
+    o.base = base;
+    o.pdup = 0;
+    o.full = cfull;
+    if (base + tile() <= end) {
+      if (ROWS) o.row = img * a.P + base + grp;
+      else o.off = off0;
+      return o;
+    }
     const int64_t want = base + (ROWS ? grp : l * V), last = end - (ROWS ? 1 : V);
     if (ROWS) {
       o.row = img * a.P + (want < last ? want : last);
       o.pdup = want > last ? V : 0;
-      o.base = base;
     } else {
       // where less than a vector is left behind the tile's start, the tile starts earlier
       const int64_t from = want < last ? want : last;
       o.pdup = want - from < V ? (int)(want - from) : V;
-      o.base = base < last ? base : last;
+      if (base > last) o.base = last;
       o.off = ((unsigned)(from - o.base) + (UNI ? 0u : (unsigned)cb * (unsigned)a.P)) * (unsigned)sizeof(T);
     }
     o.full = cfull && __all(o.pdup == 0);
@@ -277,14 +297,14 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
     float G[N], w[N], b[N];
     weights<N>(gated ? static_cast<const float*>(d.gate) + (d.gate_mode == GATE_IMAGE ? img * d.C : 0) : nullptr, 1.f, c, G);
     weights<N>(d.w_post, 1.f, c, w);
-    if (BIAS) weights<N>(d.b_post, 0.f, c, b);
+    if (GEN) weights<N>(d.b_post, 0.f, c, b);
     if (gated && d.gate_act)
 #pragma unroll
       for (int j = 0; j < N; ++j) G[j] = sigmoid(G[j]);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       gw[j] = d.scale * G[j] * w[j];
-      if (BIAS) gb[j] = d.scale * G[j] * b[j];
+      if (GEN) gb[j] = d.scale * G[j] * b[j];
     }
   }
   // (an element that is not the thread's has n = 0 and dh = 0; its weights count only through offsets)
@@ -292,7 +312,7 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
     if constexpr (ROWS) {
 #pragma unroll
       for (int k = 0; k < K; ++k) branch_weights<V>(img, ch(k), gw_ + k * V, gb_ + k * V);
-      if (BIAS && !cfull)
+      if (GEN && !cfull)
 #pragma unroll
         for (int e = 0; e < E; ++e) gb_[e] = chan_ok(e) ? gb_[e] : 0.f;
     } else {
@@ -300,8 +320,8 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
       for (int c = threadIdx.x; c < a.d.C; c += blockDim.x) {
         float g, b;
         branch_weights<1>(img, c, &g, &b);
-        lw[c * (BIAS ? 4 : 2)] = g;
-        if (BIAS) lw[c * 4 + 1] = b;
+        lw[c * (GEN ? 4 : 2)] = g;
+        if (GEN) lw[c * 4 + 1] = b;
       }
       lds_barrier();
     }
@@ -312,20 +332,20 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         weights<V>(d.w_pre, 1.f, ch(k), w1_ + k * V);
-        if (BIAS) weights<V>(d.b_pre, 0.f, ch(k), b1_ + k * V);
+        if (GEN) weights<V>(d.b_pre, 0.f, ch(k), b1_ + k * V);
       }
     } else {
       for (int c = threadIdx.x; c < d.C; c += blockDim.x) {
-        lw[c * (BIAS ? 4 : 2) + (BIAS ? 2 : 1)] = d.w_pre ? d.w_pre[c] : 1.f;
-        if (BIAS) lw[c * 4 + 3] = d.b_pre ? d.b_pre[c] : 0.f;
+        lw[c * (GEN ? 4 : 2) + (GEN ? 2 : 1)] = d.w_pre ? d.w_pre[c] : 1.f;
+        if (GEN) lw[c * 4 + 3] = d.b_pre ? d.b_pre[c] : 0.f;
       }
       lds_barrier();
     }
   }
-  __device__ __forceinline__ float gw(int e) const { return ROWS ? gw_[e % NL] : lw[ch(e / V) * (BIAS ? 4 : 2)]; }
-  __device__ __forceinline__ float gb(int e) const { return !BIAS ? 0.f : ROWS ? gb_[e % NL] : cdup(e / V) ? 0.f : lw[ch(e / V) * 4 + 1]; }
-  __device__ __forceinline__ float w1(int e) const { return ROWS ? w1_[e % NL] : lw[ch(e / V) * (BIAS ? 4 : 2) + (BIAS ? 2 : 1)]; }
-  __device__ __forceinline__ float b1(int e) const { return !BIAS ? 0.f : ROWS ? b1_[e % NL] : lw[ch(e / V) * 4 + 3]; }
+  __device__ __forceinline__ float gw(int e) const { return ROWS ? gw_[e % NL] : lw[ch(e / V) * (GEN ? 4 : 2)]; }
+  __device__ __forceinline__ float gb(int e) const { return !GEN ? 0.f : ROWS ? gb_[e % NL] : cdup(e / V) ? 0.f : lw[ch(e / V) * 4 + 1]; }
+  __device__ __forceinline__ float w1(int e) const { return ROWS ? w1_[e % NL] : lw[ch(e / V) * (GEN ? 4 : 2) + (GEN ? 2 : 1)]; }
+  __device__ __forceinline__ float b1(int e) const { return !GEN ? 0.f : ROWS ? b1_[e % NL] : lw[ch(e / V) * 4 + 3]; }
 
   // ---- sums over the channels: of Q quantities, one value for each of the thread's pixels
   template <int Q> __device__ __forceinline__ void reduce(float (&s)[Q][NP]) {
@@ -381,7 +401,7 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
   __device__ __forceinline__ void normalise(float* z, int kind, float eps, float* r) {
     const float inv = 1.f / (float)a.d.C;
     float s[1][NP];
-    if (kind == KIND_LAYER) {
+    if (GEN && kind == KIND_LAYER) {
 #pragma unroll
       for (int j = 0; j < NP; ++j) s[0][j] = 0;
 #pragma unroll
@@ -397,70 +417,107 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool BIAS> struct Threa
     for (int e = 0; e < E; ++e) s[0][pix(e)] += z[e] * z[e];
     reduce<1>(s);
 #pragma unroll
-    for (int j = 0; j < NP; ++j) r[j] = 1.f / sqrtf(s[0][j] * inv + eps);
+    for (int j = 0; j < NP; ++j) r[j] = rsqrt_hw(s[0][j] * inv + eps);
 #pragma unroll
     for (int e = 0; e < E; ++e) z[e] *= r[pix(e)];
   }
   // u of one element; q: the full gate's raw values
   template <bool FULL> __device__ __forceinline__ float branch_value(int e, float n, const Raw* q) const {
-    float u = BIAS ? gw(e) * n + gb(e) : gw(e) * n;
+    float u = GEN ? gw(e) * n + gb(e) : gw(e) * n;
     if (FULL) {
       const float g = element<V>(q[e / V], e % V);
       u *= a.d.gate_act ? sigmoid(g) : g;
     }
     return u;
   }
-  // sum the thread's per-channel values over the workgroup and write them to out[C]
-  __device__ __forceinline__ void flush(float* acc, float* out) {
+  // sum the thread's per-channel values over the workgroup and write them to out[C] (GEN: and a second set behind it)
+  __device__ __forceinline__ void flush(float* first_set, float* second_set, float* out) {
+    constexpr int Q = GEN ? 2 : 1;
+    float* const sets[2] = {first_set, second_set};
     if (!ROWS) {
-      lanes_sum<NW>(acc, 1, lanes());
-      if (l == 0)
 #pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (cdup(k) == 0) out[ch(k)] = acc[k];
+      for (int q = 0; q < Q; ++q) {
+        lanes_sum<NW>(sets[q], 1, lanes());
+        if (l == 0)
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (cdup(k) == 0) out[q * a.d.C + ch(k)] = sets[q][k];
+      }
       return;
     }
-    if (a.lanes < 64) lanes_sum<NW>(acc, a.lanes, 64);
+    if (a.lanes < 64)
+#pragma unroll
+      for (int q = 0; q < Q; ++q) lanes_sum<NW>(sets[q], a.lanes, 64);
     // waves that hold the same channels: every (lanes / 64)-th
     const int per_row = a.lanes > 64 ? a.lanes >> 6 : 1, waves = (int)blockDim.x >> 6;
     const bool first = wave < per_row && lane < a.lanes;
     if (waves > per_row) {
-      lds_barrier();                   // the buffer may still be read as a reduction's
+      lds_barrier();                     // the buffer may still be read as a reduction's
       if (lane < a.lanes)
 #pragma unroll
-        for (int i = 0; i < NW; ++i) lds[(wave * NW + i) * 64 + lane] = acc[i];
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+          for (int i = 0; i < NW; ++i) lds[((wave * Q + q) * NW + i) * 64 + lane] = sets[q][i];
       lds_barrier();
       if (first)
         for (int w = wave + per_row; w < waves; w += per_row)
 #pragma unroll
-          for (int i = 0; i < NW; ++i) acc[i] += lds[(w * NW + i) * 64 + lane];
+          for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int i = 0; i < NW; ++i) sets[q][i] += lds[((w * Q + q) * NW + i) * 64 + lane];
       lds_barrier();
     }
-    if (first) {
-      if (cfull) {
+    if (first)
 #pragma unroll
-        for (int k = 0; k < K; ++k) *reinterpret_cast<Vec<float, V>*>(out + ch(k)) = packed<V>(acc + k * V, out);
-      } else {
+      for (int q = 0; q < Q; ++q) {
+        float* const to = out + q * a.d.C;
+        if (cfull) {
 #pragma unroll
-        for (int i = 0; i < NW; ++i)
-          if (chan_ok(i)) out[chan(i)] = acc[i];
+          for (int k = 0; k < K; ++k) *reinterpret_cast<Vec<float, V>*>(to + ch(k)) = packed<V>(sets[q] + k * V, to);
+        } else {
+#pragma unroll
+          for (int i = 0; i < NW; ++i)
+            if (chan_ok(i)) to[chan(i)] = sets[q][i];
+        }
       }
-    }
   }
 };
 
-template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS>
+// When the weights are fetched: once, and again where the gate is another image's.  Maps do it after their first tile's loads
+// are on their way (16 x 64 x 64 x 64 bf16: forward 8.8 -> 8.5 us, backward 24.4 -> 22.2), rows in front of them: their
+// weights are registers, which a branch in the loop would tie up (4096 x 1024 bf16: forward 8.6 against 9.3 us).
+template <typename Th, bool ROWS> struct WeightsOf {
+  Th& t;
+  const bool has_branch, has_norm;
+  int image = -1;
+  __device__ __forceinline__ WeightsOf(Th& t_, bool f, bool n) : t(t_), has_branch(f), has_norm(n) {
+    if (!ROWS) return;
+    if (has_norm) t.norm_weights();
+    if (has_branch && t.a.d.gate_mode != GATE_IMAGE) t.branch(0);
+  }
+  __device__ __forceinline__ void item(int img) {
+    if (ROWS && has_branch && t.a.d.gate_mode == GATE_IMAGE) t.branch(img);
+  }
+  __device__ __forceinline__ void tile(int img) {
+    if (ROWS) return;
+    if (image < 0 && has_norm) t.norm_weights();
+    if (has_branch && (image < 0 || (t.a.d.gate_mode == GATE_IMAGE && image != img))) t.branch(img);
+    image = img;
+  }
+};
+
+template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool GEN>
 __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
   extern __shared__ float lds[];
-  typedef Thread<T, ROWS, UNI, K, V, BIAS> Th;
+  typedef Thread<T, ROWS, UNI, K, V, GEN> Th;
   Th t(a, lds);
   const srx_resnorm_desc& d = a.d;
-  if (d.pre_kind) t.norm_weights();
-  if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0);
-  for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
-    const int img = item / a.slices;
-    const int64_t first = (int64_t)(item - img * a.slices) * t.tile(), step = (int64_t)a.slices * t.tile();
-    if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img);
+  const int64_t step = (int64_t)a.slices * t.tile();
+  int img = blockIdx.x / a.slices, share = blockIdx.x - img * a.slices;
+  WeightsOf<Th, ROWS> w(t, d.f, d.pre_kind);
+  for (int item = blockIdx.x; item < a.items; item += gridDim.x, a.next(img, share)) {
+    w.item(img);
+    const int64_t first = (int64_t)share * t.tile();
     for (int64_t base = first; base < a.P; base += step) {
       const typename Th::Pos o = t.at(img, base, a.P);
       typename Th::Raw xr[K], fr[K], qr[K];
@@ -469,6 +526,7 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
         t.read(d.f, d.f_stride, fr, o);
         t.read(d.x, d.x_stride, xr, o);
         if (FULL) t.read(d.gate, d.gate_stride, qr, o);
+        w.tile(img);
         if (!o.full) {
           t.drop_dups(fr, o);
           t.drop_dups(xr, o);
@@ -483,6 +541,7 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
         t.write(d.y, d.y_stride, y, o);
       } else {
         t.read(d.x, d.x_stride, xr, o);
+        w.tile(img);
         if (!o.full) t.drop_dups(xr, o);
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) y[e] = element<V>(xr[e / V], e % V);
@@ -490,7 +549,7 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
       if (d.pre_kind) {
         t.normalise(y, d.pre_kind, d.pre_eps, r);
 #pragma unroll
-        for (int e = 0; e < Th::E; ++e) y[e] = BIAS ? y[e] * t.w1(e) + t.b1(e) : y[e] * t.w1(e);
+        for (int e = 0; e < Th::E; ++e) y[e] = GEN ? y[e] * t.w1(e) + t.b1(e) : y[e] * t.w1(e);
         t.write(d.h, d.h_stride, y, o);
       }
     }
@@ -503,28 +562,33 @@ __global__ __launch_bounds__(THREADS) void resnorm_fwd_kernel(const Args a) {
 //   d w_post = s sum G D n,   d b_post = s sum G D,   d G = s sum D (w n + b),
 // and where G is the same for all pixels of an image (or is 1) all three follow from sum D n and sum D: two
 // accumulators a channel instead of three.  A full gate takes G D in D's place and writes its own gradient.
-template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS>
+//
+// ALL: every tensor is there (the pass between two branches), which the compiler has to know to wait for one tensor's loads
+// and not for all that may have been issued.  (Reading the next tile while one is computed gained nothing: 177.7 us with and
+// without it for 64 maps of 64 x 128 x 128 in bf16.)
+template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool GEN, bool ALL>
 __global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
   extern __shared__ float lds[];
-  typedef Thread<T, ROWS, UNI, K, V, BIAS> Th;
+  typedef Thread<T, ROWS, UNI, K, V, GEN> Th;
   Th t(a, lds);
   const srx_resnorm_desc& d = a.d;
+  const bool has_f = ALL || d.f, has_dh = ALL || d.dh, has_dy = ALL || d.dy;
   const float inv = 1.f / (float)d.C;
   float s_dhn[Th::NW] = {}, s_dh[Th::NW] = {}, s_dn[Th::NW] = {}, s_d[Th::NW] = {};
-  if (d.dh) t.norm_weights();
-  if (d.f && d.gate_mode != GATE_IMAGE) t.branch(0);
-  for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
-    const int img = item / a.slices;
-    const int64_t first = (int64_t)(item - img * a.slices) * t.tile(), step = (int64_t)a.slices * t.tile();
-    if (d.f && d.gate_mode == GATE_IMAGE) t.branch(img);
-    for (int64_t base = first; base < a.P; base += step) {
+  const int64_t step = (int64_t)a.slices * t.tile();
+  int img = blockIdx.x / a.slices, share = blockIdx.x - img * a.slices;
+  WeightsOf<Th, ROWS> w(t, has_f, has_dh);
+  for (int item = blockIdx.x; item < a.items; item += gridDim.x, a.next(img, share)) {
+    w.item(img);
+    for (int64_t base = (int64_t)share * t.tile(); base < a.P; base += step) {
       const typename Th::Pos o = t.at(img, base, a.P);
       typename Th::Raw xr[K], fr[K], qr[K], dyr[K], dhr[K];
-      if (d.f) t.read(d.f, d.f_stride, fr, o);
-      if (d.dh) t.read(d.x, d.x_stride, xr, o);
+      if (has_f) t.read(d.f, d.f_stride, fr, o);
+      if (has_dh) t.read(d.x, d.x_stride, xr, o);
       if (FULL) t.read(d.gate, d.gate_stride, qr, o);
-      if (d.dh) t.read(d.dh, d.dh_stride, dhr, o);
-      if (d.dy) t.read(d.dy, d.dy_stride, dyr, o);
+      if (has_dh) t.read(d.dh, d.dh_stride, dhr, o);
+      if (has_dy) t.read(d.dy, d.dy_stride, dyr, o);
+      w.tile(img);
       if (!o.full) {
         t.drop_dups(fr, o);
         t.drop_dups(xr, o);
@@ -534,21 +598,21 @@ __global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
       }
       float D[Th::E], n[Th::E], r[Th::NP], r2[Th::NP];
       float s[2][Th::NP];
-      if (d.f) {
+      if (has_f) {
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) n[e] = element<V>(fr[e / V], e % V);
         if (d.post_kind) t.normalise(n, d.post_kind, d.post_eps, r2);
       }
-      if (d.dh) {
+      if (has_dh) {
         float mean_g[Th::NP] = {};
         // y, in D's place for now
-        if (d.f)
+        if (has_f)
 #pragma unroll
           for (int e = 0; e < Th::E; ++e) D[e] = element<V>(xr[e / V], e % V) + t.template branch_value<FULL>(e, n[e], qr);
         else
 #pragma unroll
           for (int e = 0; e < Th::E; ++e) D[e] = element<V>(xr[e / V], e % V);
-        if (d.pre_kind == KIND_LAYER) {
+        if (GEN && d.pre_kind == KIND_LAYER) {
 #pragma unroll
           for (int j = 0; j < Th::NP; ++j) s[0][j] = s[1][j] = 0;
 #pragma unroll
@@ -568,34 +632,34 @@ __global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
         t.template reduce<2>(s);
 #pragma unroll
         for (int j = 0; j < Th::NP; ++j) {
-          r[j] = 1.f / sqrtf(s[0][j] * inv + d.pre_eps);
+          r[j] = rsqrt_hw(s[0][j] * inv + d.pre_eps);
           s[1][j] *= inv * r[j];
         }
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) {
           const float g = element<V>(dhr[e / V], e % V), ny = D[e] * r[Th::pix(e)];
           s_dhn[Th::wi(e)] += g * ny;
-          if (BIAS) s_dh[Th::wi(e)] += g;
-          D[e] = r[Th::pix(e)] * (g * t.w1(e) - ny * s[1][Th::pix(e)] - mean_g[Th::pix(e)]);
+          if (GEN) s_dh[Th::wi(e)] += g;
+          D[e] = r[Th::pix(e)] * (GEN ? g * t.w1(e) - ny * s[1][Th::pix(e)] - mean_g[Th::pix(e)] : g * t.w1(e) - ny * s[1][Th::pix(e)]);
         }
-        if (!o.full)                  // what a mean's offset leaves where there is nothing
+        if (GEN && !o.full)           // what a mean's offset leaves where there is nothing
 #pragma unroll
           for (int e = 0; e < Th::E; ++e) D[e] = e % V < t.dropped(e / V, o) ? 0.f : D[e];
-        if (d.dy)
+        if (has_dy)
 #pragma unroll
           for (int e = 0; e < Th::E; ++e) D[e] += element<V>(dyr[e / V], e % V);
       } else {
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) D[e] = element<V>(dyr[e / V], e % V);
       }
-      if (d.dx) t.write(d.dx, d.dx_stride, D, o);
-      if (d.f) {
+      if (ALL || d.dx) t.write(d.dx, d.dx_stride, D, o);
+      if (has_f) {
         if (FULL) {
           float dq[Th::E];
 #pragma unroll
           for (int e = 0; e < Th::E; ++e) {
             const float q = element<V>(qr[e / V], e % V), G = d.gate_act ? sigmoid(q) : q;
-            dq[e] = D[e] * (BIAS ? t.gw(e) * n[e] + t.gb(e) : t.gw(e) * n[e]) * (d.gate_act ? G * (1.f - G) : 1.f);
+            dq[e] = D[e] * (GEN ? t.gw(e) * n[e] + t.gb(e) : t.gw(e) * n[e]) * (d.gate_act ? G * (1.f - G) : 1.f);
             D[e] *= G;
           }
           if (d.dgate) t.write(d.dgate, d.dgate_stride, dq, o);
@@ -603,59 +667,62 @@ __global__ __launch_bounds__(THREADS) void resnorm_bwd_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < Th::E; ++e) {
           s_dn[Th::wi(e)] += D[e] * n[e];
-          if (BIAS) s_d[Th::wi(e)] += D[e];
+          if (GEN) s_d[Th::wi(e)] += D[e];
           D[e] *= t.gw(e);
         }
-        if (d.df) {
+        if (ALL || d.df) {
           if (d.post_kind) {
 #pragma unroll
             for (int j = 0; j < Th::NP; ++j) s[0][j] = s[1][j] = 0;
 #pragma unroll
-            for (int e = 0; e < Th::E; ++e) { s[0][Th::pix(e)] += D[e] * n[e]; s[1][Th::pix(e)] += D[e]; }
-            t.template reduce<2>(s);
+            for (int e = 0; e < Th::E; ++e) {
+              s[0][Th::pix(e)] += D[e] * n[e];
+              if (GEN) s[1][Th::pix(e)] += D[e];
+            }
+            if (GEN) t.template reduce<2>(s);
+            else t.template reduce<1>(*reinterpret_cast<float(*)[1][Th::NP]>(&s));
 #pragma unroll
-            for (int j = 0; j < Th::NP; ++j) { s[0][j] *= inv; s[1][j] = d.post_kind == KIND_LAYER ? s[1][j] * inv : 0.f; }
+            for (int j = 0; j < Th::NP; ++j) {
+              s[0][j] *= inv;
+              if (GEN) s[1][j] = d.post_kind == KIND_LAYER ? s[1][j] * inv : 0.f;
+            }
 #pragma unroll
-            for (int e = 0; e < Th::E; ++e) D[e] = r2[Th::pix(e)] * (D[e] - n[e] * s[0][Th::pix(e)] - s[1][Th::pix(e)]);
+            for (int e = 0; e < Th::E; ++e)
+              D[e] = r2[Th::pix(e)] * (GEN ? D[e] - n[e] * s[0][Th::pix(e)] - s[1][Th::pix(e)] : D[e] - n[e] * s[0][Th::pix(e)]);
           }
           t.write(d.df, d.df_stride, D, o);
         }
       }
     }
-    if (d.f && d.gate_mode == GATE_IMAGE) {
-      float* out = a.part_post + (int64_t)item * 2 * d.C;
-      t.flush(s_dn, out);
-      if (BIAS) t.flush(s_d, out + d.C);
+    if (has_f && d.gate_mode == GATE_IMAGE) {
+      t.flush(s_dn, s_d, a.part_post + (int64_t)item * 2 * d.C);
 #pragma unroll
       for (int i = 0; i < Th::NW; ++i) s_dn[i] = s_d[i] = 0;
     }
   }
-  if (d.dh) {
-    float* out = a.part_pre + (int64_t)blockIdx.x * 2 * d.C;
-    t.flush(s_dhn, out);
-    if (BIAS) t.flush(s_dh, out + d.C);
-  }
-  if (d.f && d.gate_mode != GATE_IMAGE) {
-    float* out = a.part_post + (int64_t)blockIdx.x * 2 * d.C;
-    t.flush(s_dn, out);
-    if (BIAS) t.flush(s_d, out + d.C);
-  }
+  if (has_dh) t.flush(s_dhn, s_dh, a.part_pre + (int64_t)blockIdx.x * 2 * d.C);
+  if (has_f && d.gate_mode != GATE_IMAGE) t.flush(s_dn, s_d, a.part_post + (int64_t)blockIdx.x * 2 * d.C);
 }
 
-template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool BIAS> int launch_with(const Plan& p, int backward, hipStream_t s) {
-  if (backward)
-    hipLaunchKernelGGL((resnorm_bwd_kernel<T, ROWS, UNI, K, V, FULL, BIAS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
+template <typename T, bool ROWS, bool UNI, int K, int V, bool FULL, bool GEN> int launch_with(const Plan& p, int backward, hipStream_t s) {
+  const srx_resnorm_desc& d = p.a.d;
+  if (backward && d.f && d.dh && d.dy && d.dx && d.df)
+    hipLaunchKernelGGL((resnorm_bwd_kernel<T, ROWS, UNI, K, V, FULL, GEN, true>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
+  else if (backward)
+    hipLaunchKernelGGL((resnorm_bwd_kernel<T, ROWS, UNI, K, V, FULL, GEN, false>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
   else
-    hipLaunchKernelGGL((resnorm_fwd_kernel<T, ROWS, UNI, K, V, FULL, BIAS>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
+    hipLaunchKernelGGL((resnorm_fwd_kernel<T, ROWS, UNI, K, V, FULL, GEN>), dim3(p.workgroups), dim3(p.threads), p.lds_bytes, s, p.a);
   return srx_check_launch(backward ? "resnorm_bwd" : "resnorm_fwd");
 }
-// whether any offsets, or sums for them, are wanted
-inline bool has_bias(const srx_resnorm_desc& d) { return d.b_post || d.b_pre || d.db_post || d.db_pre; }
+// whether there are means or offsets, or sums for them are wanted
+inline bool general(const srx_resnorm_desc& d) {
+  return d.post_kind == KIND_LAYER || d.pre_kind == KIND_LAYER || d.b_post || d.b_pre || d.db_post || d.db_pre;
+}
 template <typename T, bool ROWS, bool UNI, int K, int V> int launch_for(const Plan& p, int backward, hipStream_t s) {
-  const bool bias = has_bias(p.a.d);
+  const bool gen = general(p.a.d);
   if (p.a.d.gate_mode == GATE_FULL)
-    return bias ? launch_with<T, ROWS, UNI, K, V, true, true>(p, backward, s) : launch_with<T, ROWS, UNI, K, V, true, false>(p, backward, s);
-  return bias ? launch_with<T, ROWS, UNI, K, V, false, true>(p, backward, s) : launch_with<T, ROWS, UNI, K, V, false, false>(p, backward, s);
+    return gen ? launch_with<T, ROWS, UNI, K, V, true, true>(p, backward, s) : launch_with<T, ROWS, UNI, K, V, true, false>(p, backward, s);
+  return gen ? launch_with<T, ROWS, UNI, K, V, false, true>(p, backward, s) : launch_with<T, ROWS, UNI, K, V, false, false>(p, backward, s);
 }
 template <typename T> int launch(const Plan& p, int backward, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);

@@ -39,8 +39,8 @@ class NormSpec(NamedTuple):
 def _checked_spec(spec: NormSpec, what: str, least: int = 1) -> None:
     if KINDS.get(spec.kind, -1) < least:
         raise ValueError(f"{what}: kind must be one of {[k for k, v in KINDS.items() if v >= least]}, got {spec.kind!r}")
-    if not 0 < spec.eps < math.inf:
-        raise ValueError(f"{what}: eps must be positive, got {spec.eps}")
+    if not 1e-37 <= spec.eps < math.inf:
+        raise ValueError(f"{what}: eps must be positive (at least 1e-37), got {spec.eps}")
 
 
 _NONE = NormSpec("none", None, None, 1.0)
