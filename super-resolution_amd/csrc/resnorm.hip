@@ -9,14 +9,14 @@ namespace {
 
 // Joins the partial sums: 16 channels a workgroup, 64 threads a channel that take every 64th partial, in a fixed order.
 constexpr int JOIN_X = 16, JOIN_Y = 64, JOIN_WAVES = JOIN_X * JOIN_Y / 64;
-// sums of p[i step] and, where second > 0, of p[i step + second] over i = y, y + 64, ... < n: eight loads of each in flight (a
-// partial sum was written on another die: a load takes the better part of a microsecond)
-__device__ __forceinline__ void join_sum(const float* p, int y, int n, int step, int second, float& s0, float& s1) {
-  for (int i0 = y; i0 < n; i0 += 8 * JOIN_Y) {
+// sums of p[i step] and, where second > 0, of p[i step + second] over i = y, y + EVERY, ... < n: eight loads of each in flight
+// (a partial sum was written on another die: a load takes the better part of a microsecond)
+template <int EVERY> __device__ __forceinline__ void join_sum(const float* p, int y, int n, int step, int second, float& s0, float& s1) {
+  for (int i0 = y; i0 < n; i0 += 8 * EVERY) {
     float v[8], u[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int i = i0 + j * JOIN_Y;
+      const int i = i0 + j * EVERY;
       v[j] = i < n ? p[(int64_t)i * step] : 0.f;
       u[j] = second && i < n ? p[(int64_t)i * step + second] : 0.f;
     }
@@ -34,23 +34,22 @@ __global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args
   const float w = ok && d.w_post ? d.w_post[c] : 1.f, b = ok && d.b_post ? d.b_post[c] : 0.f;
   const float q = ok && d.gate_mode == GATE_CHANNEL ? gate[c] : 1.f;
   float s[4] = {};                       // sum dh n, sum dh, sum D n (image gates: times s G), sum D
-  if (ok && pre) join_sum(a.part_pre + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[0], s[1]);
-  if (ok && d.f && d.gate_mode == GATE_IMAGE) {
-    for (int i = y; i < images; i += JOIN_Y) {
-      float sn = 0, sd = 0;
-      const float* p = a.part_post + (int64_t)i * a.slices * 2 * d.C + c;
-#pragma unroll 4
-      for (int k = 0; k < a.slices; ++k) {
-        sn += p[(int64_t)k * 2 * d.C];
-        if (bias) sd += p[((int64_t)k * 2 + 1) * d.C];
-      }
+  if (ok && pre) join_sum<JOIN_Y>(a.part_pre + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[0], s[1]);
+  if (d.f && d.gate_mode == GATE_IMAGE) {
+    // a wave an image: its four threads a channel share the image's partial sums
+    constexpr int YS = 64 / JOIN_X;
+    for (int i = threadIdx.x >> 6; i < images; i += JOIN_WAVES) {
+      float t[2] = {};
+      if (ok) join_sum<YS>(a.part_post + (int64_t)i * a.slices * 2 * d.C + c, y & (YS - 1), a.slices, 2 * d.C, bias ? d.C : 0, t[0], t[1]);
+      lanes_sum<2>(t, JOIN_X, 64);
+      if (!ok || (y & (YS - 1))) continue;
       const float qi = gate[(int64_t)i * d.C + c], G = d.gate_act ? sigmoid(qi) : qi;
-      if (dgate) dgate[(int64_t)i * d.C + c] = d.scale * (w * sn + b * sd) * (d.gate_act ? G * (1.f - G) : 1.f);
-      s[2] += d.scale * G * sn;
-      s[3] += d.scale * G * sd;
+      if (dgate) dgate[(int64_t)i * d.C + c] = d.scale * (w * t[0] + b * t[1]) * (d.gate_act ? G * (1.f - G) : 1.f);
+      s[2] += d.scale * G * t[0];
+      s[3] += d.scale * G * t[1];
     }
   } else if (ok && d.f) {
-    join_sum(a.part_post + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[2], s[3]);
+    join_sum<JOIN_Y>(a.part_post + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[2], s[3]);
   }
   lanes_sum<4>(s, JOIN_X, 64);
   if ((threadIdx.x & 63) < JOIN_X)
