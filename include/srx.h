@@ -407,7 +407,7 @@ typedef struct srx_adamw_desc {
   void* m; void* v;                   /* moments, 16-byte aligned                                 */
   float* m_scale; float* v_scale;     /* 8 bits: one scale for each block                         */
   int32_t* steps;                     /* DEVICE [ntensors] step counts, advanced by the call      */
-  float* coef;                        /* DEVICE workspace, 4 + 8 * ntensors floats                */
+  float* coef;                        /* DEVICE workspace, 4 + 10 * ntensors floats, zeroed once  */
   double* partial;                    /* DEVICE workspace, one per chunk (norm only)              */
   float* norm;                        /* DEVICE result (norm only)                                */
   double grad_scale, max_norm;

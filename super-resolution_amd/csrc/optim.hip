@@ -2,9 +2,16 @@
 // step whose gradients are not finite.  See include/srx.h (srx_adamw_step) for the formulas and the buffers.
 //
 // Launches of one step: [norm pass over the gradients, 448 tensors a launch] + one "prepare" workgroup (finishes the
-// norm, advances the step counts, computes each tensor's bias-corrected constants) + the update, 448 tensors a launch.
+// norm, advances the step counts, computes each tensor's bias-corrected constants) + the update, 448 tensors a launch, or
+// one launch where the norm pass has been there and left the addresses in device memory.  A small step without a norm is
+// one launch in all.
 // The gradients' addresses travel in the kernel arguments: they change from step to step (autograd allocates new
 // gradients), and a table in device memory would need a host-to-device copy that a captured graph could not repeat.
+//
+// Bound: HBM.  702 tensors of 22800 fp32 elements (16.0 M): norm pass 14 us, prepare 3 to 5 us, update 74 us (6.0 TB/s: part
+// of the 448 MB stays in the last-level cache) with 32-bit moments, 54 us with 8-bit ones; whole step with clipping 95 and
+// 73 us.
+#include <type_traits>
 #include "srx_common.h"
 
 namespace {
@@ -13,14 +20,20 @@ constexpr int BLOCK = SRX_ADAMW_BLOCK;          // elements that share one scale
 constexpr int CHUNK = SRX_ADAMW_CHUNK;          // elements of one tensor that one workgroup updates
 constexpr int TPB = 256;
 constexpr int MAX_GRADS = 448;                  // addresses per launch: 3.6 KB of the 4 KB of kernel arguments
+constexpr int SMALL_GRADS = 128;                // the same beside 32 groups of constants
+constexpr int FLAT = 0, TABLE = -1;             // the other places of the gradients' addresses
 constexpr int PREP_TENSORS = 16384;             // tensors per prepare launch: one bit each, 2 KB of kernel arguments
 constexpr int PREP_TPB = 1024;
+// Up to here a step without a norm is one launch.  Measured from the host, one launch against two: 12 tensors of 64 elements
+// 9.0 us against 12.4, 100 chunks 11.0 against 14.1, 200 chunks 12.8 against 14.3, 400 chunks 20.7 against 14.0; replayed in a
+// graph 5.1 against 5.9, 9.3 against 8.2, 12.6 against 8.9 (every workgroup adds to one counter).
+constexpr int SMALL_CHUNKS = 64;
 
 // The top 12 bits of a float are its exponent and three mantissa bits; 1.0 has 1016 there.  Code c > 0 stands for the
 // float with base + c there: 127 signed codes reach from 1 down to 1.25 * 2^-16, 255 unsigned ones to 1.25 * 2^-32.
 constexpr unsigned M_BASE = 889, V_BASE = 761;
 
-struct Ctl { float factor; int skip; float pad[2]; };            // first 16 bytes of the coefficient workspace
+struct Ctl { float factor; int skip; int arrived; int pad; };    // first 16 bytes of the coefficient workspace
 struct Coef { float decay, step_size, root, eps, b1, ob1, b2, ob2; };
 
 struct PrepArgs {
@@ -37,27 +50,42 @@ struct PrepArgs {
   uint32_t has_grad[PREP_TENSORS / 32];
 };
 
-template <int NG> struct StepArgs {
+// What the small form adds: the groups' constants, and who moves the step counts.
+struct SmallArgs {
+  int32_t* steps;
+  int* arrived;
+  double grad_scale;
+  int ntensors;              // of this launch
+  srx_adamw_group groups[SRX_ADAMW_MAX_GROUPS];
+};
+struct NoArgs {};
+
+template <int NG, bool SMALL = false> struct StepArgs {
   const srx_adamw_tensor* tensors;
   const srx_adamw_chunk* chunks;
   const float* coef;
   double* partial;
   void* m; void* v;
   float* m_scale; float* v_scale;
-  const void* flat;          // NG == 1: the flat gradient
+  const void* flat;          // NG == FLAT: the flat gradient
+  uint64_t* table;           // addresses in device memory, bit 0 set for bf16 (NG == TABLE: read; else written, if there)
   int chunk0, t0;
-  int norm_mode;
   int flat_dtype;
-  uint64_t is_bf16[(NG + 63) / 64];
-  const void* g[NG];
+  uint64_t is_bf16[(NG + 63) / 64 + (NG <= 0)];
+  const void* g[NG > 0 ? NG : 1];
+  std::conditional_t<SMALL, SmallArgs, NoArgs> small;
 };
 
 struct Grad { const void* p; bool bf; };
-template <int NG> __device__ __forceinline__ Grad grad_of(const StepArgs<NG>& a, const srx_adamw_tensor& t, int ti) {
+template <int NG, bool SMALL> __device__ __forceinline__ Grad grad_of(const StepArgs<NG, SMALL>& a, const srx_adamw_tensor& t, int ti) {
   Grad r;
-  if constexpr (NG == 1) {
+  if constexpr (NG == FLAT) {
     r.bf = a.flat_dtype == SRX_BF16;
     r.p = static_cast<const char*>(a.flat) + t.g_off * (r.bf ? 2 : 4);
+  } else if constexpr (NG == TABLE) {
+    const uint64_t p = a.table[ti];
+    r.bf = p & 1;
+    r.p = reinterpret_cast<const void*>(p & ~1ull);
   } else {
     const int k = ti - a.t0;
     r.p = a.g[k];
@@ -154,7 +182,8 @@ template <int NG> __global__ __launch_bounds__(TPB) void adamw_norm_kernel(const
   const int c = a.chunk0 + blockIdx.x;
   const srx_adamw_chunk ch = a.chunks[c];
   const srx_adamw_tensor t = a.tensors[ch.tensor];
-  const Grad g = grad_of<NG>(a, t, ch.tensor);
+  const Grad g = grad_of(a, t, ch.tensor);
+  if (NG != FLAT && a.table && ch.index == 0 && threadIdx.x == 0) a.table[ch.tensor] = reinterpret_cast<uint64_t>(g.p) | (g.bf ? 1 : 0);
   double s = 0;
   if (g.p) {
     const int64_t lo = (int64_t)ch.index * CHUNK + threadIdx.x * 4;
@@ -174,10 +203,23 @@ template <int NG> __global__ __launch_bounds__(TPB) void adamw_norm_kernel(const
   if (threadIdx.x == 0) a.partial[c] = part[0] + part[1] + part[2] + part[3];
 }
 
-__device__ double int_pow(double b, int n) {
+__device__ __forceinline__ double int_pow(double b, int n) {
   double r = 1;
   for (; n > 0; n >>= 1, b *= b)
     if (n & 1) r *= b;
+  return r;
+}
+
+__device__ __forceinline__ Coef coef_of(const srx_adamw_group& g, int step) {
+  Coef r;
+  r.decay = (float)(1 - g.lr * g.weight_decay);
+  r.step_size = (float)(g.lr / (1 - int_pow(g.beta1, step)));
+  r.root = (float)(1 / sqrt(1 - int_pow(g.beta2, step)));
+  r.eps = (float)g.eps;
+  r.b1 = (float)g.beta1;
+  r.ob1 = (float)(1 - g.beta1);
+  r.b2 = (float)g.beta2;
+  r.ob2 = (float)(1 - g.beta2);
   return r;
 }
 
@@ -222,17 +264,7 @@ __global__ __launch_bounds__(PREP_TPB) void adamw_prepare_kernel(const PrepArgs 
     const int i = a.t0 + k;
     const int step = a.steps[i] + 1;
     a.steps[i] = step;
-    const srx_adamw_group& g = a.groups[a.tensors[i].group];
-    Coef r;
-    r.decay = (float)(1 - g.lr * g.weight_decay);
-    r.step_size = (float)(g.lr / (1 - int_pow(g.beta1, step)));
-    r.root = (float)(1 / sqrt(1 - int_pow(g.beta2, step)));
-    r.eps = (float)g.eps;
-    r.b1 = (float)g.beta1;
-    r.ob1 = (float)(1 - g.beta1);
-    r.b2 = (float)g.beta2;
-    r.ob2 = (float)(1 - g.beta2);
-    coef[i] = r;
+    coef[i] = coef_of(a.groups[a.tensors[i].group], step);
   }
 }
 
@@ -281,15 +313,22 @@ template <bool SIGNED> __device__ __forceinline__ uint32_t encode4(const float* 
 
 // A wave takes whole blocks of 256, four elements a lane, so that a block's largest is a wave's.  All of a wave's four
 // blocks are read before the first is computed: a workgroup's only other wait is for the tables in front of them.
-template <int BITS, int NG> __global__ __launch_bounds__(TPB) void adamw_step_kernel(const StepArgs<NG> a) {
+template <int BITS, int NG, bool SMALL> __device__ __forceinline__ void update_chunk(const StepArgs<NG, SMALL>& a) {
   const Ctl* ctl = reinterpret_cast<const Ctl*>(a.coef);
-  if (ctl->skip) return;
+  if (!SMALL && ctl->skip) return;
   const srx_adamw_chunk ch = a.chunks[a.chunk0 + blockIdx.x];
   const srx_adamw_tensor t = a.tensors[ch.tensor];
-  const Grad g = grad_of<NG>(a, t, ch.tensor);
+  const Grad g = grad_of(a, t, ch.tensor);
   if (!g.p) return;
-  const Coef c = reinterpret_cast<const Coef*>(a.coef + 4)[ch.tensor];
-  const float factor = ctl->factor;
+  Coef c;
+  float factor;
+  if constexpr (SMALL) {
+    factor = (float)a.small.grad_scale;
+    c = coef_of(a.small.groups[t.group], a.small.steps[ch.tensor] + 1);
+  } else {
+    factor = ctl->factor;
+    c = reinterpret_cast<const Coef*>(a.coef + 4)[ch.tensor];
+  }
   const bool fast = c.eps >= 1e-15f;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int NB = CHUNK / BLOCK / (TPB / 64);
@@ -368,6 +407,27 @@ template <int BITS, int NG> __global__ __launch_bounds__(TPB) void adamw_step_ke
   }
 }
 
+// The small form is a step in one launch: each workgroup computes its tensor's constants itself, and the last one to
+// arrive, after every other has read its step count, moves the counts and clears the counter for the next launch.
+template <int BITS, int NG, bool SMALL> __global__ __launch_bounds__(TPB) void adamw_step_kernel(const StepArgs<NG, SMALL> a) {
+  update_chunk<BITS>(a);
+  if constexpr (SMALL) {
+    __shared__ int last;
+    __syncthreads();                                  // all waves of this workgroup have read their step count
+    if (threadIdx.x == 0) {
+      last = __hip_atomic_fetch_add(a.small.arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+      if (last) __hip_atomic_store(a.small.arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    for (int k = threadIdx.x; k < a.small.ntensors; k += TPB) {
+      bool has = true;
+      if constexpr (NG != FLAT) has = a.g[k] != nullptr;
+      if (has) a.small.steps[a.t0 + k] += 1;
+    }
+  }
+}
+
 // one wave per block of 256
 __global__ __launch_bounds__(TPB) void moments_to8_kernel(const float* m, const float* v, uint8_t* mc, uint8_t* vc, float* ms,
                                                           float* vs, int64_t nblocks) {
@@ -419,31 +479,56 @@ int check_moments(const char* what, const void* a, const void* b, const void* c,
   return SRX_OK;
 }
 
+template <int NG, bool SMALL = false> StepArgs<NG, SMALL> step_args(const srx_adamw_desc* d, int t0, int t1) {
+  StepArgs<NG, SMALL> a = {};
+  a.tensors = d->tensors; a.chunks = d->chunks; a.coef = d->coef; a.partial = d->partial;
+  a.m = d->m; a.v = d->v; a.m_scale = d->m_scale; a.v_scale = d->v_scale;
+  a.flat = d->flat_grad; a.flat_dtype = d->flat_dtype; a.chunk0 = d->chunk_start[t0]; a.t0 = t0;
+  if (NG == TABLE || d->ntensors > MAX_GRADS) a.table = reinterpret_cast<uint64_t*>(d->coef + 4 + 8 * (int64_t)d->ntensors);
+  if constexpr (NG > 0)
+    for (int k = 0; k < t1 - t0; ++k) {
+      a.g[k] = d->grads[t0 + k];
+      if (d->grad_dtypes && d->grad_dtypes[t0 + k] == SRX_BF16) a.is_bf16[k >> 6] |= 1ull << (k & 63);
+    }
+  return a;
+}
+
 // One pass over the tensors in launches of at most NG gradients, `fn(args, chunks)` each.
-template <int NG, typename F> int each_launch(const srx_adamw_desc* d, int norm_mode, F fn) {
-  const int per = NG == 1 ? d->ntensors : NG;
+template <int NG, typename F> int each_launch(const srx_adamw_desc* d, F fn) {
+  const int per = NG > 0 ? NG : d->ntensors;
   for (int t0 = 0; t0 < d->ntensors; t0 += per) {
     const int t1 = t0 + per < d->ntensors ? t0 + per : d->ntensors;
-    const int c0 = d->chunk_start[t0], c1 = d->chunk_start[t1];
-    if (c1 <= c0) continue;
-    StepArgs<NG> a = {};
-    a.tensors = d->tensors; a.chunks = d->chunks; a.coef = d->coef; a.partial = d->partial;
-    a.m = d->m; a.v = d->v; a.m_scale = d->m_scale; a.v_scale = d->v_scale;
-    a.flat = d->flat_grad; a.flat_dtype = d->flat_dtype; a.chunk0 = c0; a.t0 = t0; a.norm_mode = norm_mode;
-    if (NG > 1)
-      for (int k = 0; k < t1 - t0; ++k) {
-        a.g[k] = d->grads[t0 + k];
-        if (d->grad_dtypes && d->grad_dtypes[t0 + k] == SRX_BF16) a.is_bf16[k >> 6] |= 1ull << (k & 63);
-      }
-    if (int rc = fn(a, c1 - c0)) return rc;
+    const int n = d->chunk_start[t1] - d->chunk_start[t0];
+    if (n <= 0) continue;
+    if (int rc = fn(step_args<NG>(d, t0, t1), n)) return rc;
   }
   return SRX_OK;
 }
 
+template <int NG, bool SMALL> int launch_step(const srx_adamw_desc* d, const StepArgs<NG, SMALL>& a, int n, hipStream_t s) {
+  if (d->state_bits == 8) hipLaunchKernelGGL((adamw_step_kernel<8, NG, SMALL>), dim3(n), dim3(TPB), 0, s, a);
+  else hipLaunchKernelGGL((adamw_step_kernel<32, NG, SMALL>), dim3(n), dim3(TPB), 0, s, a);
+  return srx_check_launch("adamw_step");
+}
+
+template <int NG> int small_launch(const srx_adamw_desc* d, hipStream_t s) {
+  StepArgs<NG, true> a = step_args<NG, true>(d, 0, d->ntensors);
+  a.small.steps = d->steps;
+  a.small.arrived = &reinterpret_cast<Ctl*>(d->coef)->arrived;
+  a.small.grad_scale = d->grad_scale;
+  a.small.ntensors = d->ntensors;
+  for (int g = 0; g < d->ngroups; ++g) a.small.groups[g] = d->groups[g];
+  return launch_step(d, a, d->chunk_start[d->ntensors], s);
+}
+
 template <int NG> int step_launches(const srx_adamw_desc* d, hipStream_t s) {
-  const int norm = d->max_norm > 0 || d->skip_nonfinite;
+  const int norm = d->max_norm > 0 || d->skip_nonfinite, chunks = d->chunk_start[d->ntensors];
+  if (!norm && chunks > 0 && chunks <= SMALL_CHUNKS) {
+    if constexpr (NG == FLAT) return small_launch<FLAT>(d, s);
+    else if (d->ntensors <= SMALL_GRADS) return small_launch<SMALL_GRADS>(d, s);
+  }
   if (norm) {
-    int rc = each_launch<NG>(d, norm, [&](const StepArgs<NG>& a, int n) {
+    int rc = each_launch<NG>(d, [&](const StepArgs<NG>& a, int n) {
       hipLaunchKernelGGL(adamw_norm_kernel<NG>, dim3(n), dim3(TPB), 0, s, a);
       return srx_check_launch("adamw_norm");
     });
@@ -453,20 +538,19 @@ template <int NG> int step_launches(const srx_adamw_desc* d, hipStream_t s) {
     PrepArgs p = {};
     p.tensors = d->tensors; p.steps = d->steps; p.coef = d->coef; p.partial = d->partial; p.norm = d->norm;
     p.grad_scale = d->grad_scale; p.max_norm = d->max_norm; p.ntensors = d->ntensors; p.t0 = t0;
-    p.nchunks = d->chunk_start[d->ntensors];
+    p.nchunks = chunks;
     p.norm_mode = !norm ? 0 : t0 ? 2 : 1;
     p.skip_nonfinite = d->skip_nonfinite;
     for (int g = 0; g < d->ngroups; ++g) p.groups[g] = d->groups[g];
     for (int k = 0; k < PREP_TENSORS && t0 + k < d->ntensors; ++k)
-      if (NG == 1 || d->grads[t0 + k]) p.has_grad[k >> 5] |= 1u << (k & 31);
+      if (NG == FLAT || d->grads[t0 + k]) p.has_grad[k >> 5] |= 1u << (k & 31);
     hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(PREP_TPB), 0, s, p);
     if (int rc = srx_check_launch("adamw_prepare")) return rc;
   }
-  return each_launch<NG>(d, norm, [&](const StepArgs<NG>& a, int n) {
-    if (d->state_bits == 8) hipLaunchKernelGGL((adamw_step_kernel<8, NG>), dim3(n), dim3(TPB), 0, s, a);
-    else hipLaunchKernelGGL((adamw_step_kernel<32, NG>), dim3(n), dim3(TPB), 0, s, a);
-    return srx_check_launch("adamw_step");
-  });
+  const auto step = [&](const auto& a, int n) { return launch_step(d, a, n, s); };
+  // the norm pass has left the addresses in device memory: the update needs no second launch for them
+  if (NG > 0 && norm && d->ntensors > NG) return each_launch<TABLE>(d, step);
+  return each_launch<NG>(d, step);
 }
 
 }  // namespace
@@ -504,7 +588,7 @@ int srx_adamw_step(const srx_adamw_desc* d, void* stream) {
                   q.beta1, q.beta2, q.eps, q.weight_decay);
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return d->flat_grad ? step_launches<1>(d, s) : step_launches<MAX_GRADS>(d, s);
+  return d->flat_grad ? step_launches<FLAT>(d, s) : step_launches<MAX_GRADS>(d, s);
 }
 
 int srx_adamw_moments_to8(const float* m, const float* v, void* m_code, void* v_code, float* m_scale, float* v_scale,

@@ -110,7 +110,7 @@ class AdamW:
             self._v = torch.zeros_like(self._m)
             self._m_scale, self._v_scale = (zeros(self.nblocks), zeros(self.nblocks)) if state_bits == 8 else (None, None)
             self._steps = zeros(len(self.params), torch.int32)
-            self._coef = zeros(4 + 8 * len(self.params))
+            self._coef = zeros(4 + 10 * len(self.params))
             self._partial = zeros(int(start[-1]), torch.float64)
             half = [n if t == torch.bfloat16 else 0 for n, t in zip(self._n, self._dtypes)]
             self._master_at = [0]
