@@ -103,15 +103,15 @@ Tensor taken(const Order& o, const Tensor& t, int64_t& stride) {
     stride = o.C;
     if (v.is_contiguous()) return v;
     bool fits = o.C == 1 || v.stride(-1) == 1;       // one stride between all rows?
-    int64_t step = 0, next = 0;
+    int64_t step = -1, next = 0;
     for (int64_t i = v.dim() - 2; i >= 0 && fits; --i) {
       if (v.size(i) == 1) continue;
-      if (!step) step = v.stride(i);
+      if (step < 0) step = v.stride(i);
       else fits = v.stride(i) == next;
       next = v.stride(i) * v.size(i);
     }
-    if (!fits) return v.contiguous();
-    if (step) stride = step;
+    if (!fits || step == 0) return v.contiguous();       // (a row that is expanded over others: copied)
+    if (step > 0) stride = step;
     return v;
   }
   stride = o.C * o.P;
@@ -371,8 +371,13 @@ PyObject* resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
       d.gate_act = (int32_t)PyLong_AsLong(a[11]);
     }
-    const Tensor w_post = channel_vector(tensor_arg(a[3], "post.weight"), o, x, "post.weight"), b_post = channel_vector(tensor_arg(a[4], "post.bias"), o, x, "post.bias");
-    const Tensor w_pre = channel_vector(tensor_arg(a[5], "pre.weight"), o, x, "pre.weight"), b_pre = channel_vector(tensor_arg(a[6], "pre.bias"), o, x, "pre.bias");
+    variable_list given = {x, f, tensor_arg(a[2], "gate")};          // before a conversion to fp32: the graph's leaves
+    auto vector_arg = [&](int at, const char* what) {
+      given.push_back(tensor_arg(a[at], what));
+      return channel_vector(given.back(), o, x, what);
+    };
+    const Tensor w_post = vector_arg(3, "post.weight"), b_post = vector_arg(4, "post.bias");
+    const Tensor w_pre = vector_arg(5, "pre.weight"), b_pre = vector_arg(6, "pre.bias");
     if (PyErr_Occurred()) return nullptr;
     const variable_list inputs = {x, f, gate, w_post, b_post, w_pre, b_pre};
     bool grad = false;
@@ -381,7 +386,7 @@ PyObject* resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     variable_list out;
     const c10::OptionalDeviceGuard guard(x.device());
     if (grad) {
-      note_graph(*c, inputs, x.device());
+      note_graph(*c, given, x.device());
       auto opt = [](const Tensor& t) -> Opt { return t.defined() ? Opt(t) : std::nullopt; };
       out = ResNorm::apply(c, opt(x), opt(f), opt(gate), opt(w_post), opt(b_post), opt(w_pre), opt(b_pre));
     } else {
@@ -414,9 +419,9 @@ struct Buffer {
   Buffer(const Buffer&) = delete;
 };
 
-// gather(params, grads or None, bound, addresses, types, device index) -> flags.  Compares the parameters' addresses with
-// bound[n] (uint64), and writes the gradients' addresses (uint64[n], 0: none) and types (uint8[n]).  GATHER_MOVED: a
-// parameter's address differs.  GATHER_ODD: a gradient cannot be taken as it is (shape, type, device, order) and the
+// gather(params, grads or None, bound, addresses, types, device index) -> flags.  Compares the parameters with bound[2 n]
+// (uint64: addresses, then elements times two, plus one for bf16), and writes the gradients' addresses (uint64[n], 0: none)
+// and types (uint8[n]).  GATHER_MOVED: a parameter's address, size or type differs, or it is not contiguous.  GATHER_ODD: a gradient cannot be taken as it is (shape, type, device, order) and the
 // caller has to look.  GATHER_BF16: some gradient is bf16.  grads None: each parameter's .grad.
 PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
@@ -425,7 +430,7 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const Py_ssize_t n = PyList_GET_SIZE(a[0]);
     const bool given = a[1] != Py_None;
     if (given && PyList_GET_SIZE(a[1]) != n) refuse(PyExc_ValueError, PyList_GET_SIZE(a[1]), " gradients for ", n, " parameters");
-    const Buffer bound(a[2], n * 8, "bound"), addresses(a[3], n * 8, "addresses"), types(a[4], n, "types");
+    const Buffer bound(a[2], n * 16, "bound"), addresses(a[3], n * 8, "addresses"), types(a[4], n, "types");
     const long index = PyLong_AsLong(a[5]);
     if (PyErr_Occurred()) return nullptr;
     const auto* was = static_cast<const uint64_t*>(bound.b.buf);
@@ -433,8 +438,11 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     auto* ty = static_cast<uint8_t*>(types.b.buf);
     long flags = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
+      if (!THPVariable_Check(PyList_GET_ITEM(a[0], i))) refuse(PyExc_TypeError, "parameter ", i, " is not a tensor");
       const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(a[0], i));
-      if (reinterpret_cast<uint64_t>(p.data_ptr()) != was[i]) flags |= GATHER_MOVED;
+      if (reinterpret_cast<uint64_t>(p.data_ptr()) != was[i] || 2 * (uint64_t)p.numel() + (p.scalar_type() == at::kBFloat16) != was[n + i] ||
+          !p.is_contiguous())
+        flags |= GATHER_MOVED;
       to[i] = 0;
       ty[i] = SRX_F32;
       PyObject* go = given ? PyList_GET_ITEM(a[1], i) : nullptr;

@@ -574,3 +574,76 @@ def test_stack_in_bf16_and_without_gradients():
     ref, _ = _stack64(s, x.to(BF16))
     # three blocks, each a few roundings of 2^-9 deep in both the branch and the stream
     assert float((out.double().cpu() - ref.detach()).norm() / ref.detach().norm()) < 2e-2
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,dim", [((200, 24, 3, 5), 1), ((65, 72, 2, 2), 1), ((130, 3, 96), 2), ((1100, 2, 20), 2), ((70, 40, 1), 1)])
+def test_gates_of_many_images(shape, dim, dtype):
+    """More images than one workgroup joins."""
+    for k, (post, pre, act) in enumerate((("rms", "rms", "none"), ("layer", "layer", "sigmoid"))):
+        x, f, g, p, q = make(shape, dim, dtype, post, "image", pre, seed=k)
+        compare(x, f, g, p, q, act, dim=dim)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_expanded_tensors(dtype):
+    """Rows, pixels and images of stride 0 are inputs like others."""
+    cases = [((3, 5, 40), (1, 1, 40), 2), ((3, 5, 40), (3, 1, 40), 2), ((3, 5, 40), (1, 5, 40), 2), ((3, 5, 40), (3, 5, 1), 2), ((3, 5, 1), (1, 1, 1), 2),
+             ((3, 5, 1), (3, 1, 1), 2), ((3, 40, 4, 6), (1, 40, 4, 6), 1), ((3, 40, 4, 6), (3, 40, 1, 1), 1), ((3, 40, 4, 6), (1, 1, 4, 6), 1),
+             ((3, 40, 4, 6), (1, 40, 1, 6), 1), ((6, 40), (1, 40), 1), ((6, 40, 1, 1), (1, 40, 1, 1), 1)]
+    for shape, small, dim in cases:
+        spec = R().NormSpec("layer")
+        x, f = torch.randn(small, device=DEV).to(dtype), torch.randn(small, device=DEV).to(dtype)
+        d = torch.randn(small, device=DEV).to(dtype)
+        out = []
+        for wide in (lambda t: t.expand(shape), lambda t: t.expand(shape).contiguous()):
+            a, b = wide(x).detach().requires_grad_(), wide(f).detach().requires_grad_()
+            y, h = R().gated_residual(a, b, post=spec, gate=wide(x).detach(), pre=spec, channel_dim=dim)
+            out.append([y, h, *torch.autograd.grad((y, h), (a, b), (wide(d), wide(d)))])
+        assert all(torch.equal(s, t) for s, t in zip(*out)), (shape, small)
+
+
+def test_capture_beside_a_living_graph_of_bf16_weights_is_refused():
+    x = torch.randn(2, 64, 8, 8, device=DEV)
+    spec = R().NormSpec("rms", torch.ones(64, dtype=BF16, device=DEV, requires_grad=True))
+    gate = torch.ones(64, dtype=BF16, device=DEV, requires_grad=True)
+    for call in (lambda: R().channel_norm(x, spec), lambda: R().gated_residual(x, x, gate=gate)):
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            x * 2
+            with pytest.raises(RuntimeError, match="recorded before this capture"):
+                call()
+        del alive
+
+
+def test_two_streams_at_once():
+    """Calls of different sizes on two streams share nothing."""
+    sets = [make(s, 1, BF16, "rms", "image", "layer", seed=k) for k, s in enumerate(((8, 64, 32, 32), (2, 200, 40, 24)))]
+    def run(k):
+        x, f, g, post, pre = sets[k]
+        leaves = [t.requires_grad_() for t in (x, f, g, post.weight, pre.weight, pre.bias)]
+        y, h = R().gated_residual(x, f, post=post, gate=g, pre=pre)
+        return [t.detach() for t in (y, h, *torch.autograd.grad((y, h), leaves, (y.detach(), h.detach())))]
+    want = [run(0), run(1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(run(k))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
+
+
+def test_a_gate_of_each_row_in_fp32():
+    """[B, C] in bf16 with an fp32 gate of the same shape: a gate for each of B."""
+    x, f, _, post, pre = make((90, 48), 1, BF16, "rms", None, "rms")
+    g = (0.5 + 0.3 * torch.randn(90, 48, generator=torch.Generator().manual_seed(7))).to(DEV)
+    y, h = R().gated_residual(x, f, post=post, gate=g, pre=pre)
+    want = rows_of(x, 1) + g.double().cpu() * norm64(rows_of(f, 1), post)
+    lim = limits(x, f, None, post, pre, "none", float(g.abs().max()), 1)
+    check(rows_of(y, 1), want, 64 * U * lim["y"], BF16, "y")
