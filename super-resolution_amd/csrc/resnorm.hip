@@ -9,6 +9,10 @@ namespace {
 
 // Joins the partial sums: 16 channels a workgroup, 64 threads a channel that take every 64th partial, in a fixed order.
 constexpr int JOIN_X = 16, JOIN_Y = 64, JOIN_WAVES = JOIN_X * JOIN_Y / 64;
+// Images whose gates one workgroup joins; with more, a launch of its own goes before the join.  A backward pass with it,
+// without it (bf16): 8192 images of 16 x 256 rows 144 us, 737; 4096 of 64 x 8 x 8 127 us, 438; 256 of 512 x 256 rows 104 us, 117.
+constexpr int JOIN_IMAGES = 64;
+__host__ __device__ constexpr int join_groups(int images) { return images / JOIN_IMAGES + (images % JOIN_IMAGES > 0); }
 // sums of p[i step] and, where second > 0, of p[i step + second] over i = y, y + EVERY, ... < n: eight loads of each in flight
 // (a partial sum was written on another die: a load takes the better part of a microsecond)
 template <int EVERY> __device__ __forceinline__ void join_sum(const float* p, int y, int n, int step, int second, float& s0, float& s1) {
@@ -24,45 +28,77 @@ template <int EVERY> __device__ __forceinline__ void join_sum(const float* p, in
     for (int j = 0; j < 8; ++j) { s0 += v[j]; s1 += u[j]; }
   }
 }
-__global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args a, int workgroups, int images, bool bias) {
-  __shared__ float lds[4][JOIN_WAVES][JOIN_X];
+// Gates of images i0 <= i < i1: writes their gradients; s0, s1 += the images' sums of D n and D, times s G.  A wave takes an
+// image: its four threads a channel share the image's partial sums, and the first of them holds the results.
+__device__ __forceinline__ void join_images(const Args& a, int i0, int i1, int c, float w, float b, bool bias, float& s0, float& s1) {
   const srx_resnorm_desc& d = a.d;
-  const int x = threadIdx.x & (JOIN_X - 1), y = threadIdx.x / JOIN_X, c = blockIdx.x * JOIN_X + x;
-  const bool ok = c < d.C, pre = d.dh && (d.dw_pre || d.db_pre);
-  const float* gate = d.gate_mode == GATE_CHANNEL || d.gate_mode == GATE_IMAGE ? static_cast<const float*>(d.gate) : nullptr;
-  float* dgate = gate ? static_cast<float*>(d.dgate) : nullptr;
-  const float w = ok && d.w_post ? d.w_post[c] : 1.f, b = ok && d.b_post ? d.b_post[c] : 0.f;
-  const float q = ok && d.gate_mode == GATE_CHANNEL ? gate[c] : 1.f;
-  float s[4] = {};                       // sum dh n, sum dh, sum D n (image gates: times s G), sum D
-  if (ok && pre) join_sum<JOIN_Y>(a.part_pre + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[0], s[1]);
-  if (d.f && d.gate_mode == GATE_IMAGE) {
-    // a wave an image: its four threads a channel share the image's partial sums
-    constexpr int YS = 64 / JOIN_X;
-    for (int i = threadIdx.x >> 6; i < images; i += JOIN_WAVES) {
-      float t[2] = {};
-      if (ok) join_sum<YS>(a.part_post + (int64_t)i * a.slices * 2 * d.C + c, y & (YS - 1), a.slices, 2 * d.C, bias ? d.C : 0, t[0], t[1]);
-      lanes_sum<2>(t, JOIN_X, 64);
-      if (!ok || (y & (YS - 1))) continue;
-      const float qi = gate[(int64_t)i * d.C + c], G = d.gate_act ? sigmoid(qi) : qi;
-      if (dgate) dgate[(int64_t)i * d.C + c] = d.scale * (w * t[0] + b * t[1]) * (d.gate_act ? G * (1.f - G) : 1.f);
-      s[2] += d.scale * G * t[0];
-      s[3] += d.scale * G * t[1];
-    }
-  } else if (ok && d.f) {
-    join_sum<JOIN_Y>(a.part_post + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[2], s[3]);
+  constexpr int YS = 64 / JOIN_X;
+  const bool ok = c < d.C;
+  const int y = threadIdx.x / JOIN_X & (YS - 1);
+  const float* gate = static_cast<const float*>(d.gate);
+  float* dgate = static_cast<float*>(d.dgate);
+  for (int i = i0 + (threadIdx.x >> 6); i < i1; i += JOIN_WAVES) {
+    float t[2] = {};
+    if (ok) join_sum<YS>(a.part_post + (int64_t)i * a.slices * 2 * d.C + c, y, a.slices, 2 * d.C, bias ? d.C : 0, t[0], t[1]);
+    lanes_sum<2>(t, JOIN_X, 64);
+    if (!ok || y) continue;
+    const float q = gate[(int64_t)i * d.C + c], G = d.gate_act ? sigmoid(q) : q;
+    if (dgate) dgate[(int64_t)i * d.C + c] = d.scale * (w * t[0] + b * t[1]) * (d.gate_act ? G * (1.f - G) : 1.f);
+    s0 += d.scale * G * t[0];
+    s1 += d.scale * G * t[1];
   }
-  lanes_sum<4>(s, JOIN_X, 64);
+}
+// the workgroup's sums over its threads of a channel, in a fixed order; for threads below 16, channels
+template <int N> __device__ __forceinline__ void join_threads(float (&s)[N], float (*lds)[JOIN_WAVES][JOIN_X]) {
+  const int x = threadIdx.x & (JOIN_X - 1);
+  lanes_sum<N>(s, JOIN_X, 64);
   if ((threadIdx.x & 63) < JOIN_X)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds[i][threadIdx.x >> 6][x] = s[i];
+    for (int i = 0; i < N; ++i) lds[i][threadIdx.x >> 6][x] = s[i];
   __syncthreads();
-  if (y > 0 || !ok) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N; ++i) {
     s[i] = 0;
 #pragma unroll
     for (int k = 0; k < JOIN_WAVES; ++k) s[i] += lds[i][k][x];
   }
+}
+// Many images: workgroup (., k) takes JOIN_IMAGES of them and leaves the sums of their gates at part_gate[k].
+__global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_images_kernel(const Args a, float* part_gate, int images, bool bias) {
+  __shared__ float lds[2][JOIN_WAVES][JOIN_X];
+  const srx_resnorm_desc& d = a.d;
+  const int c = blockIdx.y * JOIN_X + (threadIdx.x & (JOIN_X - 1)), i0 = blockIdx.x * JOIN_IMAGES;
+  const bool ok = c < d.C;
+  const float w = ok && d.w_post ? d.w_post[c] : 1.f, b = ok && d.b_post ? d.b_post[c] : 0.f;
+  float s[2] = {};
+  join_images(a, i0, images - i0 < JOIN_IMAGES ? images : i0 + JOIN_IMAGES, c, w, b, bias, s[0], s[1]);
+  join_threads<2>(s, lds);
+  if (threadIdx.x >= JOIN_X || !ok) return;
+  part_gate[(int64_t)blockIdx.x * 2 * d.C + c] = s[0];
+  part_gate[(int64_t)blockIdx.x * 2 * d.C + d.C + c] = s[1];
+}
+__global__ __launch_bounds__(JOIN_X* JOIN_Y) void resnorm_join_kernel(const Args a, const float* part_gate, int workgroups, int images, bool bias) {
+  __shared__ float lds[4][JOIN_WAVES][JOIN_X];
+  const srx_resnorm_desc& d = a.d;
+  const int y = threadIdx.x / JOIN_X, c = blockIdx.x * JOIN_X + (threadIdx.x & (JOIN_X - 1));
+  const bool ok = c < d.C, pre = d.dh && (d.dw_pre || d.db_pre);
+  const float* gate = d.gate_mode == GATE_CHANNEL ? static_cast<const float*>(d.gate) : nullptr;
+  float* dgate = gate ? static_cast<float*>(d.dgate) : nullptr;
+  const float w = ok && d.w_post ? d.w_post[c] : 1.f, b = ok && d.b_post ? d.b_post[c] : 0.f;
+  const float q = ok && gate ? gate[c] : 1.f;
+  float s[4] = {};                       // sum dh n, sum dh, sum D n (image gates: times s G), sum D
+  if (ok && pre) join_sum<JOIN_Y>(a.part_pre + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[0], s[1]);
+  if (d.f && d.gate_mode == GATE_IMAGE) {
+    if (part_gate) {
+      if (ok) join_sum<JOIN_Y>(part_gate + c, y, join_groups(images), 2 * d.C, bias ? d.C : 0, s[2], s[3]);
+    } else {
+      join_images(a, 0, images, c, w, b, bias, s[2], s[3]);
+    }
+  } else if (ok && d.f) {
+    join_sum<JOIN_Y>(a.part_post + c, y, workgroups, 2 * d.C, bias ? d.C : 0, s[2], s[3]);
+  }
+  join_threads<4>(s, lds);
+  if (y > 0 || !ok) return;
   if (pre && d.dw_pre) d.dw_pre[c] = s[0];
   if (pre && d.db_pre) d.db_pre[c] = s[1];
   if (!d.f) return;
@@ -167,7 +203,8 @@ int64_t srx_resnorm_ws_floats(const srx_resnorm_desc* d) {
   if (check("srx_resnorm_ws_floats", d)) return -1;
   Plan p = {};
   make_plan(*d, 1, p);
-  return 2 * (int64_t)d->C * (p.workgroups + (d->f && d->gate_mode == GATE_IMAGE ? p.a.items : p.workgroups)) + 1;
+  const bool image_gate = d->f && d->gate_mode == GATE_IMAGE;
+  return 2 * (int64_t)d->C * (p.workgroups + (image_gate ? p.a.items + join_groups(p.images) : p.workgroups)) + 1;
 }
 
 int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream) {
@@ -196,7 +233,14 @@ int srx_resnorm_backward(const srx_resnorm_desc* d, void* stream) {
     if (int rc = d->dtype == SRX_BF16 ? launch_bf16(p, 1, s) : launch_f32(p, 1, s)) return rc;
   const bool sums = d->dw_pre || d->db_pre || (d->f && (d->dw_post || d->db_post || (d->dgate && d->gate_mode && d->gate_mode != GATE_FULL)));
   if (!sums) return SRX_OK;
-  hipLaunchKernelGGL(resnorm_join_kernel, dim3((d->C + JOIN_X - 1) / JOIN_X), dim3(JOIN_X * JOIN_Y), 0, s, p.a, p.workgroups, p.images, general(*d));
+  const unsigned channels = (d->C + JOIN_X - 1) / JOIN_X;
+  float* part_gate = nullptr;
+  if (d->f && d->gate_mode == GATE_IMAGE && p.images > JOIN_IMAGES && d->ws) {
+    part_gate = p.a.part_post + 2 * (int64_t)d->C * p.a.items;
+    hipLaunchKernelGGL(resnorm_join_images_kernel, dim3(join_groups(p.images), channels), dim3(JOIN_X * JOIN_Y), 0, s, p.a, part_gate, p.images, general(*d));
+    if (int rc = srx_check_launch("resnorm_join_images")) return rc;
+  }
+  hipLaunchKernelGGL(resnorm_join_kernel, dim3(channels), dim3(JOIN_X * JOIN_Y), 0, s, p.a, part_gate, p.workgroups, p.images, general(*d));
   return srx_check_launch("resnorm_join");
 }
 
