@@ -122,7 +122,7 @@ class AdamW:
             self._bind()
             self._addresses, self._types = np.zeros(len(self.params), np.uint64), np.zeros(len(self.params), np.uint8)
             self._addresses_at, self._types_at = self._addresses.ctypes.data, self._types.ctypes.data
-            self._gather = L.host().gather
+            self._gather, self._none = L.host().gather, [None] * len(self.params)
             self._copy_masters()
             d = self._desc = L.AdamwDesc()
             d.state_bits, d.ntensors, d.ngroups = state_bits, len(self.params), len(self.param_groups)
@@ -190,7 +190,7 @@ class AdamW:
         if self._tensors is not None:
             torch.cuda.synchronize(self.device)      # steps in flight still read the old table
         self._tensors = raw.to(self.device)
-        self._ptrs = np.array(ptrs, dtype=np.uint64)
+        self._bound = np.array(ptrs + [2 * n + (t == torch.bfloat16) for n, t in zip(self._n, self._dtypes)], dtype=np.uint64)
 
     def _copy_masters(self) -> None:
         for i, p in enumerate(self.params):
@@ -212,7 +212,7 @@ class AdamW:
             raise ValueError(f"grad_scale must be finite, got {grad_scale}")
         d = self._desc
         if isinstance(grads, torch.Tensor):
-            if list(map(_ptr, self.params)) != self._ptrs.tolist():
+            if self._gather(self.params, self._none, self._bound, self._addresses, self._types, self.device.index) & _MOVED:
                 self._bind()
             if not self._flat:
                 raise ValueError("a flat gradient needs parameters of one type that are views covering one flat buffer")
@@ -228,12 +228,12 @@ class AdamW:
             if grads is not None and type(grads) is not list:
                 grads = list(grads)
             index = self.device.index
-            flags = self._gather(self.params, grads, self._ptrs, self._addresses, self._types, index)
+            flags = self._gather(self.params, grads, self._bound, self._addresses, self._types, index)
             if flags & _MOVED:
                 self._bind()
             if flags & _ODD:
                 grads = self._taken(grads)
-                flags = self._gather(self.params, grads, self._ptrs, self._addresses, self._types, index)
+                flags = self._gather(self.params, grads, self._bound, self._addresses, self._types, index)
             d.grads, d.flat_grad = self._addresses_at, None
             d.grad_dtypes = self._types_at if flags & _BF16 else None
         self._check_hyper()
@@ -358,8 +358,9 @@ class AdamW:
             steps.append(int(float(st["step"])) if st is not None else 0)
             if st is None:
                 continue
-            if tuple(st["exp_avg"].shape) != tuple(shp):
-                raise ValueError(f"optimizer state for parameter {i} has shape {tuple(st['exp_avg'].shape)}, expected {tuple(shp)}")
+            for key in ("exp_avg", "exp_avg_sq", "master"):
+                if key in st and tuple(st[key].shape) != tuple(shp):
+                    raise ValueError(f"optimizer state for parameter {i}: {key} has shape {tuple(st[key].shape)}, expected {tuple(shp)}")
             at = L.ADAMW_BLOCK * self._first[i]
             m[at:at + n].copy_(st["exp_avg"].reshape(-1))
             v[at:at + n].copy_(st["exp_avg_sq"].reshape(-1))

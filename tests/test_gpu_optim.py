@@ -440,3 +440,117 @@ def test_training_checkpoint_with_8_bit_moments(tmp_path):
     assert ck.load_latest_checkpoint(gen2, tr2.opt, tmp_path) == 4
     assert torch.equal(tr2.flat, tr.flat) and torch.equal(tr2.opt._m, tr.opt._m) and torch.equal(tr2.opt._v, tr.opt._v)
     assert tr2.opt.step_counts == tr.opt.step_counts
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("flat", [False, True])
+def test_a_small_step_in_one_launch_is_the_step(bits, flat):
+    """The same tensors beside one that makes the step large, and by themselves: same bits; captured and replayed too."""
+    sizes = [300, 0, 5000, 7, 64]
+    ps, gs = make(sizes, seed=3)
+    if flat:
+        buf, grad = torch.cat([p.detach() for p in ps]), torch.cat(gs)
+        ps, gs = [torch.nn.Parameter(x) for x in buf.split(sizes)], list(grad.split(sizes))
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    small = AdamW(ps, state_bits=bits, **HYPER)
+    large = AdamW(qs + [torch.zeros(64 * 4096, device=DEV)], state_bits=bits, **HYPER)
+    given = lambda k: [None if (k % 2 and i == 2) and not flat else g for i, g in enumerate(gs)]  # noqa: E731
+    call = lambda k: small.step(grad if flat else given(k))  # noqa: E731
+    for k in range(3):
+        call(k)
+        large.step(given(k) + [torch.zeros(64 * 4096, device=DEV)])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(3)
+        call(4)
+    for k in range(3):
+        for t in gs:
+            t.mul_(-0.5)
+        graph.replay()
+        for j in (3, 4):
+            large.step(given(j) + [torch.zeros(64 * 4096, device=DEV)])
+        torch.cuda.synchronize()
+    assert small.step_counts == large.step_counts[:5] == ([9] * 5 if flat else [9, 9, 5, 9, 9])
+    assert all(torch.equal(a, b) for a, b in zip(ps, qs))
+    for a, b in zip(small.moments(), large.moments()):
+        assert torch.equal(a, b[:a.numel()])
+
+
+def test_addresses_left_by_the_norm_pass():
+    """More tensors than one launch's addresses, of both types, some without a gradient, which change from step to step."""
+    g = torch.Generator().manual_seed(2)
+    sizes = [1 + int(k) for k in torch.randint(0, 700, (1000,), generator=g)]
+    ps, gs = make(sizes, seed=6)
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt, ref = AdamW(ps, max_grad_norm=1e9, **HYPER), AdamW(qs, **HYPER)          # a norm that never clips against none
+    for step in range(3):
+        give = [None if (k + step) % 5 == 0 else x.to(BF16) if (k + step) % 3 == 0 else x.clone() for k, x in enumerate(gs)]
+        opt.step(give)
+        ref.step(give)
+        del give
+    assert all(torch.equal(a, b) for a, b in zip(ps, qs)) and opt.step_counts == ref.step_counts
+    assert all(torch.equal(a, b) for a, b in zip(opt.moments(), ref.moments()))
+
+
+def test_a_parameter_that_changed_in_place_is_seen():
+    """Same address, other size, order or type: what the tables hold no longer describes it."""
+    for change, error in ((lambda t: t[:40], RuntimeError), (lambda t: t.view(BF16)[:64], RuntimeError),
+                          (lambda t: t.view(8, 8).t(), ValueError)):
+        for grads in (lambda p: [torch.ones_like(p)], lambda p: torch.ones(p.numel(), device=DEV)):
+            p = torch.nn.Parameter(torch.zeros(64, device=DEV))
+            opt = AdamW([p])
+            p.data = change(p.data)
+            with pytest.raises(error, match="build a new optimizer|not contiguous"):
+                opt.step(grads(p))
+            assert not p.any()
+
+
+def test_state_of_other_shapes_is_refused():
+    p = torch.nn.Parameter(torch.zeros(64, dtype=BF16, device=DEV))
+    opt = AdamW([p])
+    opt.step([torch.ones_like(p)])
+    for key in ("exp_avg", "exp_avg_sq", "master"):
+        sd = opt.state_dict()
+        sd["state"][0][key] = torch.zeros(1, device=DEV)
+        with pytest.raises(ValueError, match=key):
+            opt.load_state_dict(sd)
+
+
+def test_two_optimizers_on_two_streams():
+    streams, out = [torch.cuda.Stream() for _ in range(2)], []
+    for where in (None, streams):
+        sets = [make([30000, 77, 4096], seed=k) for k in range(2)]
+        opts = [AdamW(ps, state_bits=8, max_grad_norm=0.5, **HYPER) for ps, _ in sets]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for k in range(2):
+                with torch.cuda.stream(where[k] if where else torch.cuda.current_stream()):
+                    opts[k].step(sets[k][1])
+        torch.cuda.synchronize()
+        out.append([p.detach().clone() for ps, _ in sets for p in ps])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+def test_adversarial_trainer_steps_both_networks_with_it():
+    OPT, T = pkg("optim"), pkg("train")
+    torch.manual_seed(0)
+    gen = pkg("esrgan.generator").GeneratorESRGAN(num_blocks=1).to(DEV)
+    disc = pkg("esrgan.discriminator").Discriminator().to(DEV)
+    with pytest.warns(UserWarning):
+        vgg = pkg("utils.loss").VGGLoss(device=DEV, allow_synthetic=True)
+    built = []
+
+    def mk(module):
+        built.append(OPT.AdamW(OPT.decay_groups(module, 0.1), lr=1e-3, state_bits=8, max_grad_norm=1.0))
+        return built[-1]
+    tr = T.AdversarialTrainer(gen, disc, vgg, (2, 3, 16, 16), optimizer=mk)
+    assert built == [tr.opt_g, tr.opt_d]
+    lr = ORACLE.hash_input("optim.lr", (2, 3, 16, 16)).to(DEV)
+    hr = ORACLE.hash_input("optim.hr", (2, 3, 64, 64)).to(DEV)
+    before = [tr.flat_g.clone(), tr.flat_d.clone()]
+    for _ in range(2):
+        tr.step(lr, hr)
+    assert set(tr.opt_g.step_counts) == set(tr.opt_d.step_counts) == {2}
+    for a, b in zip(before, (tr.flat_g, tr.flat_d)):
+        # two steps of lr = 1e-3 that move each value by at most about lr / sqrt(1 - b2) ... * (1 - b1) each, and decay 1e-4
+        assert not torch.equal(a, b) and torch.isfinite(b).all() and float((a - b).abs().max()) < 2 * 1e-3 * 3.2 + 2e-4 * float(a.abs().max())
