@@ -429,8 +429,10 @@ int srx_adamw_moments_from8(const void* m_code, const void* v_code, const float*
  *     kind 0: a = f * w + b;  no h.
  * w, b: fp32 [C] or NULL (1, 0).  act: the identity (0) or the sigmoid (1).  f == NULL: only h = N_pre(x).
  * Statistics, products and sums are fp32; y and h are rounded once each.
+ * No output may overlap an input.
  * Layouts: SRX_RESNORM_PLANES, pixels contiguous [B][C][P] (a map of P pixels; *_stride = image stride), C <= 1024;
- * SRX_RESNORM_ROWS, channels contiguous, row b * P + p at (b * P + p) * *_stride, C <= 8192. */
+ * SRX_RESNORM_ROWS, channels contiguous, row b * P + p at (b * P + p) * *_stride, C <= 8192.  eps: at least FLT_MIN.  An image of more than
+ * 64 channels in planes stays under 4 GB; at most 2^30 images in planes or with gates for each. */
 #define SRX_RESNORM_PLANES 0
 #define SRX_RESNORM_ROWS 1
 #define SRX_RESNORM_MAX_PLANES_C 1024

@@ -169,6 +169,8 @@ int check(const char* what, const srx_resnorm_desc* d) {
   SRX_CHECK_ARG(d->dtype == SRX_BF16 || d->dtype == SRX_F32, "%s: bad dtype %d", what, d->dtype);
   SRX_CHECK_ARG(d->layout == SRX_RESNORM_PLANES || d->layout == SRX_RESNORM_ROWS, "%s: bad layout %d", what, d->layout);
   SRX_CHECK_ARG(d->B >= 0 && d->P >= 0 && d->C > 0, "%s: bad sizes B %d C %d P %d", what, d->B, d->C, d->P);
+  const bool by_image = (d->layout == SRX_RESNORM_PLANES && d->P > 1) || (d->f && d->gate_mode == GATE_IMAGE);
+  SRX_CHECK_ARG(!by_image || d->B <= (1 << 30), "%s: %d images, at most 2^30", what, d->B);
   const int most = d->layout == SRX_RESNORM_ROWS ? MAX_ROWS_C : MAX_PLANES_C;
   SRX_CHECK_ARG(d->C <= most, "%s: %d channels, at most %d in this layout", what, d->C, most);
   SRX_CHECK_ARG(d->post_kind >= 0 && d->post_kind <= 2 && d->pre_kind >= 0 && d->pre_kind <= 2, "%s: bad norm kind", what);

@@ -368,8 +368,8 @@ template <typename T, bool ROWS, bool UNI, int K, int V, bool GEN> struct Thread
       for (int q = 0; q < Q; ++q) s[q][0] = buf[w * N + q];
       lanes_sum<N>(&s[0][0], 1, waves);
     } else {
-      // slots of waves that the workgroup does not have hold zeros: all eight reads go out together
-      const int per = lanes() * N;
+      // slots of waves that the workgroup does not have hold zeros, whatever Q: all eight reads go out together
+      const int per = lanes() * MAX_Q * NP;
       if (UNI || lane < lanes())
 #pragma unroll
         for (int i = 0; i < N; ++i) buf[wave * per + l * N + i] = s[i / NP][i % NP];

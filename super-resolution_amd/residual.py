@@ -15,7 +15,6 @@ channels-last map gives channels-last results.  Statistics and sums are float32 
 """
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -25,6 +24,7 @@ from . import _lib as L
 
 KINDS = {"none": 0, "rms": 1, "layer": 2}
 ACTS = {"none": 0, "sigmoid": 1}
+_LARGEST = torch.finfo(torch.float32).max
 
 
 class NormSpec(NamedTuple):
@@ -39,8 +39,8 @@ class NormSpec(NamedTuple):
 def _checked_spec(spec: NormSpec, what: str, least: int = 1) -> None:
     if KINDS.get(spec.kind, -1) < least:
         raise ValueError(f"{what}: kind must be one of {[k for k, v in KINDS.items() if v >= least]}, got {spec.kind!r}")
-    if not 1e-37 <= spec.eps < math.inf:
-        raise ValueError(f"{what}: eps must be positive (at least 1e-37), got {spec.eps}")
+    if not 1e-37 <= spec.eps <= _LARGEST:
+        raise ValueError(f"{what}: eps must be positive (at least 1e-37) and a float32, got {spec.eps}")
 
 
 _NONE = NormSpec("none", None, None, 1.0)
@@ -79,8 +79,8 @@ def gated_residual(x: torch.Tensor, f: torch.Tensor, *, post: Optional[NormSpec]
         _checked_spec(pre, "pre")
     if gate_act not in ACTS:
         raise ValueError(f"gate_act must be one of {sorted(ACTS)}, got {gate_act!r}")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= _LARGEST:
+        raise ValueError(f"scale must be a finite float32, got {scale}")
     return _run(x, f, gate, ACTS[gate_act], scale, _NONE if post is None else post, _NONE if pre is None else pre, channel_dim)
 
 

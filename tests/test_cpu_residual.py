@@ -54,6 +54,23 @@ def test_null_descriptors_and_workspace():
     assert lib.srx_resnorm_forward(C.byref(_desc(L, B=0)), None) == 0          # nothing to do
 
 
+def test_sizes_at_the_limits():
+    L = pkg("_lib")
+    lib = L.lib()
+    far = {n + "_stride": 1 << 62 for n in ("x", "f", "y", "h", "dy", "dh", "dx", "df", "gate", "dgate")}
+    floats = lambda **kw: lib.srx_resnorm_ws_floats(C.byref(_desc(L, **far, **kw)))  # noqa: E731
+    # images of 2^30 and more; rows without a gate for each image are counted together
+    assert floats(B=(1 << 30) + 1) == -1 and b"images" in lib.srx_last_error()
+    assert floats(B=(1 << 30) + 1, layout=1, gate_mode=2) == -1 and floats(B=(1 << 31) - 1, layout=1) > 0 and floats(B=(1 << 31) - 1, P=1) > 0
+    assert floats(B=1 << 30, layout=1, gate_mode=2, P=1) > 2 * 64 * (1 << 30)
+    # an image of 4 GB: from 65 channels on
+    assert floats(C=65, P=1 << 25) == -1 and b"4 GB" in lib.srx_last_error()
+    assert floats(C=64, P=(1 << 31) - 1) > 0 and floats(C=1024, P=(1 << 20) - 1) > 0 and floats(C=1024, P=1 << 20) == -1
+    # the workspace does not grow with the pixels, nor with more images than run at once, but with their gates
+    assert floats(P=1 << 20) == floats(P=1 << 24)
+    assert floats(B=64, P=1 << 10) <= 2 * 64 * 2 * 1024 + 1
+
+
 def test_python_refusals():
     R = pkg("residual")
     x = torch.zeros(2, 8, 4, 4)
@@ -61,6 +78,12 @@ def test_python_refusals():
         R.channel_norm(x, R.NormSpec("rms"))
     with pytest.raises(RuntimeError, match="ROCm GPU only"):
         R.gated_residual(x, x)
+    for bad in (1e-38, 0.0, -1.0, float("nan"), float("inf"), 1e39):
+        with pytest.raises(ValueError, match="eps"):
+            R.channel_norm(x, R.NormSpec("rms", eps=bad))
+    for bad in (float("nan"), float("inf"), -1e39):
+        with pytest.raises(ValueError, match="scale"):
+            R.gated_residual(x, x, scale=bad)
     with pytest.raises(ValueError, match="kind"):
         R.ChannelNorm(8, "batch")
     with pytest.raises(ValueError, match="no blocks"):

@@ -647,3 +647,42 @@ def test_a_gate_of_each_row_in_fp32():
     want = rows_of(x, 1) + g.double().cpu() * norm64(rows_of(f, 1), post)
     lim = limits(x, f, None, post, pre, "none", float(g.abs().max()), 1)
     check(rows_of(y, 1), want, 64 * U * lim["y"], BF16, "y")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,dim", [((2, 20, 300, 301), 1), ((3, 99, 300, 101), 1), ((1, 5, 700, 701), 1), ((3, 40000, 40), 2), ((2, 30000, 136), 2)])
+def test_more_tiles_than_workgroups(shape, dim, dtype):
+    """Workgroups that take several tiles, with waves that a workgroup does not have, against the same pixels in parts."""
+    for k, (post, gate, pre, act) in enumerate((("rms", "channel", "rms", "none"), ("layer", "image", "layer", "sigmoid"))):
+        x, f, g, p, q = make(shape, dim, dtype, post, gate, pre, seed=k)
+        leaves = [t.requires_grad_() for t in (x, f, g, *p[1:3], *q[1:3]) if t is not None]
+        gen = torch.Generator().manual_seed(9)
+        dy, dh = (torch.randn(shape, generator=gen).to(DEV, dtype) for _ in range(2))
+
+        def run(x, f, g, dy, dh, leaves):
+            y, h = R().gated_residual(x, f, post=p, gate=g, gate_act=act, pre=q, scale=0.2, channel_dim=dim)
+            return [y.detach(), h.detach(), *torch.autograd.grad((y, h), leaves, (dy, dh))]
+        whole = run(x, f, g, dy, dh, leaves)
+        # in parts: pixels (rows) cut into ten, images one by one, each small enough that a workgroup takes one tile
+        at, cuts = (2 if dim == 1 else 1), 10
+        parts = []
+        for i in range(shape[0]):
+            for c in range(cuts):
+                piece = lambda t: t.detach()[i:i + 1].tensor_split(cuts, at)[c].contiguous()  # noqa: E731
+                a, b = piece(x).requires_grad_(), piece(f).requires_grad_()
+                gg = g.detach()[i:i + 1].requires_grad_() if gate == "image" else g
+                parts.append((i, run(a, b, gg, piece(dy), piece(dh), [a, b, gg] + leaves[3:])))
+        for k in range(4):            # y, h, dx, df: each pixel's own; the order of a sum over channels may differ
+            want = torch.cat([torch.cat([r[k] for j, r in parts if j == i], at) for i in range(shape[0])])
+            tol = (64 * U if dtype == F32 else 2.0 ** -7) * float(want.float().abs().max())
+            assert float((whole[k].float() - want.float()).abs().max()) <= tol, k
+        n = x.numel() // shape[dim]
+        for k in range(4, len(whole)):
+            vals = torch.stack([r[k].double().reshape(-1) for _, r in parts])
+            if k == 4 and gate == "image":
+                want = torch.stack([sum(r[k].double()[0] for j, r in parts if j == i) for i in range(shape[0])])
+            else:
+                want = vals.sum(0).view(whole[k].shape)
+            # sums of n terms, each below 60 in magnitude here and with a random sign: rounding in 32 bits over chains of a
+            # few hundred stays below 2^-24 * 64 of sum |term| <= 60 n
+            assert float((whole[k].double() - want).abs().max()) <= 64 * U * 60 * n, k
