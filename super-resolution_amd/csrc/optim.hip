@@ -20,7 +20,8 @@ constexpr int BLOCK = SRX_ADAMW_BLOCK;          // elements that share one scale
 constexpr int CHUNK = SRX_ADAMW_CHUNK;          // elements of one tensor that one workgroup updates
 constexpr int TPB = 256;
 constexpr int MAX_GRADS = 448;                  // addresses per launch: 3.6 KB of the 4 KB of kernel arguments
-constexpr int SMALL_GRADS = 128;                // the same beside 32 groups of constants
+constexpr int NEAR_GRADS = 896;                 // the same as 32-bit distances from the first in memory
+constexpr int SMALL_GRADS = 128;                // addresses beside 32 groups of constants
 constexpr int FLAT = 0, TABLE = -1;             // the other places of the gradients' addresses
 constexpr int PREP_TENSORS = 16384;             // tensors per prepare launch: one bit each, 2 KB of kernel arguments
 constexpr int PREP_TPB = 1024;
@@ -59,6 +60,7 @@ struct SmallArgs {
   srx_adamw_group groups[SRX_ADAMW_MAX_GROUPS];
 };
 struct NoArgs {};
+constexpr uint32_t NO_GRAD = ~0u;
 
 template <int NG, bool SMALL = false> struct StepArgs {
   const srx_adamw_tensor* tensors;
@@ -72,9 +74,13 @@ template <int NG, bool SMALL = false> struct StepArgs {
   int chunk0, t0;
   int flat_dtype;
   uint64_t is_bf16[(NG + 63) / 64 + (NG <= 0)];
-  const void* g[NG > 0 ? NG : 1];
+  uint64_t near_base;        // NG == NEAR_GRADS: gradient k is at near_base + (g[k] << near_shift), NO_GRAD: there is none
+  int near_shift;
+  std::conditional_t<NG == NEAR_GRADS, uint32_t, const void*> g[NG > 0 ? NG : 1];
   std::conditional_t<SMALL, SmallArgs, NoArgs> small;
 };
+
+static_assert(sizeof(StepArgs<MAX_GRADS>) <= 4096 && sizeof(StepArgs<NEAR_GRADS>) <= 4096 && sizeof(StepArgs<SMALL_GRADS, true>) <= 4096, "");
 
 struct Grad { const void* p; bool bf; };
 template <int NG, bool SMALL> __device__ __forceinline__ Grad grad_of(const StepArgs<NG, SMALL>& a, const srx_adamw_tensor& t, int ti) {
@@ -88,7 +94,8 @@ template <int NG, bool SMALL> __device__ __forceinline__ Grad grad_of(const Step
     r.p = reinterpret_cast<const void*>(p & ~1ull);
   } else {
     const int k = ti - a.t0;
-    r.p = a.g[k];
+    if constexpr (NG == NEAR_GRADS) r.p = a.g[k] == NO_GRAD ? nullptr : reinterpret_cast<const void*>(a.near_base + ((uint64_t)a.g[k] << a.near_shift));
+    else r.p = a.g[k];
     r.bf = (a.is_bf16[k >> 6] >> (k & 63)) & 1;
   }
   return r;
@@ -228,10 +235,26 @@ __global__ __launch_bounds__(PREP_TPB) void adamw_prepare_kernel(const PrepArgs 
   Coef* coef = reinterpret_cast<Coef*>(a.coef + 4);
   __shared__ double part[PREP_TPB / 64];
   __shared__ int skip_s;
+  // everything that does not need the norm comes first, beside its loads: the thread's first tensor
+  const int left = a.ntensors - a.t0 < PREP_TENSORS ? a.ntensors - a.t0 : PREP_TENSORS;
+  const auto has = [&](int k) { return k < left && ((a.has_grad[k >> 5] >> (k & 31)) & 1); };
+  const bool mine = has(threadIdx.x);
+  int step = 0, group = 0;
+  if (mine) {
+    step = a.steps[a.t0 + threadIdx.x] + 1;
+    group = a.tensors[a.t0 + threadIdx.x].group;
+  }
   int skip = 0;
   if (a.norm_mode == 1) {
+    // eight loads in flight: the sums come from other dies
     double s = 0;
-    for (int i = threadIdx.x; i < a.nchunks; i += PREP_TPB) s += a.partial[i];
+    for (int i0 = threadIdx.x; i0 < a.nchunks; i0 += 8 * PREP_TPB) {
+      double v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i0 + j * PREP_TPB < a.nchunks ? a.partial[i0 + j * PREP_TPB] : 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[j];
+    }
     s = wave_sum_d(s);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -250,21 +273,29 @@ __global__ __launch_bounds__(PREP_TPB) void adamw_prepare_kernel(const PrepArgs 
       ctl->skip = skip_s;
       a.norm[0] = (float)total;
     }
-    __syncthreads();
-    skip = skip_s;
   } else if (a.norm_mode == 2) {
     skip = ctl->skip;
   } else if (threadIdx.x == 0) {
     ctl->factor = (float)a.grad_scale;
     ctl->skip = 0;
   }
+  Coef first;
+  if (mine) first = coef_of(a.groups[group], step);
+  if (a.norm_mode == 1) {
+    __syncthreads();
+    skip = skip_s;
+  }
   if (skip) return;
-  for (int k = threadIdx.x; k < PREP_TENSORS && a.t0 + k < a.ntensors; k += PREP_TPB) {
-    if (!((a.has_grad[k >> 5] >> (k & 31)) & 1)) continue;
+  if (mine) {
+    a.steps[a.t0 + threadIdx.x] = step;
+    coef[a.t0 + threadIdx.x] = first;
+  }
+  for (int k = threadIdx.x + PREP_TPB; k < left; k += PREP_TPB) {
+    if (!has(k)) continue;
     const int i = a.t0 + k;
-    const int step = a.steps[i] + 1;
-    a.steps[i] = step;
-    coef[i] = coef_of(a.groups[a.tensors[i].group], step);
+    const int n = a.steps[i] + 1;
+    a.steps[i] = n;
+    coef[i] = coef_of(a.groups[a.tensors[i].group], n);
   }
 }
 
@@ -479,28 +510,55 @@ int check_moments(const char* what, const void* a, const void* b, const void* c,
   return SRX_OK;
 }
 
-template <int NG, bool SMALL = false> StepArgs<NG, SMALL> step_args(const srx_adamw_desc* d, int t0, int t1) {
+// Addresses as 32-bit distances from the first, in units of what all distances are multiples of (512 bytes for tensors of
+// their own): twice as many fit into a launch.
+struct Near {
+  uint64_t base = ~0ull;
+  int shift = 0;
+  static bool there(const srx_adamw_desc* d, int i) { return d->grads[i] && d->chunk_start[i + 1] > d->chunk_start[i]; }
+  bool fits(const srx_adamw_desc* d) {
+    uint64_t last = 0, any = 0;
+    for (int i = 0; i < d->ntensors; ++i)
+      if (there(d, i)) {
+        const uint64_t p = reinterpret_cast<uint64_t>(d->grads[i]);
+        base = p < base ? p : base;
+        last = p > last ? p : last;
+      }
+    for (int i = 0; i < d->ntensors; ++i)
+      if (there(d, i)) any |= reinterpret_cast<uint64_t>(d->grads[i]) - base;
+    if (!any) return true;
+    shift = __builtin_ctzll(any);
+    return (last - base) >> shift < NO_GRAD;
+  }
+  uint32_t of(const srx_adamw_desc* d, int i) const {
+    return there(d, i) ? (uint32_t)((reinterpret_cast<uint64_t>(d->grads[i]) - base) >> shift) : NO_GRAD;
+  }
+};
+
+template <int NG, bool SMALL = false> StepArgs<NG, SMALL> step_args(const srx_adamw_desc* d, const Near& near, int t0, int t1) {
   StepArgs<NG, SMALL> a = {};
   a.tensors = d->tensors; a.chunks = d->chunks; a.coef = d->coef; a.partial = d->partial;
   a.m = d->m; a.v = d->v; a.m_scale = d->m_scale; a.v_scale = d->v_scale;
   a.flat = d->flat_grad; a.flat_dtype = d->flat_dtype; a.chunk0 = d->chunk_start[t0]; a.t0 = t0;
-  if (NG == TABLE || d->ntensors > MAX_GRADS) a.table = reinterpret_cast<uint64_t*>(d->coef + 4 + 8 * (int64_t)d->ntensors);
+  if (NG == TABLE || (NG > 0 && d->ntensors > NG)) a.table = reinterpret_cast<uint64_t*>(d->coef + 4 + 8 * (int64_t)d->ntensors);
+  if constexpr (NG == NEAR_GRADS) { a.near_base = near.base; a.near_shift = near.shift; }
   if constexpr (NG > 0)
     for (int k = 0; k < t1 - t0; ++k) {
-      a.g[k] = d->grads[t0 + k];
+      if constexpr (NG == NEAR_GRADS) a.g[k] = near.of(d, t0 + k);
+      else a.g[k] = d->grads[t0 + k];
       if (d->grad_dtypes && d->grad_dtypes[t0 + k] == SRX_BF16) a.is_bf16[k >> 6] |= 1ull << (k & 63);
     }
   return a;
 }
 
 // One pass over the tensors in launches of at most NG gradients, `fn(args, chunks)` each.
-template <int NG, typename F> int each_launch(const srx_adamw_desc* d, F fn) {
+template <int NG, typename F> int each_launch(const srx_adamw_desc* d, const Near& near, F fn) {
   const int per = NG > 0 ? NG : d->ntensors;
   for (int t0 = 0; t0 < d->ntensors; t0 += per) {
     const int t1 = t0 + per < d->ntensors ? t0 + per : d->ntensors;
     const int n = d->chunk_start[t1] - d->chunk_start[t0];
     if (n <= 0) continue;
-    if (int rc = fn(step_args<NG>(d, t0, t1), n)) return rc;
+    if (int rc = fn(step_args<NG>(d, near, t0, t1), n)) return rc;
   }
   return SRX_OK;
 }
@@ -512,7 +570,7 @@ template <int NG, bool SMALL> int launch_step(const srx_adamw_desc* d, const Ste
 }
 
 template <int NG> int small_launch(const srx_adamw_desc* d, hipStream_t s) {
-  StepArgs<NG, true> a = step_args<NG, true>(d, 0, d->ntensors);
+  StepArgs<NG, true> a = step_args<NG, true>(d, {}, 0, d->ntensors);
   a.small.steps = d->steps;
   a.small.arrived = &reinterpret_cast<Ctl*>(d->coef)->arrived;
   a.small.grad_scale = d->grad_scale;
@@ -521,14 +579,14 @@ template <int NG> int small_launch(const srx_adamw_desc* d, hipStream_t s) {
   return launch_step(d, a, d->chunk_start[d->ntensors], s);
 }
 
-template <int NG> int step_launches(const srx_adamw_desc* d, hipStream_t s) {
+template <int NG> int step_launches(const srx_adamw_desc* d, const Near& near, hipStream_t s) {
   const int norm = d->max_norm > 0 || d->skip_nonfinite, chunks = d->chunk_start[d->ntensors];
   if (!norm && chunks > 0 && chunks <= SMALL_CHUNKS) {
     if constexpr (NG == FLAT) return small_launch<FLAT>(d, s);
-    else if (d->ntensors <= SMALL_GRADS) return small_launch<SMALL_GRADS>(d, s);
+    else if (NG == MAX_GRADS && d->ntensors <= SMALL_GRADS) return small_launch<SMALL_GRADS>(d, s);
   }
   if (norm) {
-    int rc = each_launch<NG>(d, [&](const StepArgs<NG>& a, int n) {
+    int rc = each_launch<NG>(d, near, [&](const StepArgs<NG>& a, int n) {
       hipLaunchKernelGGL(adamw_norm_kernel<NG>, dim3(n), dim3(TPB), 0, s, a);
       return srx_check_launch("adamw_norm");
     });
@@ -549,8 +607,8 @@ template <int NG> int step_launches(const srx_adamw_desc* d, hipStream_t s) {
   }
   const auto step = [&](const auto& a, int n) { return launch_step(d, a, n, s); };
   // the norm pass has left the addresses in device memory: the update needs no second launch for them
-  if (NG > 0 && norm && d->ntensors > NG) return each_launch<TABLE>(d, step);
-  return each_launch<NG>(d, step);
+  if (NG > 0 && norm && d->ntensors > NG) return each_launch<TABLE>(d, near, step);
+  return each_launch<NG>(d, near, step);
 }
 
 }  // namespace
@@ -588,7 +646,10 @@ int srx_adamw_step(const srx_adamw_desc* d, void* stream) {
                   q.beta1, q.beta2, q.eps, q.weight_decay);
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return d->flat_grad ? step_launches<FLAT>(d, s) : step_launches<MAX_GRADS>(d, s);
+  Near near;
+  if (d->flat_grad) return step_launches<FLAT>(d, near, s);
+  if (d->ntensors > MAX_GRADS && near.fits(d)) return step_launches<NEAR_GRADS>(d, near, s);
+  return step_launches<MAX_GRADS>(d, near, s);
 }
 
 int srx_adamw_moments_to8(const float* m, const float* v, void* m_code, void* v_code, float* m_scale, float* v_scale,

@@ -554,3 +554,25 @@ def test_adversarial_trainer_steps_both_networks_with_it():
     for a, b in zip(before, (tr.flat_g, tr.flat_d)):
         # two steps of lr = 1e-3 that move each value by at most about lr / sqrt(1 - b2) ... * (1 - b1) each, and decay 1e-4
         assert not torch.equal(a, b) and torch.isfinite(b).all() and float((a - b).abs().max()) < 2 * 1e-3 * 3.2 + 2e-4 * float(a.abs().max())
+
+
+@pytest.mark.parametrize("count", [460, 950])
+@pytest.mark.parametrize("clip", [None, 1e9])
+def test_gradients_far_apart(count, clip):
+    """Gradients more than 2^32 elements apart at addresses that share no alignment, against gradients side by side."""
+    sizes = [1 + k % 7 for k in range(count)]
+    ps, gs = make(sizes, seed=8)
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    space = torch.empty((1 << 32) + (1 << 20), device=DEV)
+    far, at = [], 1
+    for k, g in enumerate(gs):
+        lo = at if k % 2 else at + (1 << 32)
+        far.append(space[lo:lo + g.numel()])
+        far[-1].copy_(g)
+        at += g.numel()
+    give = lambda xs: [None if k % 11 == 5 else x for k, x in enumerate(xs)]  # noqa: E731
+    a, b = AdamW(ps, max_grad_norm=clip, **HYPER), AdamW(qs, max_grad_norm=clip, **HYPER)
+    for _ in range(2):
+        n, m = a.step(give(far)), b.step(give(gs))
+        assert clip is None or torch.equal(n, m)
+    assert all(torch.equal(x, y) for x, y in zip(ps, qs)) and a.step_counts == b.step_counts
