@@ -318,26 +318,34 @@ __device__ __forceinline__ float updated(float w, float m, float v, const Coef& 
 }
 // Codes of four values x against a block's largest, s: the nearest code of the correctly rounded quotient |x| / s.  The
 // reciprocal's product is within 3 units of it, so it gives the same code unless it lies that close to the middle
-// between two codes: then the division is made.
+// between two codes (about one block in 500): then the divisions are made.
 template <bool SIGNED> __device__ __forceinline__ uint32_t encode4(const float* x, float s) {
   constexpr unsigned base = SIGNED ? M_BASE : V_BASE, least = SIGNED ? 0 : 1;
   const float r = __builtin_amdgcn_rcpf(s);
-  float t[4];
-  bool near = !(s > 1e-30f && s < 1e30f);           // (a reciprocal that is no normal number)
+  unsigned t[4], middle = ~0u;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    t[j] = fabsf(x[j]) * r;
-    near = near || ((__float_as_uint(t[j]) + 0x80004u) & 0xFFFFFu) < 8u;
+    t[j] = __float_as_uint(fabsf(x[j]) * r);
+    const unsigned d = (t[j] << 12) + (0x80004u << 12);      // distance from four units below the middle, in the top 20 bits
+    middle = d < middle ? d : middle;
   }
-  if (__any(near))
-#pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = fabsf(x[j]) / s;
   uint32_t out = 0;
+  if (__any(!(s > 1e-30f && s < 1e30f) || middle < (8u << 12))) {           // (or a reciprocal that is no normal number)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unsigned c = encode(fabsf(x[j]) / s, base, least);
+      if (SIGNED) c |= c && x[j] < 0 ? 128u : 0u;   // a first moment that rounds to 0 loses its sign: one code for each value
+      out |= c << (8 * j);
+    }
+    return out;
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    unsigned c = encode(t[j], base, least);
-    if (SIGNED) c |= c && x[j] < 0 ? 128u : 0u;     // a first moment that rounds to 0 loses its sign: one code for each value
-    out |= c << (8 * j);
+    int c = (int)(t[j] + (0x80000u - (base << 20))) >> 20;   // no ties here
+    c = c > (int)least ? c : (int)least;
+    if (SIGNED) c |= (c + 127) & (__float_as_uint(x[j]) >> 24) & 128;       // the sign, where c > 0
+    else c = t[j] ? c : 0;
+    out |= (unsigned)c << (8 * j);
   }
   return out;
 }
