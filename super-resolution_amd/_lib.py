@@ -29,7 +29,6 @@ OP_RDB_BWD = 14
 vp, i32, i64, f32, f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_double
 
 ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_GROUPS = 256, 4096, 32
-RESNORM_PLANES, RESNORM_ROWS = 0, 1
 
 
 class PackSeg(C.Structure):

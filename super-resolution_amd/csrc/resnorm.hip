@@ -132,7 +132,12 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
   p.a.P = rows && !image_gate ? (int64_t)d.B * d.P : d.P;
   int tile;
   if (rows) {
-    p.elems = d.C <= 8 * THREADS ? 8 : 16;
+    // 16 elements a thread: where 8 would need more threads than there are, and where a wave then holds a row by itself and needs
+    // no barrier: forward in bf16, 4096 rows of 1024 7.5 us against 8.2, 32768 of 520 27.3 against 30.3, with means 4096 of 1024
+    // 10.3 against 11.3; not for few rows (100 of 768 3.9 against 3.5, 1000 4.3 against 4.2), a full gate beside (1531 of 1000 7.1
+    // against 6.6), in fp32 (8192 of 777 25.1 against 20.9) or backward (registers).
+    const bool row_in_wave = !backward && d.dtype == SRX_BF16 && d.gate_mode != GATE_FULL && d.C > 512 && d.C <= 1024 && p.a.P * p.images > 2048;
+    p.elems = d.C <= 8 * THREADS && !row_in_wave ? 8 : 16;
     p.a.lanes = pow2_at_least((d.C + p.elems - 1) / p.elems);
     p.threads = backward || p.a.lanes > 256 ? THREADS : 256;
     tile = p.threads / p.a.lanes;

@@ -686,3 +686,12 @@ def test_more_tiles_than_workgroups(shape, dim, dtype):
             # sums of n terms, each below 60 in magnitude here and with a random sign: rounding in 32 bits over chains of a
             # few hundred stays below 2^-24 * 64 of sum |term| <= 60 n
             assert float((whole[k].double() - want).abs().max()) <= 64 * U * 60 * n, k
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(3, 700, 520), (2, 1030, 1000), (1, 2049, 1024), (1, 2048, 1024), (2100, 513)])
+def test_rows_enough_for_a_wave_each(shape, dtype):
+    """Rows of more than 512 channels, on both sides of the number of rows from which a wave takes one by itself."""
+    for k, (post, gate, pre, act) in enumerate((("rms", "channel", "rms", "none"), ("layer", None, "layer", "none"))):
+        x, f, g, p, q = make(shape, len(shape) - 1, dtype, post, gate, pre, seed=k)
+        compare(x, f, g, p, q, act, dim=len(shape) - 1)
