@@ -130,6 +130,9 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
   const bool image_gate = d.f && d.gate_mode == GATE_IMAGE;
   p.images = rows && !image_gate ? 1 : d.B;
   p.a.P = rows && !image_gate ? (int64_t)d.B * d.P : d.P;
+  // Backward: as many workgroups as run at once, since each pays for its start, its sums over the lanes and its partial sums
+  // (about 9 us).
+  int64_t most = backward ? 256 : 4096;
   int tile;
   if (rows) {
     // 16 elements a thread: where 8 would need more threads than there are, and where a wave then holds a row by itself and needs
@@ -140,20 +143,32 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     p.elems = d.C <= 8 * THREADS && !row_in_wave ? 8 : 16;
     p.a.lanes = pow2_at_least((d.C + p.elems - 1) / p.elems);
     p.threads = backward || p.a.lanes > 256 ? THREADS : 256;
+    // Registers (113 in lean rows, 132 with a full gate, 147 general, 175 both) leave a compute unit two workgroups of eight
+    // waves, or one, or three and two of four waves.  The small ones need rows for their starts: from eight tiles each on.
+    // One of eight waves against several of four: 32768 rows of 520 in bf16 full 122 -> 92 us, general 135 -> 104, both 164 -> 158,
+    // fp32 general 185 -> 132; 4096 rows of 1024 29.7 -> 30.9, 1531 of 1000 24 -> 29.7 (not taken).
+    const bool lean = !general(d), full = d.gate_mode == GATE_FULL;
+    if (backward && p.elems == 8 && lean && !full) {
+      most = 512;
+    } else if (backward && p.elems == 8 && p.a.lanes <= 256) {
+      const int64_t many = !lean && full ? 512 : 768;
+      if (p.a.P * p.images / (256 / p.a.lanes) >= 8 * many) {
+        p.threads = 256;
+        most = many;
+      }
+    }
     tile = p.threads / p.a.lanes;
   } else {
     const int groups = d.C < PLANES_K ? d.C : (d.C + PLANES_K - 1) / PLANES_K;        // few channels: one a wave
     p.a.lanes = 64;
     while (groups * p.a.lanes > THREADS) p.a.lanes /= 2;
     p.threads = 64 * ((groups * p.a.lanes + 63) / 64);
+    if (backward) most = most * THREADS / p.threads;
     tile = p.a.lanes * PLANES_V;
   }
   // Workgroups walk the tiles side by side, neighbours in time being neighbours in memory.  With a gate for each image an item
   // stays within its image, so that its sums are the image's.
-  // Backward: as many workgroups as run at once, since each pays for its start, its sums over the lanes and its partial sums
-  // (about 9 us): 16 waves a compute unit for rows of root mean squares (113 registers), 8 otherwise.
   const int64_t tiles = (p.a.P + tile - 1) / tile;
-  const int64_t most = !backward ? 4096 : 256 * (rows && p.elems == 8 && !general(d) && d.gate_mode != GATE_FULL ? 1024 : 512) / p.threads;
   int64_t s = tiles;
   if (image_gate && p.images > 0 && s > (most + p.images - 1) / p.images) s = (most + p.images - 1) / p.images;
   if (p.images > 0 && s > (1LL << 30) / p.images) s = (1LL << 30) / p.images;

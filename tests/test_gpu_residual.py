@@ -695,3 +695,28 @@ def test_rows_enough_for_a_wave_each(shape, dtype):
     for k, (post, gate, pre, act) in enumerate((("rms", "channel", "rms", "none"), ("layer", None, "layer", "none"))):
         x, f, g, p, q = make(shape, len(shape) - 1, dtype, post, gate, pre, seed=k)
         compare(x, f, g, p, q, act, dim=len(shape) - 1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_many_rows_with_a_full_gate(kind, dtype):
+    """Enough rows for workgroups of four waves backward, against the same rows in parts that are too few for them."""
+    for rows, c in ((110000, 72), (13000, 1030)):
+        x, f, g, p, q = make((rows, c), 1, dtype, kind, "full", kind, seed=rows)
+        gen = torch.Generator().manual_seed(3)
+        dy, dh = (torch.randn((rows, c), generator=gen).to(DEV, dtype) for _ in range(2))
+        weights = [t.requires_grad_() for t in (*p[1:3], *q[1:3]) if t is not None]
+
+        def run(*ts):
+            a, b, k = (t.detach().requires_grad_() for t in ts[:3])
+            y, h = R().gated_residual(a, b, post=p, gate=k, gate_act="sigmoid", pre=q, scale=0.3, channel_dim=1)
+            return [y.detach(), h.detach(), *torch.autograd.grad((y, h), [a, b, k] + weights, ts[3:])]
+        whole = run(x, f, g, dy, dh)
+        parts = [run(*ts) for ts in zip(*(t.tensor_split(20) for t in (x, f, g, dy, dh)))]
+        for k in range(5):
+            want = torch.cat([r[k] for r in parts])
+            tol = (64 * U if dtype == F32 else 2.0 ** -7) * float(want.float().abs().max())
+            assert float((whole[k].float() - want.float()).abs().max()) <= tol, (rows, k)
+        for k in range(5, len(whole)):            # sums of `rows` terms below 60 each, as above
+            want = torch.stack([r[k].double() for r in parts]).sum(0)
+            assert float((whole[k].double() - want).abs().max()) <= 64 * U * 60 * rows, (rows, k)
