@@ -164,7 +164,16 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     while (groups * p.a.lanes > THREADS) p.a.lanes /= 2;
     p.threads = 64 * ((groups * p.a.lanes + 63) / 64);
     if (backward) most = most * THREADS / p.threads;
-    tile = p.a.lanes * PLANES_V;
+    // Pixels a thread: two; one where that leaves no more than half the compute units a workgroup (forward / backward, bf16: 1 x
+    // 64 x 64 x 64 3.9 / 12.2 us against 4.9 / 12.7 with two, means 5.2 / 16.8 against 6.6 / 18.9; but 16 x 64 x 64 x 64 9.5 against
+    // 8.7); four where few lanes lie along the pixels (16 x 512 x 64 x 64 50 / 136 against 54 / 167, 16 x 1024 x 64 x 64
+    // 153 / 263 against 245 / 366; but 16 x 256 x 16 x 16 7.0 / 17.6 against 5.4 / 13.8) and nothing else needs the registers
+    // (means: 8 x 1024 x 32 x 32 34 / 84 against 34 / 63).
+    const auto tiles = [&](int v) { return (p.a.P + p.a.lanes * v - 1) / (p.a.lanes * v) * p.images; };
+    p.elems = 2;
+    if (d.C >= PLANES_K && tiles(2) <= 128) p.elems = 1;
+    if (d.C > 256 && p.a.P >= 4 && tiles(4) >= 256 && !general(d) && d.gate_mode != GATE_FULL) p.elems = 4;
+    tile = p.a.lanes * p.elems;
   }
   // Workgroups walk the tiles side by side, neighbours in time being neighbours in memory.  With a gate for each image an item
   // stays within its image, so that its sums are the image's.
@@ -178,7 +187,7 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
   p.a.jump_images = p.workgroups / p.a.slices;
   p.a.jump_shares = p.workgroups % p.a.slices;
   const int waves = p.threads / 64;
-  int bytes = 2 * WAVES * MAX_Q * (rows ? 1 : p.a.lanes * PLANES_V) * 4;            // two buffers of a reduction: at most 16 KB
+  int bytes = 2 * WAVES * MAX_Q * (rows ? 1 : p.a.lanes * p.elems) * 4;            // two buffers of a reduction: at most 16 KB
   if (!rows) bytes += p.threads / p.a.lanes * PLANES_K * 16;                        // weights: at most 16 KB
   if (backward && rows && p.a.lanes < p.threads && bytes < waves * p.elems * 128 * 4) bytes = waves * p.elems * 128 * 4;   // flush: at most 64 KB
   p.lds_bytes = bytes;

@@ -4,7 +4,7 @@
 //
 // One kernel body serves both layouts.  A thread holds K x V elements of each tensor in registers:
 //   rows   (channels contiguous): V neighbouring channels, K times, of ONE row; `lanes` threads share a row.
-//   planes (pixels contiguous):   V neighbouring pixels of K channels; `lanes` threads of a wave sit side by side
+//   planes (pixels contiguous):   V neighbouring pixels (1, 2 or 4) of K channels; `lanes` threads of a wave sit side by side
 //                                 along the pixels, the others hold other channels of the same pixels.
 // Every tensor is read once: statistics, norm and gradients come out of the registers, in fp32.  The backward pass takes
 // x and f and forms y again: the same traffic as reading y, and not y's rounding to bf16 (which would put 2^-9 of
@@ -44,10 +44,10 @@ struct Args {
 struct Plan {
   Args a;
   int threads, workgroups, images;
-  int elems;               // rows: elements a thread holds
+  int elems;               // rows: elements a thread holds; planes: pixels
   int lds_bytes;
 };
-constexpr int PLANES_K = 8, PLANES_V = 2;
+constexpr int PLANES_K = 8;
 int launch_bf16(const Plan& p, int backward, hipStream_t s);
 int launch_f32(const Plan& p, int backward, hipStream_t s);
 
@@ -744,9 +744,13 @@ template <typename T, bool ROWS, bool UNI, int K, int V> int launch_for(const Pl
 }
 template <typename T> int launch(const Plan& p, int backward, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  if (p.a.d.layout == SRX_RESNORM_PLANES && p.a.d.C < PLANES_K) return launch_for<T, false, true, 1, PLANES_V>(p, backward, s);
-  if (p.a.d.layout == SRX_RESNORM_PLANES)
-    return p.a.lanes == 64 ? launch_for<T, false, true, PLANES_K, PLANES_V>(p, backward, s) : launch_for<T, false, false, PLANES_K, PLANES_V>(p, backward, s);
+  if (p.a.d.layout == SRX_RESNORM_PLANES) {
+    const bool uni = p.a.lanes == 64;
+    if (p.a.d.C < PLANES_K) return launch_for<T, false, true, 1, 2>(p, backward, s);
+    if (p.elems == 4) return launch_with<T, false, false, PLANES_K, 4, false, false>(p, backward, s);
+    if (p.elems == 1) return uni ? launch_for<T, false, true, PLANES_K, 1>(p, backward, s) : launch_for<T, false, false, PLANES_K, 1>(p, backward, s);
+    return uni ? launch_for<T, false, true, PLANES_K, 2>(p, backward, s) : launch_for<T, false, false, PLANES_K, 2>(p, backward, s);
+  }
   if (p.a.d.C < V) return launch_for<T, true, false, V, 1>(p, backward, s);           // rows shorter than a vector: one thread a row
   return p.elems == 8 ? launch_for<T, true, false, 8 / V, V>(p, backward, s) : launch_for<T, true, false, 16 / V, V>(p, backward, s);
 }

@@ -720,3 +720,12 @@ def test_many_rows_with_a_full_gate(kind, dtype):
         for k in range(5, len(whole)):            # sums of `rows` terms below 60 each, as above
             want = torch.stack([r[k].double() for r in parts]).sum(0)
             assert float((whole[k].double() - want).abs().max()) <= 64 * U * 60 * rows, (rows, k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(5, 64, 64, 66), (1, 130, 64, 66), (5, 300, 48, 47), (3, 1024, 40, 41), (9, 513, 18, 27), (300, 260, 5),
+                                   (300, 260, 3), (260, 700, 4), (150, 40, 2), (140, 300, 7)])
+def test_maps_with_two_and_four_pixels_a_thread(shape, dtype):
+    for k, (post, gate, pre, act) in enumerate((("rms", "channel", "rms", "none"), ("layer", "image", "layer", "sigmoid"), ("rms", "full", "rms", "none"))):
+        x, f, g, p, q = make(shape, 1, dtype, post, gate, pre, seed=k)
+        compare(x, f, g, p, q, act)
