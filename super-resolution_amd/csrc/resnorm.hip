@@ -148,7 +148,7 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     // One of eight waves against several of four: 32768 rows of 520 in bf16 full 122 -> 92 us, general 135 -> 104, both 164 -> 158,
     // fp32 general 185 -> 132; 4096 rows of 1024 29.7 -> 30.9, 1531 of 1000 24 -> 29.7 (not taken).
     const bool lean = !general(d), full = d.gate_mode == GATE_FULL;
-    if (backward && p.elems == 8 && lean && !full) {
+    if (backward && p.elems == 8 && lean && !full && d.C * (d.dtype == SRX_BF16 ? 2 : 4) >= 16) {
       most = 512;
     } else if (backward && p.elems == 8 && p.a.lanes <= 256) {
       const int64_t many = !lean && full ? 512 : 768;
@@ -163,7 +163,12 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     p.a.lanes = 64;
     while (groups * p.a.lanes > THREADS) p.a.lanes /= 2;
     p.threads = 64 * ((groups * p.a.lanes + 63) / 64);
-    if (backward) most = most * THREADS / p.threads;
+    // Whole workgroups that fit by their registers (140 lean: 12 waves a compute unit; 160 to 224: 8): with a few more, the chip
+    // runs twice for them (16 x 99 x 128 x 128 in bf16 178 us with 292, 112 with 256).  A channel a wave (60): more would fit than
+    // pay (three channels of 16 x 128 x 128 17 us, 20 with 24 waves; seven 34 us with one workgroup, 24 with two).
+    const bool light = p.a.lanes == 64 && !general(d) && d.gate_mode != GATE_FULL;
+    const int resident = d.C < PLANES_K ? 14 : light ? 12 : 8, waves = p.threads / 64;
+    if (backward) most *= waves < resident ? resident / waves : 1;
     // Pixels a thread: two; one where that leaves no more than half the compute units a workgroup (forward / backward, bf16: 1 x
     // 64 x 64 x 64 3.9 / 12.2 us against 4.9 / 12.7 with two, means 5.2 / 16.8 against 6.6 / 18.9; but 16 x 64 x 64 x 64 9.5 against
     // 8.7); four where few lanes lie along the pixels (16 x 512 x 64 x 64 50 / 136 against 54 / 167, 16 x 1024 x 64 x 64
@@ -179,7 +184,16 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
   // stays within its image, so that its sums are the image's.
   const int64_t tiles = (p.a.P + tile - 1) / tile;
   int64_t s = tiles;
-  if (image_gate && p.images > 0 && s > (most + p.images - 1) / p.images) s = (most + p.images - 1) / p.images;
+  if (image_gate && p.images > 0) {
+    // the shares of an image: as few rounds of workgroups as short as they can be (a share's own sums cost about two tiles); bf16
+    // 20 x 64 x 64 x 64 backward 27.6 us against 34.8 with the least number that keeps all compute units busy, 300 images 229 against 303
+    const int64_t base = most / p.images > 1 ? most / p.images : 1;
+    int64_t best = 0;
+    for (int64_t n = base; n <= base + 8 && n <= tiles; ++n) {
+      const int64_t cost = (p.images * n + most - 1) / most * ((tiles + n - 1) / n + 2);
+      if (!best || cost < best) { best = cost; s = n; }
+    }
+  }
   if (p.images > 0 && s > (1LL << 30) / p.images) s = (1LL << 30) / p.images;
   p.a.slices = s < 1 ? 1 : (int)s;
   p.a.items = p.a.P > 0 ? p.images * p.a.slices : 0;
