@@ -576,3 +576,24 @@ def test_gradients_far_apart(count, clip):
         n, m = a.step(give(far)), b.step(give(gs))
         assert clip is None or torch.equal(n, m)
     assert all(torch.equal(x, y) for x, y in zip(ps, qs)) and a.step_counts == b.step_counts
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_scalars_and_odd_shapes(bits):
+    shapes = [(), (1,), (3, 1, 5), (0, 4), (257,)]
+    ps = [torch.nn.Parameter(torch.full(s, 2.0, device=DEV)) for s in shapes]
+    for p in ps:
+        p.grad = torch.full(p.shape, 0.25, device=DEV)
+    opt = AdamW(ps, lr=0.125, weight_decay=0.0, state_bits=bits, eps=0.0)
+    opt.step()
+    # a first step: m / (1 - b1) = g, sqrt(v / (1 - b2)) = |g|: lr g / |g|, off by the roundings of ten operations on it
+    assert all(float((p.detach() - 1.875).abs().max()) <= 0.125 * 12 * 2.0 ** -23 + 2.0 ** -23 for p in ps if p.numel())
+    sd = opt.state_dict()
+    assert [tuple(sd["state"][k]["exp_avg"].shape) for k in range(5)] == shapes
+    other = AdamW([torch.nn.Parameter(p.detach().clone()) for p in ps], lr=0.125, weight_decay=0.0, state_bits=bits, eps=0.0)
+    other.load_state_dict(sd)
+    for p, q in zip(ps, other.params):
+        q.grad = p.grad
+    opt.step()
+    other.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, other.params)) and other.step_counts == opt.step_counts == [2] * 5

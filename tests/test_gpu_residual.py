@@ -729,3 +729,56 @@ def test_maps_with_two_and_four_pixels_a_thread(shape, dtype):
     for k, (post, gate, pre, act) in enumerate((("rms", "channel", "rms", "none"), ("layer", "image", "layer", "sigmoid"), ("rms", "full", "rms", "none"))):
         x, f, g, p, q = make(shape, 1, dtype, post, gate, pre, seed=k)
         compare(x, f, g, p, q, act)
+
+
+@pytest.mark.parametrize("dim,shape", [(1, (3, 40, 9, 11)), (2, (3, 50, 72))])
+def test_one_tensor_in_every_place(dim, shape):
+    """x, f and a full gate that are one leaf, norms that share their weights: gradients add up."""
+    c = shape[dim]
+    gen = torch.Generator().manual_seed(4)
+    t = torch.randn(shape, generator=gen).to(DEV).requires_grad_()
+    w, b = ((1 + 0.1 * torch.randn(c, generator=gen)).to(DEV).requires_grad_() for _ in range(2))
+    dy, dh = (torch.randn(shape, generator=gen).to(DEV) for _ in range(2))
+
+    def run(x, f, g, w2, b2, w1, b1):
+        y, h = R().gated_residual(x, f, post=R().NormSpec("layer", w2, b2), gate=g, pre=R().NormSpec("layer", w1, b1), channel_dim=dim)
+        return y, h
+    got = torch.autograd.grad(run(t, t, t, w, b, w, b), [t, w, b], (dy, dh))
+    parts = [v.detach().clone().requires_grad_() for v in (t, t, t, w, b, w, b)]
+    apart = torch.autograd.grad(run(*parts), parts, (dy, dh))
+    for g, want in zip(got, (apart[0] + apart[1] + apart[2], apart[3] + apart[5], apart[4] + apart[6])):
+        # the same kernels; only the order in which autograd adds two or three gradients may differ
+        assert float((g - want).abs().max()) <= 3 * 2.0 ** -24 * float(sum(v.abs().max() for v in apart[:3]) if g.shape == t.shape else 2 * want.abs().max() + 100)
+
+
+def test_graphs_of_two_calls_replayed_in_turn():
+    """Two captured passes of one shape hold workspaces of their own."""
+    sets = []
+    for k in range(2):
+        x, f, g, post, pre = make((4, 64, 20, 22), 1, BF16, "rms", "channel", "rms", seed=50 + k)
+        leaves = [t.requires_grad_() for t in (x, f, g, post.weight, pre.weight)]
+        sets.append((x, f, g, post, pre, leaves))
+
+    def run(s):
+        y, h = R().gated_residual(s[0], s[1], post=s[3], gate=s[2], pre=s[4])
+        return [v.detach() for v in (y, h, *torch.autograd.grad((y, h), s[5], (s[0].detach(), s[1].detach())))]
+    want = [[v.clone() for v in run(s)] for s in sets]
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(s))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(4):
+        for k in (0, 1) if turn % 2 else (1, 0):
+            for v in outs[k]:
+                v.zero_()
+        torch.cuda.synchronize()
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                graphs[k].replay()
+        run(sets[turn % 2])
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[k], want[k])), turn
