@@ -782,3 +782,11 @@ def test_graphs_of_two_calls_replayed_in_turn():
         torch.cuda.synchronize()
         for k in range(2):
             assert all(torch.equal(a, b) for a, b in zip(outs[k], want[k])), turn
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,dim", [((300, 64, 10, 22), 1), ((20, 64, 40, 41), 1), ((520, 8, 12, 12), 1), ((300, 40, 260), 2), ((600, 9, 70), 2)])
+def test_shares_of_images_in_rounds(shape, dim, dtype):
+    """Numbers of images that do not divide the workgroups: shares of one image on several, several on one."""
+    x, f, g, p, q = make(shape, dim, dtype, "rms", "image", "rms", seed=3)
+    compare(x, f, g, p, q, "sigmoid", dim=dim)
