@@ -1,16 +1,16 @@
 // AdamW over many tensors at once, moments in 32 or 8 bits, with the global gradient norm, clipping and the skip of a
 // step whose gradients are not finite.  See include/srx.h (srx_adamw_step) for the formulas and the buffers.
 //
-// Launches of one step: [norm pass over the gradients, 448 tensors a launch] + one "prepare" workgroup (finishes the
-// norm, advances the step counts, computes each tensor's bias-corrected constants) + the update, 448 tensors a launch, or
-// one launch where the norm pass has been there and left the addresses in device memory.  A small step without a norm is
-// one launch in all.
+// Launches of one step: [norm pass over the gradients, 448 tensors a launch, or 896 whose gradients lie near each other] + one
+// "prepare" workgroup (finishes the norm, advances the step counts, computes each tensor's bias-corrected constants) + the
+// update, in as many launches, or one where the norm pass has left the addresses in device memory.  A small step without a
+// norm is one launch in all.
 // The gradients' addresses travel in the kernel arguments: they change from step to step (autograd allocates new
 // gradients), and a table in device memory would need a host-to-device copy that a captured graph could not repeat.
 //
-// Bound: HBM.  702 tensors of 22800 fp32 elements (16.0 M): norm pass 14 us, prepare 3 to 5 us, update 74 us (6.0 TB/s: part
-// of the 448 MB stays in the last-level cache) with 32-bit moments, 54 us with 8-bit ones; whole step with clipping 95 and
-// 73 us.
+// Bound: HBM.  702 tensors of 22800 fp32 elements (16.0 M): norm pass 13 us, prepare 4 to 5 us, update 74 us (6.0 TB/s: part
+// of the 448 MB stays in the last-level cache) with 32-bit moments, 51 us with 8-bit ones; whole step with clipping 91 and
+// 66 us.
 #include <type_traits>
 #include "srx_common.h"
 

@@ -122,8 +122,8 @@ int pow2_at_least(int64_t n) {
   return p;
 }
 
-// The decomposition of a call: workspace size and launch use the same one.
-void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
+// The decomposition of a call; gen: whether it takes the general form.  Workspace size and launch use the same one.
+void make_plan(const srx_resnorm_desc& d, int backward, bool gen, Plan& p) {
   p.a.d = d;
   if (d.P == 1) p.a.d.layout = SRX_RESNORM_ROWS;          // one pixel an image: its channels are contiguous
   const bool rows = p.a.d.layout == SRX_RESNORM_ROWS;
@@ -147,7 +147,7 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     // waves, or one, or three and two of four waves.  The small ones need rows for their starts: from eight tiles each on.
     // One of eight waves against several of four: 32768 rows of 520 in bf16 full 122 -> 92 us, general 135 -> 104, both 164 -> 158,
     // fp32 general 185 -> 132; 4096 rows of 1024 29.7 -> 30.9, 1531 of 1000 24 -> 29.7 (not taken).
-    const bool lean = !general(d), full = d.gate_mode == GATE_FULL;
+    const bool lean = !gen, full = d.gate_mode == GATE_FULL;
     if (backward && p.elems == 8 && lean && !full && d.C * (d.dtype == SRX_BF16 ? 2 : 4) >= 16) {
       most = 512;
     } else if (backward && p.elems == 8 && p.a.lanes <= 256) {
@@ -166,7 +166,7 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     // Whole workgroups that fit by their registers (140 lean: 12 waves a compute unit; 160 to 224: 8): with a few more, the chip
     // runs twice for them (16 x 99 x 128 x 128 in bf16 178 us with 292, 112 with 256).  A channel a wave (60): more would fit than
     // pay (three channels of 16 x 128 x 128 17 us, 20 with 24 waves; seven 34 us with one workgroup, 24 with two).
-    const bool light = p.a.lanes == 64 && !general(d) && d.gate_mode != GATE_FULL;
+    const bool light = p.a.lanes == 64 && !gen && d.gate_mode != GATE_FULL;
     const int resident = d.C < PLANES_K ? 14 : light ? 12 : 8, waves = p.threads / 64;
     if (backward) most *= waves < resident ? resident / waves : 1;
     // Pixels a thread: two; one where that leaves no more than half the compute units a workgroup (forward / backward, bf16: 1 x
@@ -177,7 +177,7 @@ void make_plan(const srx_resnorm_desc& d, int backward, Plan& p) {
     const auto tiles = [&](int v) { return (p.a.P + p.a.lanes * v - 1) / (p.a.lanes * v) * p.images; };
     p.elems = 2;
     if (d.C >= PLANES_K && tiles(2) <= 128) p.elems = 1;
-    if (d.C > 256 && p.a.P >= 4 && tiles(4) >= 256 && !general(d) && d.gate_mode != GATE_FULL) p.elems = 4;
+    if (d.C > 256 && p.a.P >= 4 && tiles(4) >= 256 && !gen && d.gate_mode != GATE_FULL) p.elems = 4;
     tile = p.a.lanes * p.elems;
   }
   // Workgroups walk the tiles side by side, neighbours in time being neighbours in memory.  With a gate for each image an item
@@ -246,10 +246,16 @@ extern "C" {
 
 int64_t srx_resnorm_ws_floats(const srx_resnorm_desc* d) {
   if (check("srx_resnorm_ws_floats", d)) return -1;
-  Plan p = {};
-  make_plan(*d, 1, p);
-  const bool image_gate = d->f && d->gate_mode == GATE_IMAGE;
-  return 2 * (int64_t)d->C * (p.workgroups + (image_gate ? p.a.items + join_groups(p.images) : p.workgroups)) + 1;
+  // enough for either form: addresses decide between them
+  int64_t floats = 1;
+  for (const bool gen : {false, true}) {
+    Plan p = {};
+    make_plan(*d, 1, gen, p);
+    const bool image_gate = d->f && d->gate_mode == GATE_IMAGE;
+    const int64_t need = 2 * (int64_t)d->C * (p.workgroups + (image_gate ? p.a.items + join_groups(p.images) : p.workgroups)) + 1;
+    if (need > floats) floats = need;
+  }
+  return floats;
 }
 
 int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream) {
@@ -257,7 +263,7 @@ int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream) {
   if ((int64_t)d->B * d->P == 0) return SRX_OK;
   SRX_CHECK_ARG(d->x && (!d->f || d->y) && (!d->pre_kind || d->h), "srx_resnorm_forward: null tensor");
   Plan p = {};
-  make_plan(*d, 0, p);
+  make_plan(*d, 0, general(*d), p);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return d->dtype == SRX_BF16 ? launch_bf16(p, 0, s) : launch_f32(p, 0, s);
 }
@@ -269,7 +275,7 @@ int srx_resnorm_backward(const srx_resnorm_desc* d, void* stream) {
   SRX_CHECK_ARG(!d->dh || (d->pre_kind && (d->x || empty)), "srx_resnorm_backward: dh needs the norm before the next branch, and x");
   SRX_CHECK_ARG(empty || d->ws, "srx_resnorm_backward: null workspace");
   Plan p = {};
-  make_plan(*d, 1, p);
+  make_plan(*d, 1, general(*d), p);
   if (empty) p.a.slices = 0;            // the gradients of weights and gates are zeros
   p.a.part_pre = d->ws;
   p.a.part_post = d->ws + 2 * (int64_t)d->C * p.workgroups;

@@ -71,6 +71,23 @@ def test_sizes_at_the_limits():
     assert floats(B=64, P=1 << 10) <= 2 * 64 * 2 * 1024 + 1
 
 
+def test_workspace_does_not_go_by_addresses():
+    """Asked before the tensors are there, with weights or without, the size is enough for every form of the call."""
+    L = pkg("_lib")
+    lib = L.lib()
+    far = {n + "_stride": 1 << 62 for n in ("x", "f", "y", "h", "dy", "dh", "dx", "df", "gate", "dgate")}
+    for layout in (0, 1):
+        for c in (1, 5, 8, 24, 64, 99, 300, 520, 1000):
+            for b, p in ((1, 64), (16, 4096), (300, 1000), (3, 1), (2, 100000)):
+                for gate_mode in (0, 1, 2, 3):
+                    for kind in (1, 2):
+                        base = dict(far, layout=layout, C=c, B=b, P=p, gate_mode=gate_mode, post_kind=kind, pre_kind=kind, dtype=0)
+                        want = lib.srx_resnorm_ws_floats(C.byref(_desc(L, **base)))
+                        for more in (dict(b_post=256), dict(b_pre=256, db_pre=256), dict(x=None, y=None, h=None), dict(dy=256, dh=256, dx=256, df=256),
+                                     dict(pre_kind=0), dict(post_kind=0)):
+                            assert lib.srx_resnorm_ws_floats(C.byref(_desc(L, **{**base, **more}))) == want > 0
+
+
 def test_python_refusals():
     R = pkg("residual")
     x = torch.zeros(2, 8, 4, 4)
