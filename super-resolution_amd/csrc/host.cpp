@@ -136,10 +136,11 @@ Tensor fresh(const Order& o, const Tensor& like) {
 }
 
 // ------------------------------------------------------------------------------------------------ the operator
-// Calls recorded outside of a capture whose graphs still live: their leaves, and the stream they were recorded on.
-std::mutex eager_lock;
+// Calls recorded outside of a capture whose graphs still live: their leaves, and the stream they were recorded on.  (Never
+// destroyed: a graph may outlive this module's statics.)
 struct Call;
-std::unordered_map<const Call*, std::pair<std::vector<const void*>, const void*>> eager;
+std::mutex& eager_lock = *new std::mutex;
+auto& eager = *new std::unordered_map<const Call*, std::pair<std::vector<const void*>, const void*>>;
 
 struct Call : torch::CustomClassHolder {
   srx_resnorm_desc d;       // kinds, sizes, layout, gate
