@@ -57,7 +57,7 @@ def side_stream(device) -> "torch.cuda.Stream":
     caller's stream: on this runtime a stream that waits for an event of a LOWER-priority stream can
     keep that stream from ever being scheduled (observed: a high-priority stream waiting for the
     main stream, and the main stream waiting for a low-priority side stream while other processes
-    share the card; tools/stream_priority_probe.py), and a step's streams wait for each other in
+    share the card), and a step's streams wait for each other in
     both directions.  With equal priorities the hardware scheduler time-slices and every wait ends.
     The runtime gives each of the first four streams of a priority its own hardware queue, so this
     stream is created when the first plan or trainer is built (before a process group's streams):
@@ -67,10 +67,9 @@ def side_stream(device) -> "torch.cuda.Stream":
     idx = torch.cuda.current_device() if idx is None else idx
     st = _SIDE_STREAMS.get(idx)
     if st is None:
-        prio = int(os.environ.get("SRX_SIDE_STREAM_PRIORITY", "0"))     # A/B runs only
         out = C.c_void_p()
         with torch.cuda.device(idx):
-            L.check(L.lib().srx_stream_create(prio, C.byref(out)), "srx_stream_create")
+            L.check(L.lib().srx_stream_create(0, C.byref(out)), "srx_stream_create")
         st = torch.cuda.ExternalStream(out.value, device=torch.device("cuda", idx))
         _SIDE_STREAMS[idx] = st
     return st
