@@ -3,6 +3,7 @@
 //   resnorm(...)   residual.py's operator: argument checks, memory order, outputs, the autograd node (its backward pass runs
 //                  without Python), and the calls of libsrx's srx_resnorm_* entry points.
 //   gather(...)    optim.py's lists: addresses and types of hundreds of parameters and gradients in one pass.
+//   written(...)   tells autograd that a step has written those parameters.
 //   bind(...)      the addresses of libsrx's entry points (the library that _lib.py has loaded).
 //
 // libsrx itself stays free of torch: this module is to it what the ctypes binding is, for tensors.
@@ -465,6 +466,33 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   });
 }
 
+// written(params, addresses or None, others): advances the version counters of the parameters with an address (None: of
+// all) and, if there was one, of the other tensors, as an in-place operation would: a graph that saved one of them then refuses its
+// backward pass.  (Tensors made in inference mode have no counter and cannot be saved.)
+PyObject* written(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    if (nargs != 3) refuse(PyExc_TypeError, "written takes 3 arguments");
+    if (!PyList_Check(a[0]) || !PyList_Check(a[2])) refuse(PyExc_TypeError, "lists expected");
+    const Py_ssize_t n = PyList_GET_SIZE(a[0]);
+    std::optional<Buffer> addresses;
+    if (a[1] != Py_None) addresses.emplace(a[1], n * 8, "addresses");
+    const auto* at = addresses ? static_cast<const uint64_t*>(addresses->b.buf) : nullptr;
+    auto bump = [](PyObject* list, Py_ssize_t i) {
+      if (!THPVariable_Check(PyList_GET_ITEM(list, i))) refuse(PyExc_TypeError, "element ", i, " is not a tensor");
+      const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    bool any = false;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (!at || at[i]) {
+        bump(a[0], i);
+        any = true;
+      }
+    for (Py_ssize_t i = 0; any && i < PyList_GET_SIZE(a[2]); ++i) bump(a[2], i);
+    Py_RETURN_NONE;
+  });
+}
+
 // bind(srx_resnorm_forward, srx_resnorm_backward, srx_resnorm_ws_floats, srx_last_error): their addresses
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 4) {
@@ -488,6 +516,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {{"resnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(resnorm)), METH_FASTCALL, nullptr},
                          {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gather)), METH_FASTCALL, nullptr},
+                         {"written", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(written)), METH_FASTCALL, nullptr},
                          {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_srxhost", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

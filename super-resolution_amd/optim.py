@@ -44,7 +44,8 @@ class AdamW:
 
     ``param_groups`` holds the hyper-parameters under torch's names and is read at every step; ``lr`` sets them all.
     A captured step replays with the hyper-parameters and ``grad_scale`` it was captured with; its step count
-    advances.  One optimizer's steps share its state and workspaces: they must not overlap."""
+    advances.  One optimizer's steps share its state and workspaces: they must not overlap.  To autograd a step is an
+    in-place change of every parameter that it moves: a graph that saved one of them refuses its backward pass."""
 
     def __init__(self, params: Iterable, lr: float = 2e-4, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, max_grad_norm: Optional[float] = None,
@@ -122,7 +123,8 @@ class AdamW:
             self._bind()
             self._addresses, self._types = np.zeros(len(self.params), np.uint64), np.zeros(len(self.params), np.uint8)
             self._addresses_at, self._types_at = self._addresses.ctypes.data, self._types.ctypes.data
-            self._gather, self._none = L.host().gather, [None] * len(self.params)
+            self._gather, self._written, self._none = L.host().gather, L.host().written, [None] * len(self.params)
+            self._own = [t for t in (self._m, self._v, self.master) if t is not None]
             self._copy_masters()
             d = self._desc = L.AdamwDesc()
             d.state_bits, d.ntensors, d.ngroups = state_bits, len(self.params), len(self.param_groups)
@@ -246,6 +248,7 @@ class AdamW:
             norm = torch.empty((), dtype=torch.float32, device=self.device)
             d.norm = norm.data_ptr()
         L.check(self._lib.srx_adamw_step(C.byref(d), engine.stream_ptr(self.device)), "srx_adamw_step")
+        self._written(self.params, None if d.flat_grad else self._addresses, self._own)
         return norm
 
     def _empty_norm(self):
