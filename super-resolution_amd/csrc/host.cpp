@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
@@ -70,6 +71,24 @@ struct Order {
 };
 
 Tensor channels_last(const Tensor& t) { return t.movedim(1, -1); }
+
+// whether a tensor's storage holds all of it (a storage can be resized under its tensors; unstored zeros have one without memory)
+bool held(const Tensor& t) {
+  if (!t.numel()) return true;
+  if (!t.storage().data()) return false;
+  const size_t end = t.is_contiguous() ? (t.storage_offset() + t.numel()) * t.itemsize()
+                                       : at::detail::computeStorageNbytes(t.sizes(), t.strides(), t.itemsize(), t.storage_offset());
+  return end <= t.storage().nbytes();
+}
+void need_held(const Tensor& t) { TORCH_CHECK(held(t), "a tensor of shape ", t.sizes(), " whose memory has been freed"); }
+// t with its values in memory: a view whose values are the negatives of what lies there, and a tensor of zeros without memory,
+// are copied (both count as contiguous)
+Tensor in_memory(const Tensor& t) {
+  if (!t.defined() || t.layout() != at::kStrided) return t;
+  if (t._is_zerotensor()) return t.clone();
+  need_held(t);
+  return t.is_neg() ? t.clone() : t;
+}
 
 Order order_of(const Tensor& x, int64_t channel_dim) {
   const int64_t dims = x.dim();
@@ -154,18 +173,23 @@ struct Call : torch::CustomClassHolder {
   }
 };
 
-const void* address(const Tensor& t) { return t.numel() ? t.data_ptr() : reinterpret_cast<const void*>(16); }       // nothing is read from an empty tensor
+const void* address(const Tensor& t) {
+  if (!t.numel()) return reinterpret_cast<const void*>(16);       // nothing is read from an empty tensor
+  need_held(t);
+  return t.data_ptr();
+}
 
 struct Put {                // tensors that have to live until the launch
   std::vector<Tensor> keep;
   const Order& order;
   template <typename P> void operator()(const Tensor& t, P& ptr, int64_t& stride) {
     if (!t.defined()) return;
+    need_held(t);
     keep.push_back(taken(order, t, stride));
     ptr = const_cast<void*>(address(keep.back()));
   }
 };
-const float* vec(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+const float* vec(const Tensor& t) { return t.defined() ? static_cast<const float*>(address(t)) : nullptr; }
 
 void put_common(Put& put, srx_resnorm_desc& d, const Tensor& gate, const Tensor& w_post, const Tensor& b_post, const Tensor& w_pre,
                 const Tensor& b_pre) {
@@ -218,7 +242,7 @@ struct ResNorm : torch::autograd::Function<ResNorm> {
     const Call& c = static_cast<const Call&>(*holder);
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &f = saved[1], &gate = saved[2];
-    const Tensor dy = c.branch ? grads.front() : Tensor(), dh = c.d.pre_kind ? grads.back() : Tensor();
+    const Tensor dy = in_memory(c.branch ? grads.front() : Tensor()), dh = in_memory(c.d.pre_kind ? grads.back() : Tensor());
     variable_list out(8);                       // of the call, x, f, gate, w_post, b_post, w_pre, b_pre
     if (!dy.defined() && !dh.defined()) return out;
     // inputs that were given, in order, are the node's edges
@@ -288,7 +312,7 @@ Tensor channel_vector(const Tensor& t, const Order& o, const Tensor& x, const ch
   if (!t.defined()) return t;
   if (t.dim() != 1 || t.size(0) != o.C || t.device() != x.device() || !t.is_floating_point())
     refuse(PyExc_ValueError, what, ": ", o.C, " values on ", x.device(), " expected, got ", t.scalar_type(), " of shape ", t.sizes(), " on ", t.device());
-  return t.to(at::kFloat).contiguous();
+  return in_memory(t).to(at::kFloat).contiguous();
 }
 
 // Autograd keeps one accumulator per leaf for as long as any graph of that leaf lives, bound to the stream it was first used
@@ -333,10 +357,10 @@ double float_arg(PyObject* o) {
 PyObject* resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 14) refuse(PyExc_TypeError, "resnorm takes 14 arguments");
-    const Tensor x = tensor_arg(a[0], "x");
-    if (!x.defined()) refuse(PyExc_TypeError, "x must be a tensor");
-    const Tensor f = tensor_arg(a[1], "f");
-    Tensor gate = tensor_arg(a[2], "gate");
+    variable_list given = {tensor_arg(a[0], "x"), tensor_arg(a[1], "f"), tensor_arg(a[2], "gate")};       // before any copy or conversion: the graph's leaves
+    if (!given[0].defined()) refuse(PyExc_TypeError, "x must be a tensor");
+    const Tensor x = in_memory(given[0]), f = in_memory(given[1]);
+    Tensor gate = in_memory(given[2]);
     auto c = c10::make_intrusive<Call>();
     c->order = order_of(x, PyLong_AsLongLong(a[13]));
     const Order& o = c->order;
@@ -373,7 +397,6 @@ PyObject* resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
       d.gate_act = (int32_t)PyLong_AsLong(a[11]);
     }
-    variable_list given = {x, f, tensor_arg(a[2], "gate")};          // before a conversion to fp32: the graph's leaves
     auto vector_arg = [&](int at, const char* what) {
       given.push_back(tensor_arg(a[at], what));
       return channel_vector(given.back(), o, x, what);
@@ -423,8 +446,8 @@ struct Buffer {
 
 // gather(params, grads or None, bound, addresses, types, device index) -> flags.  Compares the parameters with bound[2 n]
 // (uint64: addresses, then elements times two, plus one for bf16), and writes the gradients' addresses (uint64[n], 0: none)
-// and types (uint8[n]).  GATHER_MOVED: a parameter's address, size or type differs, or it is not contiguous.  GATHER_ODD: a gradient cannot be taken as it is (shape, type, device, order) and the
-// caller has to look.  GATHER_BF16: some gradient is bf16.  grads None: each parameter's .grad.
+// and types (uint8[n]).  GATHER_MOVED: a parameter's address, size or type differs, or it is not contiguous, a negative view or without its memory.
+// GATHER_ODD: a gradient cannot be taken as it is (shape, type, device, order, a negative view, no memory) and the caller has to look.  GATHER_BF16: some gradient is bf16.  grads None: each parameter's .grad.
 PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     if (nargs != 6) refuse(PyExc_TypeError, "gather takes 6 arguments");
@@ -443,7 +466,7 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       if (!THPVariable_Check(PyList_GET_ITEM(a[0], i))) refuse(PyExc_TypeError, "parameter ", i, " is not a tensor");
       const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(a[0], i));
       if (reinterpret_cast<uint64_t>(p.data_ptr()) != was[i] || 2 * (uint64_t)p.numel() + (p.scalar_type() == at::kBFloat16) != was[n + i] ||
-          !p.is_contiguous())
+          !p.is_contiguous() || p.is_neg() || !held(p))
         flags |= GATHER_MOVED;
       to[i] = 0;
       ty[i] = SRX_F32;
@@ -451,7 +474,7 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       if (given && go != Py_None && !THPVariable_Check(go)) refuse(PyExc_TypeError, "gradient ", i, " is a ", Py_TYPE(go)->tp_name, ", not a tensor");
       const Tensor& g = given ? (go == Py_None ? Tensor() : THPVariable_Unpack(go)) : p.grad();
       if (!g.defined()) continue;
-      if (g.layout() != at::kStrided || g.sizes() != p.sizes() || g.device().index() != index || g.device().type() != p.device().type() ||
+      if (g.layout() != at::kStrided || g.is_neg() || !held(g) || g.sizes() != p.sizes() || g.device().index() != index || g.device().type() != p.device().type() ||
           (g.scalar_type() != at::kFloat && g.scalar_type() != at::kBFloat16) || !g.is_contiguous()) {
         flags |= GATHER_ODD;
         continue;

@@ -23,6 +23,21 @@ _MOVED, _ODD, _BF16 = 1, 2, 4              # flags of the host module's gather()
 _DTYPE_ID = {torch.bfloat16: L.BF16, torch.float32: L.F32}
 
 
+def _need_held(t: torch.Tensor, what: str) -> None:
+    """A storage can be resized under its tensors."""
+    end = t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+    if t.numel() and end * t.element_size() > t.untyped_storage().nbytes():
+        raise ValueError(f"{what}: its memory has been freed")
+
+
+def _in_memory(t: torch.Tensor, what: str) -> torch.Tensor:
+    """t with its values in memory: a negative view and a tensor of zeros without memory are copied (both count as contiguous)."""
+    if t._is_zerotensor():
+        return t.detach().clone()
+    _need_held(t, what)
+    return t.detach().clone() if t.is_neg() else t
+
+
 def decay_groups(module: torch.nn.Module, weight_decay: float = 1e-2) -> List[dict]:
     """Two parameter groups of a module, in ``parameters()`` order within each: tensors with two or more dimensions
     (kernels) decay; norm weights, gates and biases do not."""
@@ -169,6 +184,9 @@ class AdamW:
                                    f"{p.dtype} of {p.numel()} on {p.device}: build a new optimizer")
             if not p.is_contiguous():
                 raise ValueError(f"AdamW: parameter {i} is not contiguous")
+            if p.is_neg():
+                raise ValueError(f"AdamW: parameter {i} is a negative view: its memory holds other values than it")
+            _need_held(p, f"AdamW: parameter {i}")
         spans = sorted((a, a + n * p.element_size(), i) for i, (a, n, p) in enumerate(zip(ptrs, self._n, self.params)) if n)
         for (_, end, i), (begin, _, k) in zip(spans, spans[1:]):
             if begin < end:
@@ -221,6 +239,7 @@ class AdamW:
             if grads.device != self.device or grads.dtype not in _DTYPE_ID or grads.numel() != sum(self._n) or not grads.is_contiguous():
                 raise ValueError(f"flat gradient: {sum(self._n)} contiguous float32 or bfloat16 values on {self.device} expected, got "
                                  f"{grads.dtype} of {tuple(grads.shape)} on {grads.device}")
+            grads = _in_memory(grads, "flat gradient")
             d.grads, d.grad_dtypes = None, None
             d.flat_grad, d.flat_dtype = grads.data_ptr(), _DTYPE_ID[grads.dtype]
             if grads.numel() == 0:
@@ -264,7 +283,7 @@ class AdamW:
                 raise ValueError(f"gradient {i} has shape {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {p.device}")
             if g.dtype not in _DTYPE_ID or g.layout != torch.strided:
                 raise ValueError(f"gradient {i}: a dense float32 or bfloat16 tensor expected, got {g.dtype}, {g.layout}")
-        return [g if g is None else g.contiguous() for g in grads]
+        return [g if g is None else _in_memory(g, f"gradient {i}").contiguous() for i, g in enumerate(grads)]
 
     def zero_grad(self, set_to_none: bool = True) -> None:
         for p in self.params:

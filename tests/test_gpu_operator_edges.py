@@ -51,3 +51,100 @@ def test_versions_of_masters_moments_and_inference_tensors():
     # a first step of lr g / |g|, off by 12 roundings of it
     off = float((q - 0.5).abs().max())
     assert off <= 12 * 2.0 ** -24
+
+
+def negative(t):
+    """t's values as a view with the negative bit: the memory holds -t."""
+    n = torch._neg_view(-t.detach())
+    assert n.is_neg() and torch.equal(n, t)
+    return n
+
+
+@pytest.mark.parametrize("shape,dim", [((2, 40, 6, 10), 1), ((3, 20, 40), 2)])
+def test_negative_views_are_their_values(shape, dim):
+    g = torch.Generator().manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=g).to(DEV)  # noqa: E731
+    c = shape[dim]
+    plain = [rand(*shape), rand(*shape), rand(*shape), 1 + rand(c), rand(c), 1 + rand(c), rand(c), rand(*shape), rand(*shape)]
+
+    def run(t):
+        leaves = [a.detach().requires_grad_() for a in t[:7]]
+        x, f, gate, w2, b2, w1, b1 = leaves
+        y, h = R().gated_residual(x, f, post=R().NormSpec("layer", w2, b2), gate=gate, gate_act="sigmoid", scale=0.5,
+                                  pre=R().NormSpec("layer", w1, b1), channel_dim=dim)
+        with torch.no_grad():
+            serving = R().gated_residual(x, f, post=R().NormSpec("layer", w2, b2), gate=gate, gate_act="sigmoid", scale=0.5,
+                                         pre=R().NormSpec("layer", w1, b1), channel_dim=dim)
+        return [y, h, *serving, *torch.autograd.grad((y, h), leaves, t[7:])]
+    want = run(plain)
+    for i in range(9):
+        got = run([negative(t) if k == i else t for k, t in enumerate(plain)])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+    z = torch.view_as_real(torch.complex(plain[0], plain[1]))[..., 1]          # strides of two, no bit
+    assert torch.equal(R().channel_norm(z, R().NormSpec("rms"), dim), R().channel_norm(plain[1], R().NormSpec("rms"), dim))
+    z = torch.complex(plain[0], plain[1]).conj().imag
+    assert z.is_neg() and torch.equal(R().channel_norm(z, R().NormSpec("rms"), dim), R().channel_norm(-plain[1], R().NormSpec("rms"), dim))
+
+
+def test_negative_gates_of_images():
+    x, f = torch.randn(3, 40, 9, device=DEV), torch.randn(3, 40, 9, device=DEV)
+    for gate in (torch.randn(40, device=DEV), torch.randn(3, 40, device=DEV), torch.randn(3, 40, device=DEV, dtype=BF16)):
+        assert torch.equal(R().gated_residual(x, f, gate=negative(gate)), R().gated_residual(x, f, gate=gate))
+
+
+def test_adamw_takes_negative_gradients_for_their_values_and_refuses_such_parameters():
+    p0, g = torch.randn(500, device=DEV), torch.randn(500, device=DEV)
+    out = []
+    for way in (lambda o: o.step([g]), lambda o: o.step([negative(g)]), lambda o: o.step(negative(g)), lambda o: o.step([negative(g.to(BF16)).float()])):
+        p = torch.nn.Parameter(p0.clone())
+        opt = pkg("optim").AdamW([p], max_grad_norm=1.0)
+        way(opt)
+        out.append((p.detach(), *opt.moments()))
+    assert all(torch.equal(a, b) for k in (1, 2) for a, b in zip(out[0], out[k]))
+    with pytest.raises(ValueError, match="negative view"):
+        pkg("optim").AdamW([negative(p0)])
+    opt = pkg("optim").AdamW([torch.nn.Parameter(p0.clone())], state_bits=8)
+    m, v = opt.moments()
+    opt.load_moments(negative(m + 1), negative(v + 1), 1)
+    assert torch.equal(opt.moments()[0][:256], m[:256] + 1)
+
+
+def freed(t):
+    t = t.clone()
+    t.untyped_storage().resize_(0)
+    return t
+
+
+def test_tensors_without_memory():
+    """Zeros that are not stored count as zeros; a storage that was freed under its tensors is an error."""
+    x, f, w, p0 = (torch.randn(s, device=DEV) for s in ((6, 40), (6, 40), (40,), (40,)))
+    zero = torch._efficientzerotensor(6, 40, device=DEV)
+    spec = R().NormSpec("rms", w)
+    assert torch.equal(R().gated_residual(x, zero, post=spec), x) and not R().channel_norm(zero, spec).any()
+    for call in (lambda: R().channel_norm(freed(x), spec), lambda: R().channel_norm(freed(torch.randn(40, 6, device=DEV).t()), spec), lambda: R().gated_residual(x, freed(f)),
+                 lambda: R().channel_norm(x, R().NormSpec("rms", freed(w))), lambda: R().gated_residual(x, f, gate=freed(w)),
+                 lambda: R().gated_residual(x, f, gate=freed(x))):
+        with pytest.raises(RuntimeError, match="memory has been freed"):
+            call()
+    a = x.clone().requires_grad_()
+    h = R().channel_norm(a, spec)
+    dx, = torch.autograd.grad(h, a, zero, retain_graph=True)
+    assert not dx.any()
+    a.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="memory has been freed"):
+        torch.autograd.grad(h, a, torch.ones_like(h))
+    p = torch.nn.Parameter(p0.clone())
+    opt = pkg("optim").AdamW([p], lr=0.5, weight_decay=0.5)
+    for step in (lambda: opt.step([torch._efficientzerotensor(40, device=DEV)]), lambda: opt.step(torch._efficientzerotensor(40, device=DEV))):
+        before = p.detach().clone()
+        step()
+        off = float((p.detach() - 0.75 * before).abs().max())           # a gradient of zeros: the decay alone
+        assert off <= 2.0 ** -23 * 4
+    assert opt.step_counts == [2]
+    for step in (lambda: opt.step([freed(w)]), lambda: opt.step(freed(w))):
+        with pytest.raises(ValueError, match="freed"):
+            step()
+    opt.step([None])
+    p.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="freed"):
+        opt.step([w])
