@@ -16,6 +16,9 @@
 #include <c10/core/DeviceGuard.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/custom_class.h>
 #include <mutex>
 #include <unordered_map>
@@ -46,6 +49,21 @@ template <typename F> PyObject* guarded(F f) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
   return nullptr;
+}
+
+// ------------------------------------------------------------------------------------------------ what cannot follow these calls
+// A trace records torch's own operations: it would hold the allocation of the outputs and nothing that writes them.
+void need_untraced(const char* what) {
+  const bool proxies = c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                       c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+  if (torch::jit::tracer::isTracing() || proxies || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch))
+    refuse(PyExc_RuntimeError, what, " cannot be traced (torch.jit.trace, make_fx, torch.export): its kernels are no torch operations");
+}
+// A tangent (torch.autograd.forward_ad) would be dropped.
+void need_no_tangent(const variable_list& given) {
+  for (const Tensor& t : given)
+    if (t.defined() && t._fw_grad(/*level=*/0).defined())
+      refuse(PyExc_RuntimeError, "gated_residual and channel_norm have no forward-mode derivative: an input carries a tangent");
 }
 
 // ------------------------------------------------------------------------------------------------ libsrx
@@ -245,6 +263,12 @@ struct ResNorm : torch::autograd::Function<ResNorm> {
     const Tensor dy = in_memory(c.branch ? grads.front() : Tensor()), dh = in_memory(c.d.pre_kind ? grads.back() : Tensor());
     variable_list out(8);                       // of the call, x, f, gate, w_post, b_post, w_pre, b_pre
     if (!dy.defined() && !dh.defined()) return out;
+    try {
+      need_untraced("the backward pass of gated_residual and channel_norm");
+      need_no_tangent(grads);
+    } catch (const Refused& r) {
+      TORCH_CHECK(false, r.msg);
+    }
     // inputs that were given, in order, are the node's edges
     bool need[8] = {};
     size_t edge = 0;
@@ -357,11 +381,15 @@ double float_arg(PyObject* o) {
 PyObject* resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 14) refuse(PyExc_TypeError, "resnorm takes 14 arguments");
-    variable_list given = {tensor_arg(a[0], "x"), tensor_arg(a[1], "f"), tensor_arg(a[2], "gate")};       // before any copy or conversion: the graph's leaves
+    static const char* const names[] = {"x", "f", "gate", "post.weight", "post.bias", "pre.weight", "pre.bias"};
+    variable_list given;             // before any copy or conversion: the graph's leaves
+    for (int i = 0; i < 7; ++i) given.push_back(tensor_arg(a[i], names[i]));
     if (!given[0].defined()) refuse(PyExc_TypeError, "x must be a tensor");
+    need_untraced("gated_residual and channel_norm");
+    need_no_tangent(given);
+    auto c = c10::make_intrusive<Call>();
     const Tensor x = in_memory(given[0]), f = in_memory(given[1]);
     Tensor gate = in_memory(given[2]);
-    auto c = c10::make_intrusive<Call>();
     c->order = order_of(x, PyLong_AsLongLong(a[13]));
     const Order& o = c->order;
     c->branch = f.defined();
@@ -397,12 +425,8 @@ PyObject* resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
       }
       d.gate_act = (int32_t)PyLong_AsLong(a[11]);
     }
-    auto vector_arg = [&](int at, const char* what) {
-      given.push_back(tensor_arg(a[at], what));
-      return channel_vector(given.back(), o, x, what);
-    };
-    const Tensor w_post = vector_arg(3, "post.weight"), b_post = vector_arg(4, "post.bias");
-    const Tensor w_pre = vector_arg(5, "pre.weight"), b_pre = vector_arg(6, "pre.bias");
+    auto vector_arg = [&](int at) { return channel_vector(given[at], o, x, names[at]); };
+    const Tensor w_post = vector_arg(3), b_post = vector_arg(4), w_pre = vector_arg(5), b_pre = vector_arg(6);
     if (PyErr_Occurred()) return nullptr;
     const variable_list inputs = {x, f, gate, w_post, b_post, w_pre, b_pre};
     bool grad = false;
@@ -452,6 +476,7 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     if (nargs != 6) refuse(PyExc_TypeError, "gather takes 6 arguments");
     if (!PyList_Check(a[0]) || (a[1] != Py_None && !PyList_Check(a[1]))) refuse(PyExc_TypeError, "lists expected");
+    need_untraced("AdamW.step");
     const Py_ssize_t n = PyList_GET_SIZE(a[0]);
     const bool given = a[1] != Py_None;
     if (given && PyList_GET_SIZE(a[1]) != n) refuse(PyExc_ValueError, PyList_GET_SIZE(a[1]), " gradients for ", n, " parameters");

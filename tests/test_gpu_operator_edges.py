@@ -148,3 +148,22 @@ def test_tensors_without_memory():
     p.untyped_storage().resize_(0)
     with pytest.raises(ValueError, match="freed"):
         opt.step([w])
+
+
+def test_a_traced_backward_pass_is_refused_and_other_modes_are_not():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    x = torch.randn(2, 40, 9, device=DEV, requires_grad=True)
+    spec = R().NormSpec("rms", torch.ones(40, device=DEV))
+    h = R().channel_norm(x, spec)
+    dh = torch.randn_like(h)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda d: torch.autograd.grad(h, x, d, retain_graph=True)[0])(dh)
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        torch.autograd.grad(h, x, fw.make_dual(dh, dh), retain_graph=True)
+    want, = torch.autograd.grad(h, x, dh, retain_graph=True)
+    with FlopCounterMode(display=False):
+        again = R().channel_norm(x, spec)
+        got, = torch.autograd.grad(again, x, dh)
+    assert torch.equal(again, h) and torch.equal(got, want)
