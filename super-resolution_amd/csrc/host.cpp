@@ -20,8 +20,6 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/custom_class.h>
-#include <mutex>
-#include <unordered_map>
 #include "srx.h"
 
 namespace {
@@ -174,21 +172,10 @@ Tensor fresh(const Order& o, const Tensor& like) {
 }
 
 // ------------------------------------------------------------------------------------------------ the operator
-// Calls recorded outside of a capture whose graphs still live: their leaves, and the stream they were recorded on.  (Never
-// destroyed: a graph may outlive this module's statics.)
-struct Call;
-std::mutex& eager_lock = *new std::mutex;
-auto& eager = *new std::unordered_map<const Call*, std::pair<std::vector<const void*>, const void*>>;
-
 struct Call : torch::CustomClassHolder {
   srx_resnorm_desc d;       // kinds, sizes, layout, gate
   Order order;
-  bool branch, noted = false;
-  ~Call() override {
-    if (!noted) return;
-    const std::lock_guard<std::mutex> g(eager_lock);
-    eager.erase(this);
-  }
+  bool branch;
 };
 
 const void* address(const Tensor& t) {
@@ -339,28 +326,20 @@ Tensor channel_vector(const Tensor& t, const Order& o, const Tensor& x, const ch
   return in_memory(t).to(at::kFloat).contiguous();
 }
 
-// Autograd keeps one accumulator per leaf for as long as any graph of that leaf lives, bound to the stream it was first used
-// on.  A backward pass captured on another stream would then make the capture wait for that stream, and ROCm's runtime ends
-// the process when such a capture closes.  So the forward call is refused instead.
-void note_graph(Call& c, const variable_list& inputs, const c10::Device& dev) {
-  std::vector<const void*> leaves;
-  for (const Tensor& t : inputs)
-    if (t.defined() && t.requires_grad() && t.is_leaf()) leaves.push_back(t.unsafeGetTensorImpl());
-  if (leaves.empty()) return;
-  const void* stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).stream();
-  const std::lock_guard<std::mutex> g(eager_lock);
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) {
-    eager[&c] = {std::move(leaves), stream};
-    c.noted = true;
-    return;
+// Autograd keeps one accumulator per leaf for as long as any graph of that leaf lives, whoever recorded it, bound to the stream
+// that the first of them was recorded on.  A backward pass captured on another stream would then make the capture wait for that
+// stream, and ROCm's runtime ends the process when such a capture closes.  So the forward call is refused instead.
+void need_own_accumulators(const variable_list& inputs, const c10::Device& dev) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const c10::Stream stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(dev.index()).unwrap();
+  for (const Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (accumulator && accumulator->stream() != stream)
+      refuse(PyExc_RuntimeError,
+             "a graph that was recorded before this capture, on another stream, still holds one of these leaves (an output of an "
+             "earlier call is alive): delete it, or capture on the stream that it was recorded on");
   }
-  for (const auto& e : eager)
-    if (e.second.second != stream)
-      for (const void* p : e.second.first)
-        if (std::find(leaves.begin(), leaves.end(), p) != leaves.end())
-          refuse(PyExc_RuntimeError,
-                 "a graph that was recorded before this capture, on another stream, still holds one of these leaves (an output of an "
-                 "earlier call is alive): delete it, or capture on the stream that it was recorded on");
 }
 
 Tensor tensor_arg(PyObject* o, const char* what) {
@@ -435,7 +414,7 @@ PyObject* resnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     variable_list out;
     const c10::OptionalDeviceGuard guard(x.device());
     if (grad) {
-      note_graph(*c, given, x.device());
+      need_own_accumulators(given, x.device());
       auto opt = [](const Tensor& t) -> Opt { return t.defined() ? Opt(t) : std::nullopt; };
       out = ResNorm::apply(c, opt(x), opt(f), opt(gate), opt(w_post), opt(b_post), opt(w_pre), opt(b_pre));
     } else {

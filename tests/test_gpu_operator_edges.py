@@ -167,3 +167,44 @@ def test_a_traced_backward_pass_is_refused_and_other_modes_are_not():
         again = R().channel_norm(x, spec)
         got, = torch.autograd.grad(again, x, dh)
     assert torch.equal(again, h) and torch.equal(got, want)
+
+
+def test_any_living_graph_of_a_leaf_on_another_stream_refuses_the_capture():
+    """Autograd's accumulator of a leaf is bound to the stream of the leaf's oldest graph, not to that of each graph."""
+    x = torch.randn(2, 64, 9, device=DEV)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    call = lambda: R().channel_norm(x, R().NormSpec("rms", w))  # noqa: E731
+    side = torch.cuda.Stream()
+
+    def captured(stream, backward):
+        graph = torch.cuda.CUDAGraph()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=stream):
+            z = x * 2
+            if not backward:
+                with pytest.raises(RuntimeError, match="recorded before this capture"):
+                    call()
+                return graph, z
+            h = call()
+            g, = torch.autograd.grad(h, w, torch.ones_like(h))
+            return graph, h.detach(), g
+    alive = w * 2                       # a graph of other operations
+    captured(side, False)
+    first = alive
+    with torch.cuda.stream(side):       # a second one, on the stream of the capture, does not move the accumulator
+        alive = call()
+    del first
+    captured(side, False)
+    torch.cuda.synchronize()
+    del alive
+    with torch.cuda.stream(side):       # the same stream: nothing to wait for
+        alive = call()
+    torch.cuda.synchronize()
+    graph, h, g = captured(side, True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(h, alive)
+    del alive
+    want = call()
+    assert torch.equal(g, torch.autograd.grad(want, w, torch.ones_like(want))[0])
