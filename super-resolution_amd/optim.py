@@ -58,8 +58,9 @@ class AdamW:
     skip_nonfinite: a step whose gradient norm is infinite or NaN changes nothing.
 
     ``param_groups`` holds the hyper-parameters under torch's names and is read at every step; ``lr`` sets them all.
-    A captured step replays with the hyper-parameters and ``grad_scale`` it was captured with; its step count
-    advances.  One optimizer's steps share its state and workspaces: they must not overlap.  To autograd a step is an
+    A captured step replays with the hyper-parameters and ``grad_scale`` it was captured with, and reads its gradients
+    where they were then; its step count advances.  Where parameters have got new storage since, one eager step
+    makes it follow them.  One optimizer's steps share its state and workspaces: they must not overlap.  To autograd a step is an
     in-place change of every parameter that it moves: a graph that saved one of them refuses its backward pass."""
 
     def __init__(self, params: Iterable, lr: float = 2e-4, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -207,9 +208,12 @@ class AdamW:
                 t.g_off = (ptrs[i] - base) // esize if self._flat and self._n[i] else 0
                 i += 1
         raw = torch.frombuffer(bytearray(C.string_at(C.addressof(arr), C.sizeof(arr))), dtype=torch.uint8)
-        if self._tensors is not None:
-            torch.cuda.synchronize(self.device)      # steps in flight still read the old table
-        self._tensors = raw.to(self.device)
+        if self._tensors is None:
+            self._tensors = raw.to(self.device)
+        else:
+            # in place: a captured step holds the table's address, and follows the parameters too
+            torch.cuda.synchronize(self.device)      # steps in flight still read the old entries
+            self._tensors.copy_(raw)
         self._bound = np.array(ptrs + [2 * n + (t == torch.bfloat16) for n, t in zip(self._n, self._dtypes)], dtype=np.uint64)
 
     def _copy_masters(self) -> None:

@@ -208,3 +208,33 @@ def test_any_living_graph_of_a_leaf_on_another_stream_refuses_the_capture():
     del alive
     want = call()
     assert torch.equal(g, torch.autograd.grad(want, w, torch.ones_like(want))[0])
+
+
+@pytest.mark.parametrize("sizes,clip", [([300, 5000, 7], None), ([300, 70000, 64] * 200, 1.0)])
+def test_a_captured_step_follows_parameters_to_new_storage(sizes, clip):
+    """The table of addresses that a captured step reads is the optimizer's for good: binding again writes it in place."""
+    g = torch.Generator().manual_seed(1)
+    start = [torch.randn(n, generator=g).to(DEV) for n in sizes]
+    grads = [torch.randn(n, generator=g).to(DEV) for n in sizes]
+    ps, qs = ([torch.nn.Parameter(t.clone()) for t in start] for _ in range(2))
+    opt, ref = (pkg("optim").AdamW(x, lr=1e-2, state_bits=8, max_grad_norm=clip) for x in (ps, qs))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(grads)
+    graph.replay()
+    ref.step(grads)
+    torch.cuda.synchronize()
+    table, old = opt._tensors.data_ptr(), [p.data for p in ps]
+    for p in ps:
+        p.data = p.data.clone()
+    opt.step(grads)
+    ref.step(grads)
+    kept = [t.clone() for t in old]
+    fill = [torch.full((len(opt._tensors),), 255, dtype=torch.uint8, device=DEV) for _ in range(8)]      # into memory that was given back, if any was
+    for _ in range(3):
+        graph.replay()
+        ref.step(grads)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ps, qs))
+    assert opt._tensors.data_ptr() == table and len(fill) == 8
+    assert all(torch.equal(a, b) for a, b in zip(old, kept)) and opt.step_counts == ref.step_counts == [5] * len(sizes)
