@@ -460,7 +460,8 @@ int srx_resnorm_forward(const srx_resnorm_desc* d, void* stream);
  *     D = dy + N_pre'(y)^T dh,  dx = D,  df = N_post'(f)^T (scale act(gate) D),  dgate = scale act'(gate) sum D a,
  *     dw_pre = sum dh n_y, db_pre = sum dh, dw_post = sum scale act(gate) D n_f, db_post = sum scale act(gate) D. */
 int srx_resnorm_backward(const srx_resnorm_desc* d, void* stream);
-/* Floats of workspace for the backward pass of d (addresses and strides are not looked at); -1: d is refused. */
+/* Floats of workspace for the backward pass of d; -1: d is refused.  Goes by dtype, layout, sizes, kinds and gate_mode alone: tensors,
+ * weights and strides are not looked at and may be set later. */
 int64_t srx_resnorm_ws_floats(const srx_resnorm_desc* d);
 
 /* -------------------------------------------------------- tiled inference */

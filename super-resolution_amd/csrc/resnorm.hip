@@ -207,18 +207,27 @@ void make_plan(const srx_resnorm_desc& d, int backward, bool gen, Plan& p) {
   p.lds_bytes = bytes;
 }
 
-int check(const char* what, const srx_resnorm_desc* d) {
+// what a call computes: types, sizes, kinds
+int check_form(const char* what, const srx_resnorm_desc* d) {
   SRX_CHECK_ARG(d != nullptr, "%s: null descriptor", what);
   SRX_CHECK_ARG(d->dtype == SRX_BF16 || d->dtype == SRX_F32, "%s: bad dtype %d", what, d->dtype);
   SRX_CHECK_ARG(d->layout == SRX_RESNORM_PLANES || d->layout == SRX_RESNORM_ROWS, "%s: bad layout %d", what, d->layout);
   SRX_CHECK_ARG(d->B >= 0 && d->P >= 0 && d->C > 0, "%s: bad sizes B %d C %d P %d", what, d->B, d->C, d->P);
-  const bool by_image = (d->layout == SRX_RESNORM_PLANES && d->P > 1) || (d->f && d->gate_mode == GATE_IMAGE);
+  const bool by_image = (d->layout == SRX_RESNORM_PLANES && d->P > 1) || d->gate_mode == GATE_IMAGE;
   SRX_CHECK_ARG(!by_image || d->B <= (1 << 30), "%s: %d images, at most 2^30", what, d->B);
   const int most = d->layout == SRX_RESNORM_ROWS ? MAX_ROWS_C : MAX_PLANES_C;
   SRX_CHECK_ARG(d->C <= most, "%s: %d channels, at most %d in this layout", what, d->C, most);
   SRX_CHECK_ARG(d->post_kind >= 0 && d->post_kind <= 2 && d->pre_kind >= 0 && d->pre_kind <= 2, "%s: bad norm kind", what);
   SRX_CHECK_ARG(d->gate_mode >= 0 && d->gate_mode <= 3 && (d->gate_act == 0 || d->gate_act == 1), "%s: bad gate mode", what);
   SRX_CHECK_ARG((!d->post_kind || d->post_eps >= FLT_MIN) && (!d->pre_kind || d->pre_eps >= FLT_MIN), "%s: eps must be positive (a normal number)", what);
+  // beyond 64 channels a workgroup's lanes address their channels with 32 bits
+  SRX_CHECK_ARG(d->layout == SRX_RESNORM_ROWS || d->C <= 64 || (int64_t)d->C * d->P * (d->dtype == SRX_BF16 ? 2 : 4) < (1LL << 32),
+                "%s: an image of more than 64 channels must stay under 4 GB", what);
+  return SRX_OK;
+}
+// and what it computes on
+int check(const char* what, const srx_resnorm_desc* d) {
+  if (int rc = check_form(what, d)) return rc;
   SRX_CHECK_ARG(d->f || (!d->post_kind && !d->gate_mode), "%s: a norm after the branch or a gate without a branch", what);
   SRX_CHECK_ARG(d->f || d->pre_kind, "%s: neither a branch nor a norm", what);
   SRX_CHECK_ARG(!d->gate_mode || d->gate, "%s: null gate", what);
@@ -235,8 +244,6 @@ int check(const char* what, const srx_resnorm_desc* d) {
       SRX_CHECK_ARG(strides[i] >= 0 && (strides[i] >= least || (i < 2 || i == 4 || i == 5 || i == 8)),
                     "%s: tensor %d: stride %lld of an output is under %lld", what, i, (long long)strides[i], (long long)least);
     }
-  // beyond 64 channels a workgroup's lanes address their channels with 32 bits
-  SRX_CHECK_ARG(rows || d->C <= 64 || (int64_t)d->C * d->P * esize < (1LL << 32), "%s: an image of more than 64 channels must stay under 4 GB", what);
   return SRX_OK;
 }
 
@@ -245,13 +252,15 @@ int check(const char* what, const srx_resnorm_desc* d) {
 extern "C" {
 
 int64_t srx_resnorm_ws_floats(const srx_resnorm_desc* d) {
-  if (check("srx_resnorm_ws_floats", d)) return -1;
-  // enough for either form: addresses decide between them
+  if (check_form("srx_resnorm_ws_floats", d)) return -1;
+  // enough for either form: addresses decide between them, and may not be there yet
+  srx_resnorm_desc asked = *d;
+  if (d->gate_mode) asked.f = &asked;                     // a gate is on a branch
+  const bool image_gate = d->gate_mode == GATE_IMAGE;
   int64_t floats = 1;
   for (const bool gen : {false, true}) {
     Plan p = {};
-    make_plan(*d, 1, gen, p);
-    const bool image_gate = d->f && d->gate_mode == GATE_IMAGE;
+    make_plan(asked, 1, gen, p);
     const int64_t need = 2 * (int64_t)d->C * (p.workgroups + (image_gate ? p.a.items + join_groups(p.images) : p.workgroups)) + 1;
     if (need > floats) floats = need;
   }

@@ -57,3 +57,24 @@ def test_a_traced_step_is_refused():
         with pytest.raises(RuntimeError, match="AdamW.step cannot be traced"):
             trace()
     lists(torch.ones(4))
+
+
+def test_workspace_is_asked_for_before_there_are_tensors():
+    """The size for a descriptor of types, sizes and kinds alone is the size for the same call with its tensors, and sizes are still refused."""
+    L = pkg("_lib")
+    lib = L.lib()
+    names = ("x", "f", "y", "h", "dy", "dh", "dx", "df", "gate", "dgate")
+    for layout in (0, 1):
+        for c, b, p in ((1, 1, 64), (24, 300, 1000), (64, 16, 4096), (300, 3, 1), (1000, 2, 4000), (64, 1, 1)):
+            for gate_mode in (0, 1, 2, 3):
+                for post, pre in ((1, 2), (2, 0), (0, 1), (0, 0)):
+                    form = dict(dtype=0, layout=layout, C=c, B=b, P=p, gate_mode=gate_mode, post_kind=post, pre_kind=pre, post_eps=1e-6, pre_eps=1e-6)
+                    bare = lib.srx_resnorm_ws_floats(C.byref(L.ResnormDesc(**form)))
+                    there = {n: 256 for n in names}
+                    full = lib.srx_resnorm_ws_floats(C.byref(L.ResnormDesc(**form, **there, **{n + "_stride": 1 << 62 for n in names}, b_post=256, db_pre=256)))
+                    assert bare == full > 0, (form, lib.srx_last_error())
+                    # an address without its stride, and one that a tensor could not have
+                    assert lib.srx_resnorm_ws_floats(C.byref(L.ResnormDesc(**form, x=257, f=3, dx=256))) == bare
+    for bad in (dict(C=0), dict(B=-1), dict(gate_mode=7), dict(pre_kind=1, pre_eps=0.0), dict(dtype=9), dict(layout=0, C=65, P=1 << 25),
+                dict(gate_mode=2, B=(1 << 30) + 1)):
+        assert lib.srx_resnorm_ws_floats(C.byref(L.ResnormDesc(**{**dict(dtype=0, layout=1, C=8, B=2, P=3), **bad}))) == -1, bad
