@@ -164,8 +164,8 @@ class AdamW:
         for g in self.param_groups:
             g["lr"] = value
 
-    def _check_hyper(self) -> None:
-        for i, g in enumerate(self.param_groups):
+    def _check_hyper(self, groups: Optional[List[dict]] = None) -> None:
+        for i, g in enumerate(self.param_groups if groups is None else groups):
             b = g["betas"]
             if not (0 <= g["lr"] < math.inf and len(b) == 2 and 0 <= b[0] < 1 and 0 <= b[1] < 1 and 0 <= g["eps"] < math.inf
                     and 0 <= g["weight_decay"] < math.inf):
@@ -315,8 +315,8 @@ class AdamW:
         """Set the whole state: moments as :meth:`moments` returns them, step counts (one, or one per parameter), and the
         masters of the bf16 parameters (None: taken from the parameters)."""
         steps = [int(step)] * len(self.params) if isinstance(step, int) else [int(k) for k in step]
-        if len(steps) != len(self.params) or min(steps) < 0:
-            raise ValueError("step: one count that is not negative, or one per parameter")
+        if len(steps) != len(self.params) or not 0 <= min(steps) <= max(steps) < 2 ** 31:
+            raise ValueError("step: one count from 0 to 2^31 - 1, or one per parameter")
         for name, t, n in (("m", m, self._m.numel()), ("v", v, self._v.numel())) + \
                 ((("master", master, self._master_at[-1]),) if master is not None else ()):
             if t.numel() != n or t.dtype != torch.float32 or t.device != self.device:
@@ -366,7 +366,7 @@ class AdamW:
 
     def load_state_dict(self, sd: dict) -> None:
         """Accepts a state_dict written by this class (any ``state_bits``) or by ``torch.optim.AdamW`` over the same parameters
-        in the same groups."""
+        in the same groups.  One that is refused changes nothing."""
         groups = sd["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError(f"optimizer state_dict does not match: groups of {[len(g['params']) for g in groups]} parameters, "
@@ -392,10 +392,9 @@ class AdamW:
             v[at:at + n].copy_(st["exp_avg_sq"].reshape(-1))
             if "master" in st and self._dtypes[i] == torch.bfloat16:
                 master[self._master_at[i]:self._master_at[i + 1]].copy_(st["master"].reshape(-1))
-        for g, new in zip(self.param_groups, groups):
-            for key in ("lr", "eps", "weight_decay"):
-                g[key] = float(new[key])
-            g["betas"] = tuple(new["betas"])
-            g["initial_lr"] = new.get("initial_lr", g["initial_lr"])
-        self._check_hyper()
+        hyper = [{**{key: float(new[key]) for key in ("lr", "eps", "weight_decay")}, "betas": tuple(new["betas"]),
+                  "initial_lr": new.get("initial_lr", g["initial_lr"])} for g, new in zip(self.param_groups, groups)]
+        self._check_hyper(hyper)
         self.load_moments(m, v, steps, master)
+        for g, new in zip(self.param_groups, hyper):
+            g.update(new)

@@ -1,6 +1,8 @@
 """GPU: unusual calls of the residual norms and the AdamW step that the documentation allows, or that are refused: what autograd is
 told of a step, views with the negative bit, forward-mode differentiation and tracing, captures beside living graphs, parameters
 that move under a captured step, states that are refused, second moments below the normal numbers, 8-bit moments over thousands of steps."""
+import copy
+
 import pytest
 import torch
 
@@ -238,3 +240,32 @@ def test_a_captured_step_follows_parameters_to_new_storage(sizes, clip):
         assert all(torch.equal(a, b) for a, b in zip(ps, qs))
     assert opt._tensors.data_ptr() == table and len(fill) == 8
     assert all(torch.equal(a, b) for a, b in zip(old, kept)) and opt.step_counts == ref.step_counts == [5] * len(sizes)
+
+
+def test_a_refused_state_changes_nothing():
+    p = [torch.nn.Parameter(torch.randn(300, device=DEV)), torch.nn.Parameter(torch.randn(40, device=DEV).to(BF16))]
+    opt = pkg("optim").AdamW(p, lr=1e-3)
+    opt.step([torch.ones_like(t) for t in p])
+    good = opt.state_dict()
+    opt.step([torch.ones_like(t) for t in p])
+
+    def all_of_it():
+        return ([{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups], opt.step_counts,
+                [t.clone() for t in (*opt.moments(), opt.master)])
+    before = all_of_it()
+    for where, key, value, error in (("group", "lr", -1.0, ValueError), ("group", "betas", (0.9, 1.0), ValueError), ("group", "eps", None, (TypeError, ValueError)),
+                                     (0, "step", torch.tensor(-1.0), ValueError), (1, "step", torch.tensor(2.0 ** 31), ValueError),
+                                     (0, "exp_avg_sq", torch.zeros(1, device=DEV), ValueError), (1, "master", torch.zeros(1, device=DEV), ValueError)):
+        sd = copy.deepcopy(good)
+        (sd["param_groups"][0] if where == "group" else sd["state"][where])[key] = value
+        if key != "lr":
+            sd["param_groups"][0]["lr"] = 0.5
+        with pytest.raises(error):
+            opt.load_state_dict(sd)
+        after = all_of_it()
+        assert after[:2] == before[:2] and all(torch.equal(a, b) for a, b in zip(after[2], before[2])), (where, key)
+    with pytest.raises(ValueError, match="step"):
+        opt.load_moments(*(torch.ones_like(t) for t in opt.moments()), 2 ** 31)
+    assert all(torch.equal(a, b) for a, b in zip(all_of_it()[2], before[2]))
+    opt.load_state_dict(good)
+    assert opt.step_counts == [1, 1]
