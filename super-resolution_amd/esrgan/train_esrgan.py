@@ -84,8 +84,9 @@ def fit(gen, disc, vgg_loss, train_loader: Iterable, val_loader: Iterable, check
     """The body of the reference's ``main`` (:139-208) for modules that already sit on the GPU.
     ``train_loader`` / ``val_loader`` are re-iterated every epoch and yield ``(lr, hr)`` batches
     in [-1, 1]; ``batch_shape`` is the LR batch shape ``(B, 3, h, w)``; ``optimizer(module)``, if given, builds
-    the optimizers (default Adam with ``lr``; the epoch's learning rate is set on them either way).  Returns one dictionary
-    per finished adversarial epoch (losses, learning rate, validation numbers)."""
+    the optimizers (default Adam with ``lr``; the epoch's learning rate is set on them either way, groups of ``optim.AdamW``
+    with one of their own keeping their ratio).  Returns one dictionary per finished adversarial epoch (losses, learning
+    rate, validation numbers)."""
     if mode not in ("pretrain", "train", "all"):
         raise ValueError(f"mode must be pretrain, train or all (got {mode!r})")
     cdir = Path(checkpoint_dir)

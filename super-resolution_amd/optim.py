@@ -57,7 +57,8 @@ class AdamW:
     max_grad_norm: gradients are scaled by ``min(1, max_grad_norm / (norm + 1e-6))``, norm over all tensors.
     skip_nonfinite: a step whose gradient norm is infinite or NaN changes nothing.
 
-    ``param_groups`` holds the hyper-parameters under torch's names and is read at every step; ``lr`` sets them all.
+    ``param_groups`` holds the hyper-parameters under torch's names and is read at every step; ``lr`` sets one learning
+    rate for all, ``schedule_lr`` one that respects the groups' own.
     A captured step replays with the hyper-parameters and ``grad_scale`` it was captured with, and reads its gradients
     where they were then; its step count advances.  Where parameters have got new storage since, one eager step
     makes it follow them.  One optimizer's steps share its state and workspaces: they must not overlap.  To autograd a step is an
@@ -90,6 +91,7 @@ class AdamW:
             group["betas"] = tuple(group["betas"])
             group.setdefault("initial_lr", group["lr"])
             self.param_groups.append(group)
+        self._lr_ratio = [g["lr"] / lr if lr > 0 else 1.0 for g in self.param_groups]
         self.params: List[torch.Tensor] = [p for g in self.param_groups for p in g["params"]]
         if not self.params:
             raise ValueError("no parameters")
@@ -163,6 +165,11 @@ class AdamW:
     def lr(self, value: float) -> None:
         for g in self.param_groups:
             g["lr"] = value
+
+    def schedule_lr(self, value: float) -> None:
+        """The learning rate of a schedule: a group that was given one of its own keeps its ratio to the constructor's ``lr``."""
+        for g, ratio in zip(self.param_groups, self._lr_ratio):
+            g["lr"] = value * ratio
 
     def _check_hyper(self, groups: Optional[List[dict]] = None) -> None:
         for i, g in enumerate(self.param_groups if groups is None else groups):

@@ -162,7 +162,7 @@ def _make_optimizer(optimizer: Optional[Callable], module, flat: torch.Tensor, l
     """The optimizer of a trainer: ``optimizer(module)`` — for instance ``lambda m: optim.AdamW(optim.decay_groups(m),
     lr=2e-4, max_grad_norm=1.0, state_bits=8)`` — or FlatAdam.  It is built after the module's parameters
     have become views of one flat buffer and before the first step, its ``step`` gets the flat gradient, and
-    ``lr`` and ``state_dict`` / ``load_state_dict`` are used as FlatAdam's are."""
+    ``lr`` (``schedule_lr`` where it has one) and ``state_dict`` / ``load_state_dict`` are used as FlatAdam's are."""
     if optimizer is None:
         return FlatAdam(flat, lr=lr, shapes=[p.shape for p in module.parameters()])
     opt = optimizer(module)
@@ -363,8 +363,11 @@ class AdversarialTrainer:
     overlap_real_pass = True
 
     def set_lr(self, lr: float) -> None:
-        self.opt_g.lr = lr
-        self.opt_d.lr = lr
+        for opt in (self.opt_g, self.opt_d):
+            if hasattr(opt, "schedule_lr"):         # groups with learning rates of their own
+                opt.schedule_lr(lr)
+            else:
+                opt.lr = lr
 
     def _acc_ptr(self, i: int) -> int:
         return self.acc.data_ptr() + 4 * i

@@ -269,3 +269,29 @@ def test_a_refused_state_changes_nothing():
     assert all(torch.equal(a, b) for a, b in zip(all_of_it()[2], before[2]))
     opt.load_state_dict(good)
     assert opt.step_counts == [1, 1]
+
+
+def test_a_schedule_keeps_the_groups_learning_rates_apart():
+    """The trainers' epoch schedule through an optimizer whose groups differ, and through one whose groups do not."""
+    OPT, T = pkg("optim"), pkg("train")
+    gen = pkg("esrgan.generator").GeneratorESRGAN(num_blocks=1).to(DEV)
+    disc = pkg("esrgan.discriminator").Discriminator().to(DEV)
+    with pytest.warns(UserWarning):
+        vgg = pkg("utils.loss").VGGLoss(device=DEV, allow_synthetic=True)
+
+    def mk(module):
+        groups = OPT.decay_groups(module, 0.1)
+        if module is gen:
+            groups[1]["lr"] = 5e-4
+        return OPT.AdamW(groups, lr=1e-3)
+    tr = T.AdversarialTrainer(gen, disc, vgg, (2, 3, 16, 16), optimizer=mk)
+    lrs = lambda opt: [g["lr"] for g in opt.param_groups]  # noqa: E731
+    for epoch in range(3):
+        lr = T.cosine_lr(1e-3, epoch, t_max=3, eta_min=1e-7)
+        tr.set_lr(lr)
+        assert lrs(tr.opt_g) == [lr, lr * 0.5] and lrs(tr.opt_d) == [lr, lr]
+    tr.opt_g.lr = 3e-4                  # for all, as documented
+    assert lrs(tr.opt_g) == [3e-4, 3e-4]
+    plain = T.AdversarialTrainer(gen, disc, vgg, (2, 3, 16, 16))
+    plain.set_lr(1e-5)
+    assert plain.opt_g.lr == plain.opt_d.lr == 1e-5
