@@ -311,7 +311,8 @@ __device__ __forceinline__ void moments(float& m, float& v, float g, const Coef&
   v = v + vg;
 }
 // The hardware's square root and reciprocal are within 2^-23 of the value: 2^-21 of the update at most, which is itself
-// far below the parameter.  They take a denormal for zero, so an eps that does not cover such a root gets the exact forms.
+// far below the parameter.  The root takes a denormal for zero: 2^-63 root of the denominator, below 2^-21 of it where eps is at
+// least 2^-42 root (2.3e-13, 7.2e-12 at a first step with beta2 = 0.999); a smaller eps gets the exact forms.
 __device__ __forceinline__ float updated(float w, float m, float v, const Coef& c, bool fast) {
   const float u = fast ? m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * c.root + c.eps) : m / (sqrtf(v) * c.root + c.eps);
   return w * c.decay - c.step_size * u;
@@ -368,7 +369,7 @@ template <int BITS, int NG, bool SMALL> __device__ __forceinline__ void update_c
     factor = ctl->factor;
     c = reinterpret_cast<const Coef*>(a.coef + 4)[ch.tensor];
   }
-  const bool fast = c.eps >= 1e-15f;
+  const bool fast = c.eps >= 0x1p-42f * c.root;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int NB = CHUNK / BLOCK / (TPB / 64);
   const int64_t lo = (int64_t)ch.index * CHUNK + wave * NB * BLOCK;        // the wave's first element in its tensor

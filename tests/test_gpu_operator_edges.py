@@ -295,3 +295,18 @@ def test_a_schedule_keeps_the_groups_learning_rates_apart():
     plain = T.AdversarialTrainer(gen, disc, vgg, (2, 3, 16, 16))
     plain.set_lr(1e-5)
     assert plain.opt_g.lr == plain.opt_d.lr == 1e-5
+
+
+@pytest.mark.parametrize("eps", [1e-15, 1e-14, 1e-13, 1e-12, 1e-8])
+def test_second_moments_below_the_smallest_normal_number(eps):
+    """v = (1 - beta2) g^2 = 9e-39 at a first step: its root, 3e-18 with the bias correction, still counts beside eps = 1e-15."""
+    p = torch.nn.Parameter(torch.zeros(600, device=DEV))
+    g = torch.full((600,), 3e-18)
+    opt = pkg("optim").AdamW([p], lr=1.0, weight_decay=0.0, eps=eps)
+    opt.step([g.to(DEV)])
+    g = float(g[0].double())
+    want = -g / (g + eps)
+    # v is a multiple of 2^-149 within half: 2^-150 / 9e-39 = 2^-23.6 of itself, and 12 more roundings of 2^-24 of the operations, or 2^-21 of
+    # the update from the hardware's root and reciprocal
+    off = float((p.detach().double() / want - 1).abs().max())
+    assert off <= 2.0 ** -21 + 16 * 2.0 ** -24
