@@ -633,6 +633,7 @@ int srx_adamw_step(const srx_adamw_desc* d, void* stream) {
   SRX_CHECK_ARG(d->tensors && d->chunks && d->chunk_start && d->groups && d->steps && d->coef, "srx_adamw_step: null table");
   SRX_CHECK_ARG((d->grads != nullptr) != (d->flat_grad != nullptr), "srx_adamw_step: give either grads or flat_grad");
   SRX_CHECK_ARG(!d->flat_grad || d->flat_dtype == SRX_BF16 || d->flat_dtype == SRX_F32, "srx_adamw_step: bad flat_dtype %d", d->flat_dtype);
+  SRX_CHECK_ARG((uintptr_t)d->flat_grad % (d->flat_dtype == SRX_BF16 ? 2 : 4) == 0, "srx_adamw_step: flat_grad is not aligned to its type");
   SRX_CHECK_ARG(d->m && d->v && (d->state_bits == 32 || (d->m_scale && d->v_scale)), "srx_adamw_step: null moments");
   SRX_CHECK_ARG(((uintptr_t)d->m | (uintptr_t)d->v) % 16 == 0, "srx_adamw_step: moments must be 16-byte aligned");
   SRX_CHECK_ARG(!(d->max_norm < 0) && d->max_norm == d->max_norm, "srx_adamw_step: max_norm must not be negative or NaN");

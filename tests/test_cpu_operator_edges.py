@@ -78,3 +78,13 @@ def test_workspace_is_asked_for_before_there_are_tensors():
     for bad in (dict(C=0), dict(B=-1), dict(gate_mode=7), dict(pre_kind=1, pre_eps=0.0), dict(dtype=9), dict(layout=0, C=65, P=1 << 25),
                 dict(gate_mode=2, B=(1 << 30) + 1)):
         assert lib.srx_resnorm_ws_floats(C.byref(L.ResnormDesc(**{**dict(dtype=0, layout=1, C=8, B=2, P=3), **bad}))) == -1, bad
+
+
+def test_a_flat_gradient_off_its_alignment_is_refused():
+    L = pkg("_lib")
+    start = (C.c_int32 * 2)(0, 1)
+    groups = (L.AdamwGroup * 1)(L.AdamwGroup(1e-3, 0.9, 0.999, 1e-8, 0.01))
+    for dtype, address in ((L.F32, 66), (L.F32, 65), (L.BF16, 65)):
+        d = L.AdamwDesc(state_bits=32, ntensors=1, ngroups=1, chunk_start=C.addressof(start), groups=C.addressof(groups), flat_grad=address,
+                        flat_dtype=dtype, tensors=256, chunks=256, steps=256, coef=256, m=256, v=256, grad_scale=1.0)
+        assert L.lib().srx_adamw_step(C.byref(d), None) == 1 and b"flat_grad is not aligned" in L.lib().srx_last_error()
