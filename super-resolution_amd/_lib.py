@@ -120,7 +120,7 @@ class AdamwGroup(C.Structure):
 class AdamwDesc(C.Structure):
     _fields_ = [("state_bits", i32), ("ntensors", i32), ("ngroups", i32), ("skip_nonfinite", i32),
                 ("tensors", vp), ("chunks", vp), ("chunk_start", vp), ("groups", vp), ("grads", vp),
-                ("grad_dtypes", vp), ("flat_grad", vp), ("flat_dtype", i32), ("pad_", i32),
+                ("grad_dtypes", vp), ("flat_grad", vp), ("flat_dtype", i32), ("rounding", i32),
                 ("m", vp), ("v", vp), ("m_scale", vp), ("v_scale", vp), ("steps", vp), ("coef", vp),
                 ("partial", vp), ("norm", vp), ("grad_scale", f64), ("max_norm", f64)]
 

@@ -53,7 +53,6 @@ struct PrepArgs {
 
 // What the small form adds: the groups' constants, and who moves the step counts.
 struct SmallArgs {
-  int32_t* steps;
   int* arrived;
   double grad_scale;
   int ntensors;              // of this launch
@@ -69,6 +68,7 @@ template <int NG, bool SMALL = false> struct StepArgs {
   double* partial;
   void* m; void* v;
   float* m_scale; float* v_scale;
+  int32_t* steps;            // step counts: moved by the prepare launch, or by the small form itself
   const void* flat;          // NG == FLAT: the flat gradient
   uint64_t* table;           // addresses in device memory, bit 0 set for bf16 (NG == TABLE: read; else written, if there)
   int chunk0, t0;
@@ -351,9 +351,39 @@ template <bool SIGNED> __device__ __forceinline__ uint32_t encode4(const float* 
   return out;
 }
 
+// 32 bits that depend on every bit of a quad of elements (its number in the whole state), a step count and a salt: rounds of
+// a shift, an exclusive or and a product, with the odd numbers at 2^32 times the fractional parts of the roots of 3, 5 and 7.
+__device__ __forceinline__ uint32_t random_word(int64_t quad, uint32_t step, uint32_t salt) {
+  uint32_t h = (uint32_t)quad ^ ((uint32_t)(quad >> 32) * 0xA54FF53Bu) ^ ((4 * step + salt) * 0xBB67AE85u);
+  h = (h ^ (h >> 16)) * 0x3C6EF373u;
+  h = (h ^ (h >> 15)) * 0xBB67AE85u;
+  h = (h ^ (h >> 16)) * 0xA54FF53Bu;
+  return h ^ (h >> 15);
+}
+// Codes of four values, rounded up or down at random with the mean that the value has: 16 random bits, in the middle of the 20
+// that a code drops, are added to the correctly rounded quotient before they go.  Between two codes a float's bits are
+// linear in its value, and no quotient is above 1, so nothing carries past the last code.
+template <bool SIGNED> __device__ __forceinline__ uint32_t encode4_random(const float* x, float s, int64_t quad, uint32_t step) {
+  constexpr unsigned base = SIGNED ? M_BASE : V_BASE;
+  constexpr float smallest = SIGNED ? 1.25f * 0x1p-16f : 1.25f * 0x1p-32f;
+  const uint32_t r[2] = {random_word(quad, step, SIGNED ? 0 : 2), random_word(quad, step, SIGNED ? 1 : 3)};
+  uint32_t out = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float t = fabsf(x[j]) / s;
+    const uint32_t add = ((r[j / 2] >> (16 * (j & 1))) & 0xFFFFu) << 4 | 8u;
+    unsigned c = ((__float_as_uint(t) + add) >> 20) - base;
+    if (t < smallest) c = !SIGNED || (float)add < t * (0x1p20f / smallest);
+    if (!(t > 0.f)) c = 0;
+    if (SIGNED) c |= c && x[j] < 0 ? 128u : 0u;
+    out |= c << (8 * j);
+  }
+  return out;
+}
+
 // A wave takes whole blocks of 256, four elements a lane, so that a block's largest is a wave's.  All of a wave's four
 // blocks are read before the first is computed: a workgroup's only other wait is for the tables in front of them.
-template <int BITS, int NG, bool SMALL> __device__ __forceinline__ void update_chunk(const StepArgs<NG, SMALL>& a) {
+template <int BITS, int NG, bool SMALL, bool RANDOM> __device__ __forceinline__ void update_chunk(const StepArgs<NG, SMALL>& a) {
   const Ctl* ctl = reinterpret_cast<const Ctl*>(a.coef);
   if (!SMALL && ctl->skip) return;
   const srx_adamw_chunk ch = a.chunks[a.chunk0 + blockIdx.x];
@@ -364,11 +394,12 @@ template <int BITS, int NG, bool SMALL> __device__ __forceinline__ void update_c
   float factor;
   if constexpr (SMALL) {
     factor = (float)a.small.grad_scale;
-    c = coef_of(a.small.groups[t.group], a.small.steps[ch.tensor] + 1);
+    c = coef_of(a.small.groups[t.group], a.steps[ch.tensor] + 1);
   } else {
     factor = ctl->factor;
     c = reinterpret_cast<const Coef*>(a.coef + 4)[ch.tensor];
   }
+  const uint32_t step = RANDOM ? (uint32_t)a.steps[ch.tensor] + SMALL : 0;       // of this step
   const bool fast = c.eps >= 0x1p-42f * c.root;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int NB = CHUNK / BLOCK / (TPB / 64);
@@ -440,8 +471,8 @@ template <int BITS, int NG, bool SMALL> __device__ __forceinline__ void update_c
       *reinterpret_cast<F4*>(static_cast<float*>(a.v) + s) = v[b];
     } else {
       const float nm = __uint_as_float(wave_max_u(mmax)), nv = __uint_as_float(wave_max_u(vmax));
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s) = encode4<true>(m[b].e, nm);
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s) = encode4<false>(v[b].e, nv);
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s) = RANDOM ? encode4_random<true>(m[b].e, nm, s / 4, step) : encode4<true>(m[b].e, nm);
+      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s) = RANDOM ? encode4_random<false>(v[b].e, nv, s / 4, step) : encode4<false>(v[b].e, nv);
       if (lane == 0) { a.m_scale[blk + b] = nm; a.v_scale[blk + b] = nv; }
     }
   }
@@ -449,8 +480,8 @@ template <int BITS, int NG, bool SMALL> __device__ __forceinline__ void update_c
 
 // The small form is a step in one launch: each workgroup computes its tensor's constants itself, and the last one to
 // arrive, after every other has read its step count, moves the counts and clears the counter for the next launch.
-template <int BITS, int NG, bool SMALL> __global__ __launch_bounds__(TPB) void adamw_step_kernel(const StepArgs<NG, SMALL> a) {
-  update_chunk<BITS>(a);
+template <int BITS, int NG, bool SMALL, bool RANDOM> __global__ __launch_bounds__(TPB) void adamw_step_kernel(const StepArgs<NG, SMALL> a) {
+  update_chunk<BITS, NG, SMALL, RANDOM>(a);
   if constexpr (SMALL) {
     __shared__ int last;
     __syncthreads();                                  // all waves of this workgroup have read their step count
@@ -463,7 +494,7 @@ template <int BITS, int NG, bool SMALL> __global__ __launch_bounds__(TPB) void a
     for (int k = threadIdx.x; k < a.small.ntensors; k += TPB) {
       bool has = true;
       if constexpr (NG != FLAT) has = a.g[k] != nullptr;
-      if (has) a.small.steps[a.t0 + k] += 1;
+      if (has) a.steps[a.t0 + k] += 1;
     }
   }
 }
@@ -547,7 +578,7 @@ struct Near {
 template <int NG, bool SMALL = false> StepArgs<NG, SMALL> step_args(const srx_adamw_desc* d, const Near& near, int t0, int t1) {
   StepArgs<NG, SMALL> a = {};
   a.tensors = d->tensors; a.chunks = d->chunks; a.coef = d->coef; a.partial = d->partial;
-  a.m = d->m; a.v = d->v; a.m_scale = d->m_scale; a.v_scale = d->v_scale;
+  a.m = d->m; a.v = d->v; a.m_scale = d->m_scale; a.v_scale = d->v_scale; a.steps = d->steps;
   a.flat = d->flat_grad; a.flat_dtype = d->flat_dtype; a.chunk0 = d->chunk_start[t0]; a.t0 = t0;
   if (NG == TABLE || (NG > 0 && d->ntensors > NG)) a.table = reinterpret_cast<uint64_t*>(d->coef + 4 + 8 * (int64_t)d->ntensors);
   if constexpr (NG == NEAR_GRADS) { a.near_base = near.base; a.near_shift = near.shift; }
@@ -573,14 +604,14 @@ template <int NG, typename F> int each_launch(const srx_adamw_desc* d, const Nea
 }
 
 template <int NG, bool SMALL> int launch_step(const srx_adamw_desc* d, const StepArgs<NG, SMALL>& a, int n, hipStream_t s) {
-  if (d->state_bits == 8) hipLaunchKernelGGL((adamw_step_kernel<8, NG, SMALL>), dim3(n), dim3(TPB), 0, s, a);
-  else hipLaunchKernelGGL((adamw_step_kernel<32, NG, SMALL>), dim3(n), dim3(TPB), 0, s, a);
+  if (d->state_bits == 32) hipLaunchKernelGGL((adamw_step_kernel<32, NG, SMALL, false>), dim3(n), dim3(TPB), 0, s, a);
+  else if (d->rounding) hipLaunchKernelGGL((adamw_step_kernel<8, NG, SMALL, true>), dim3(n), dim3(TPB), 0, s, a);
+  else hipLaunchKernelGGL((adamw_step_kernel<8, NG, SMALL, false>), dim3(n), dim3(TPB), 0, s, a);
   return srx_check_launch("adamw_step");
 }
 
 template <int NG> int small_launch(const srx_adamw_desc* d, hipStream_t s) {
   StepArgs<NG, true> a = step_args<NG, true>(d, {}, 0, d->ntensors);
-  a.small.steps = d->steps;
   a.small.arrived = &reinterpret_cast<Ctl*>(d->coef)->arrived;
   a.small.grad_scale = d->grad_scale;
   a.small.ntensors = d->ntensors;
@@ -627,6 +658,7 @@ extern "C" {
 int srx_adamw_step(const srx_adamw_desc* d, void* stream) {
   SRX_CHECK_ARG(d != nullptr, "srx_adamw_step: null descriptor");
   SRX_CHECK_ARG(d->state_bits == 32 || d->state_bits == 8, "srx_adamw_step: state_bits must be 32 or 8, got %d", d->state_bits);
+  SRX_CHECK_ARG(d->rounding == 0 || (d->rounding == 1 && d->state_bits == 8), "srx_adamw_step: rounding must be 0, or 1 with 8 bits, got %d", d->rounding);
   SRX_CHECK_ARG(d->ntensors > 0, "srx_adamw_step: ntensors must be positive");
   SRX_CHECK_ARG(d->ngroups > 0 && d->ngroups <= SRX_ADAMW_MAX_GROUPS, "srx_adamw_step: %d groups, 1 to %d are supported",
                 d->ngroups, SRX_ADAMW_MAX_GROUPS);

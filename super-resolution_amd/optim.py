@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import warnings
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -54,6 +55,10 @@ class AdamW:
         contiguous fp32 or bf16 tensors on one GPU.  A bf16 parameter gets an fp32 master copy; writing the
         parameter (loading a checkpoint, say) also moves its master.
     state_bits: 32, or 8: moments of one byte with a scale for every 256 elements of a tensor.
+    rounding: of 8-bit moments.  "random" keeps their averages (with the same bits for the same inputs): the choice for
+        training.  "nearest", the default, gives the nearest codes, but its second moments do not follow a slow average: with
+        beta2 = 0.999 a value's ratio to the largest of its 256 stays put until one gradient's square exceeds 30 to 60 times
+        it.  A warning says so where neither is given.
     max_grad_norm: gradients are scaled by ``min(1, max_grad_norm / (norm + 1e-6))``, norm over all tensors.
     skip_nonfinite: a step whose gradient norm is infinite or NaN changes nothing.
 
@@ -66,9 +71,13 @@ class AdamW:
 
     def __init__(self, params: Iterable, lr: float = 2e-4, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, max_grad_norm: Optional[float] = None,
-                 skip_nonfinite: bool = False):
+                 skip_nonfinite: bool = False, rounding: Optional[str] = None):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if rounding not in (None, "nearest", "random"):
+            raise ValueError(f"rounding must be 'nearest' or 'random', got {rounding!r}")
+        if rounding == "random" and state_bits == 32:
+            raise ValueError("rounding: 32-bit moments are not rounded")
         if max_grad_norm is not None and not 0 < max_grad_norm < math.inf:
             raise ValueError(f"max_grad_norm must be positive and finite, got {max_grad_norm}")
         params = list(params)
@@ -105,8 +114,12 @@ class AdamW:
             if p.dtype not in _DTYPE_ID:
                 raise ValueError(f"parameter {i} is {p.dtype}: float32 or bfloat16 are supported")
         self._check_hyper()
+        if state_bits == 8 and rounding is None:
+            warnings.warn("AdamW: 8-bit moments rounded to nearest do not follow their average over many steps; give rounding='random' for "
+                          "training (or 'nearest' for this rounding without a warning)", stacklevel=2)
         self.device = self.params[0].device
         self.state_bits, self.max_grad_norm, self.skip_nonfinite = state_bits, max_grad_norm, bool(skip_nonfinite)
+        self.rounding = rounding or "nearest"
         self._lib = L.lib()
         self._n = [p.numel() for p in self.params]
         self._shapes = [p.shape for p in self.params]
@@ -146,6 +159,7 @@ class AdamW:
             self._copy_masters()
             d = self._desc = L.AdamwDesc()
             d.state_bits, d.ntensors, d.ngroups = state_bits, len(self.params), len(self.param_groups)
+            d.rounding = rounding == "random"
             self._start = start
             d.chunks, d.chunk_start = self._chunks.data_ptr(), start.ctypes.data
             d.m, d.v = self._m.data_ptr() or self._steps.data_ptr(), self._v.data_ptr() or self._steps.data_ptr()
