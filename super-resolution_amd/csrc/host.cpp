@@ -449,8 +449,9 @@ struct Buffer {
 
 // gather(params, grads or None, bound, addresses, types, device index) -> flags.  Compares the parameters with bound[2 n]
 // (uint64: addresses, then elements times two, plus one for bf16), and writes the gradients' addresses (uint64[n], 0: none)
-// and types (uint8[n]).  GATHER_MOVED: a parameter's address, size or type differs, or it is not contiguous, a negative view or without its memory.
-// GATHER_ODD: a gradient cannot be taken as it is (shape, type, device, order, a negative view, no memory) and the caller has to look.  GATHER_BF16: some gradient is bf16.  grads None: each parameter's .grad.
+// and types (uint8[n]).  GATHER_MOVED: a parameter's address, size or type differs, or it is not contiguous or a negative view.
+// GATHER_ODD: a gradient cannot be taken as it is (shape, type, device, order, a negative view, no memory) and the caller has to look.
+// GATHER_BF16: some gradient is bf16.  grads None: each parameter's .grad.
 PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     if (nargs != 6) refuse(PyExc_TypeError, "gather takes 6 arguments");
@@ -465,21 +466,22 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     const auto* was = static_cast<const uint64_t*>(bound.b.buf);
     auto* to = static_cast<uint64_t*>(addresses.b.buf);
     auto* ty = static_cast<uint8_t*>(types.b.buf);
+    const Tensor none;
     long flags = 0;
     for (Py_ssize_t i = 0; i < n; ++i) {
       if (!THPVariable_Check(PyList_GET_ITEM(a[0], i))) refuse(PyExc_TypeError, "parameter ", i, " is not a tensor");
       const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(a[0], i));
       if (reinterpret_cast<uint64_t>(p.data_ptr()) != was[i] || 2 * (uint64_t)p.numel() + (p.scalar_type() == at::kBFloat16) != was[n + i] ||
-          !p.is_contiguous() || p.is_neg() || !held(p))
+          !p.is_contiguous() || p.is_neg())
         flags |= GATHER_MOVED;
       to[i] = 0;
       ty[i] = SRX_F32;
       PyObject* go = given ? PyList_GET_ITEM(a[1], i) : nullptr;
       if (given && go != Py_None && !THPVariable_Check(go)) refuse(PyExc_TypeError, "gradient ", i, " is a ", Py_TYPE(go)->tp_name, ", not a tensor");
-      const Tensor& g = given ? (go == Py_None ? Tensor() : THPVariable_Unpack(go)) : p.grad();
+      const Tensor& g = !given ? p.grad() : go == Py_None ? none : THPVariable_Unpack(go);
       if (!g.defined()) continue;
-      if (g.layout() != at::kStrided || g.is_neg() || !held(g) || g.sizes() != p.sizes() || g.device().index() != index || g.device().type() != p.device().type() ||
-          (g.scalar_type() != at::kFloat && g.scalar_type() != at::kBFloat16) || !g.is_contiguous()) {
+      if (g.layout() != at::kStrided || g.is_neg() || g.sizes() != p.sizes() || g.device().index() != index || g.device().type() != p.device().type() ||
+          (g.scalar_type() != at::kFloat && g.scalar_type() != at::kBFloat16) || !g.is_contiguous() || !held(g)) {
         flags |= GATHER_ODD;
         continue;
       }

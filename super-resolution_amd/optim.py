@@ -250,7 +250,7 @@ class AdamW:
         where the parameters are views that cover one flat buffer, one flat gradient of the same layout.
         ``grad_scale`` multiplies every gradient first (1 / loss scale).  Returns the gradient norm before clipping
         (0-dim tensor, not synchronised) if ``max_grad_norm`` or ``skip_nonfinite`` is set, else None."""
-        if torch.cuda.current_device() != self.device.index:
+        if torch._C._cuda_getDevice() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.step(grads, grad_scale)
         if not math.isfinite(grad_scale):
@@ -291,7 +291,7 @@ class AdamW:
         if self.max_grad_norm or self.skip_nonfinite:
             norm = torch.empty((), dtype=torch.float32, device=self.device)
             d.norm = norm.data_ptr()
-        L.check(self._lib.srx_adamw_step(C.byref(d), engine.stream_ptr(self.device)), "srx_adamw_step")
+        L.check(self._lib.srx_adamw_step(C.byref(d), torch._C._cuda_getCurrentRawStream(self.device.index)), "srx_adamw_step")
         self._written(self.params, None if d.flat_grad else self._addresses, self._own)
         return norm
 
