@@ -8,6 +8,7 @@
 //
 // libsrx itself stays free of torch: this module is to it what the ctypes binding is, for tensors.
 #include <Python.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -41,10 +42,8 @@ template <typename F> PyObject* guarded(F f) {
     return f();
   } catch (const Refused& r) {
     PyErr_SetString(r.type, r.msg.c_str());
-  } catch (const c10::Error& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {           // torch's own: a Python exception from a hook, out of memory, ... keep their types
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

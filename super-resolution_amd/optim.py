@@ -27,7 +27,7 @@ _DTYPE_ID = {torch.bfloat16: L.BF16, torch.float32: L.F32}
 def _need_held(t: torch.Tensor, what: str) -> None:
     """A storage can be resized under its tensors."""
     end = t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
-    if t.numel() and end * t.element_size() > t.untyped_storage().nbytes():
+    if t.numel() and (not t.data_ptr() or end * t.element_size() > t.untyped_storage().nbytes()):
         raise ValueError(f"{what}: its memory has been freed")
 
 

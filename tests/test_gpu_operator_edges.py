@@ -405,3 +405,41 @@ def test_the_default_rounding_says_what_it_is():
         warnings.simplefilter("error")
         for k in (dict(state_bits=8, rounding="nearest"), dict(state_bits=8, rounding="random"), dict()):
             pkg("optim").AdamW([p], **k)
+
+
+@pytest.mark.parametrize("shape,dim", [((2, 40, 6, 10), 1), ((3, 20, 40), 2)])
+def test_inside_a_checkpoint(shape, dim):
+    """Recomputation ends with an exception of its own inside the call that saves the last tensor."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator().manual_seed(3)
+    c = shape[dim]
+    leaves = [t.to(DEV).requires_grad_() for t in (torch.randn(*shape, generator=g), torch.randn(*shape, generator=g), torch.randn(c, generator=g), torch.randn(c, generator=g))]
+
+    def run(x, f, w2, w1):
+        y, h = R().gated_residual(x, f * 2, post=R().NormSpec("rms", w2), pre=R().NormSpec("layer", w1), channel_dim=dim)
+        return R().channel_norm(y + h, R().NormSpec("rms", w1), dim)
+    want = torch.autograd.grad(run(*leaves).square().sum(), leaves)
+    for reentrant in (False, True):
+        for t in leaves:
+            t.grad = None
+        checkpoint(run, *leaves, use_reentrant=reentrant).square().sum().backward()
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want)), reentrant
+
+
+def test_exceptions_keep_their_types():
+    class Stop(Exception):
+        pass
+
+    def stop(t):
+        raise Stop
+    x = torch.randn(4, 40, device=DEV, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(stop, lambda t: t), pytest.raises(Stop):
+        R().channel_norm(x, R().NormSpec("rms"))
+    wide = torch.zeros(1, 40, device=DEV).expand(1 << 22, 40)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.001)          # of 288 GB: less than the 671 MB of one output
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            R().channel_norm(wide, R().NormSpec("rms"))
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
