@@ -8,9 +8,9 @@
 // The gradients' addresses travel in the kernel arguments: they change from step to step (autograd allocates new
 // gradients), and a table in device memory would need a host-to-device copy that a captured graph could not repeat.
 //
-// Bound: HBM.  702 tensors of 22800 fp32 elements (16.0 M): norm pass 13 us, prepare 4 to 5 us, update 74 us (6.0 TB/s: part
-// of the 448 MB stays in the last-level cache) with 32-bit moments, 51 us with 8-bit ones; whole step with clipping 91 and
-// 66 us.
+// Bound: HBM.  702 tensors of together 16.9 M fp32 elements: norm pass 13 us, prepare 5 us, update 73 us (6.5 TB/s: part
+// of the 474 MB stays in the last-level cache) with 32-bit moments, 50 us (5.4 TB/s) with 8-bit ones rounded to nearest, 62 us
+// rounded at random (the hash and a division for each code).
 #include <type_traits>
 #include "srx_common.h"
 

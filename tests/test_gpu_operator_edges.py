@@ -443,3 +443,17 @@ def test_exceptions_keep_their_types():
             R().channel_norm(wide, R().NormSpec("rms"))
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
+
+
+def test_sigmoid_of_far_gates():
+    """y = sigmoid(q) for q over all that fp32 can hold: the gate's own bound, (1.5 |q| + 6) 2^-24 of the value, and four more
+    roundings of the factors 1 around it; where it leaves the normal numbers, 2^-126."""
+    q = torch.cat([torch.linspace(-87, 87, 40 * 500), torch.linspace(-2000, 2000, 40 * 10)]).view(-1, 40).to(DEV)
+    x, f = torch.zeros_like(q), torch.ones_like(q)
+    want = torch.sigmoid(q.double().cpu())
+    for gate, out in ((q, lambda g: R().gated_residual(x, f, gate=g, gate_act="sigmoid")),
+                      (q, lambda g: R().gated_residual(x[:, :, None].expand(-1, -1, 2), f[:, :, None].expand(-1, -1, 2), gate=g, gate_act="sigmoid")[..., 1])):
+        got = out(gate).double().cpu()
+        allowed = (1.5 * q.double().cpu().abs() + 10) * 2.0 ** -24 * want + 2.0 ** -126
+        worst = float(((got - want).abs() / allowed).max())
+        assert worst <= 1, worst
