@@ -3,6 +3,7 @@
 //   resnorm(...)   residual.py's operator: argument checks, memory order, outputs, the autograd node (its backward pass runs
 //                  without Python), and the calls of libsrx's srx_resnorm_* entry points.
 //   gather(...)    optim.py's lists: addresses and types of hundreds of parameters and gradients in one pass.
+//   unheld(...)    finds a tensor whose storage does not hold it.
 //   written(...)   tells autograd that a step has written those parameters.
 //   bind(...)      the addresses of libsrx's entry points (the library that _lib.py has loaded).
 //
@@ -494,6 +495,18 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   });
 }
 
+// unheld(tensors) -> the first one whose storage does not hold it, or -1
+PyObject* unheld(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  return guarded([&]() -> PyObject* {
+    if (nargs != 1 || !PyList_Check(a[0])) refuse(PyExc_TypeError, "a list expected");
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); ++i) {
+      if (!THPVariable_Check(PyList_GET_ITEM(a[0], i))) refuse(PyExc_TypeError, "element ", i, " is not a tensor");
+      if (!held(THPVariable_Unpack(PyList_GET_ITEM(a[0], i)))) return PyLong_FromSsize_t(i);
+    }
+    return PyLong_FromLong(-1);
+  });
+}
+
 // written(params, addresses or None, others): advances the version counters of the parameters with an address (None: of
 // all) and, if there was one, of the other tensors, as an in-place operation would: a graph that saved one of them then refuses its
 // backward pass.  (Tensors made in inference mode have no counter and cannot be saved.)
@@ -544,6 +557,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {{"resnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(resnorm)), METH_FASTCALL, nullptr},
                          {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gather)), METH_FASTCALL, nullptr},
+                         {"unheld", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(unheld)), METH_FASTCALL, nullptr},
                          {"written", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(written)), METH_FASTCALL, nullptr},
                          {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

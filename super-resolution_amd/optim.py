@@ -24,18 +24,12 @@ _MOVED, _ODD, _BF16 = 1, 2, 4              # flags of the host module's gather()
 _DTYPE_ID = {torch.bfloat16: L.BF16, torch.float32: L.F32}
 
 
-def _need_held(t: torch.Tensor, what: str) -> None:
-    """A storage can be resized under its tensors."""
-    end = t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
-    if t.numel() and (not t.data_ptr() or end * t.element_size() > t.untyped_storage().nbytes()):
-        raise ValueError(f"{what}: its memory has been freed")
-
-
 def _in_memory(t: torch.Tensor, what: str) -> torch.Tensor:
     """t with its values in memory: a negative view and a tensor of zeros without memory are copied (both count as contiguous)."""
     if t._is_zerotensor():
         return t.detach().clone()
-    _need_held(t, what)
+    if L.host().unheld([t]) >= 0:          # a storage can be resized under its tensors
+        raise ValueError(f"{what}: its memory has been freed")
     return t.detach().clone() if t.is_neg() else t
 
 
@@ -208,7 +202,9 @@ class AdamW:
                 raise ValueError(f"AdamW: parameter {i} is not contiguous")
             if p.is_neg():
                 raise ValueError(f"AdamW: parameter {i} is a negative view: its memory holds other values than it")
-            _need_held(p, f"AdamW: parameter {i}")
+        freed = L.host().unheld(self.params)
+        if freed >= 0:
+            raise ValueError(f"AdamW: the memory of parameter {freed} has been freed")
         spans = sorted((a, a + n * p.element_size(), i) for i, (a, n, p) in enumerate(zip(ptrs, self._n, self.params)) if n)
         for (_, end, i), (begin, _, k) in zip(spans, spans[1:]):
             if begin < end:
