@@ -12,6 +12,8 @@ branch, in one pass over the data, forward and backward::
 Tensors: float32 or bfloat16 on a GPU, channels at dim 1 (``[B, C, ...]`` maps, ``channel_dim=1``) or last (tokens,
 ``channel_dim=-1``); at most 1024 channels in maps, 8192 in channels-last tensors.  Memory order is kept: a
 channels-last map gives channels-last results.  Statistics and sums are float32 whatever the type.
+
+The calls are no torch operations: tracing them (``torch.jit.trace``, ``make_fx``) and forward-mode differentiation are refused.
 """
 from __future__ import annotations
 
