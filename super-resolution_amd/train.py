@@ -160,7 +160,7 @@ def _backward_and_step(plan, opt: "FlatAdam") -> bool:
 
 def _make_optimizer(optimizer: Optional[Callable], module, flat: torch.Tensor, lr: float):
     """The optimizer of a trainer: ``optimizer(module)`` — for instance ``lambda m: optim.AdamW(optim.decay_groups(m),
-    lr=2e-4, max_grad_norm=1.0, state_bits=8)`` — or FlatAdam.  It is built after the module's parameters
+    lr=2e-4, max_grad_norm=1.0, state_bits=8, rounding="random")`` — or FlatAdam.  It is built after the module's parameters
     have become views of one flat buffer and before the first step, its ``step`` gets the flat gradient, and
     ``lr`` (``schedule_lr`` where it has one) and ``state_dict`` / ``load_state_dict`` are used as FlatAdam's are."""
     if optimizer is None:
